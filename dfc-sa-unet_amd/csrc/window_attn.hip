@@ -1,0 +1,1084 @@
+// Attention with a sliding window and always-visible first tokens ("sinks"), grouped key heads,
+// forward, backward and over a cache (dfcsa.token_ops.window_attention / window_attention_cached).
+//
+//   O[i] = sum_j P[i][j] V[j],  P[i] = softmax over the visible j of scale * q_i . k_j
+//   key j is visible to the query at position p when j < length, j <= p if causal, and
+//   |p - j| < window or j < sinks.  A query that sees nothing (padding) gives zeros.
+//   backward, with L the log-sum-exp of a row and delta = dO . O:
+//   P = exp(scale q.k - L), dV = P^T dO, dS = P (dO V^T - delta), dQ = scale dS K, dK = scale dS^T Q
+//
+// Work: 4 D flop for each visible pair and head forward, 14 D backward (S and dP are formed twice: a
+// query-major pass owns dQ, a key-major pass owns dK and dV, so there are no float atomics and the
+// results do not depend on the order workgroups run in); only tiles that hold a visible pair are
+// visited, so the cost follows N * (window + sinks), not N^2.
+//
+// Rows.  The G = H / Hk query heads of a key head are packed with the tokens: row r = t * G + g.  A
+// tile of 128 rows then spans 128 / G tokens, so a grouped call reads each key once for its group and
+// visits fewer half-masked tiles at the window's edges.
+//
+// Matrix instructions: 32x32x16 bf16, or 32x32x2 fp32 four at a time (fp32 inputs stay fp32 all the
+// way).  The accumulator of one product is the B operand of the next without moving between lanes:
+// the accumulator's row order (8 g + 4 (lane / 32) + r) is taken as the contraction order, and the A
+// operand is read from LDS in that order -- transposed by ds_read_b64_tr_b16 for bf16.  P and dS are
+// rounded to bf16 for that second product (bf16 inputs only): relative 2^-9 each, averaged over the
+// keys of a row, below the rounding of the outputs themselves.
+//
+// LDS images hold one row per key (or query row) with 16-byte chunks XOR-swizzled by the row, on the
+// source side of an LDS-DMA load: rows are read by 16-byte reads and columns by transposing reads
+// without bank conflicts from the same image.  Rows no query of the workgroup sees load as zeros (the
+// buffer descriptor's bounds check), so what lies in padding is never multiplied.
+#include <algorithm>
+
+#include "common.h"
+#include "dfcsa_internal.h"
+
+namespace {
+
+typedef __bf16 bh8_t __attribute__((ext_vector_type(8)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef short s8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef float f16_t __attribute__((ext_vector_type(16)));
+typedef int i4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4_t lds_s4;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kGrow = 8.0f;   // the running maximum moves only when a row outgrows it by 2^8
+
+struct WArgs {
+  int B, T, M, H, Hk, G, D, R;
+  int window, sinks, causal, cached;
+  float scale, scale2;   // scale2 = scale * log2(e)
+  DivMod dmG;
+  const void *q, *k, *v;
+  int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh;   // bytes
+  const int* lengths;
+  void* o;
+  float* lse;            // [B][Hk][R], log2 of the sum of exp2(scale2 q.k)
+  float* part;           // split results: O [splits][B*Hk*R][D], then lse [splits][B*Hk*R]
+  int splits, tiles;     // row (or key) tiles per (batch, key head)
+  // backward
+  const void *dO;
+  int64_t ob, ot, oh;    // dO strides, bytes
+  float* delta;
+  void *dq, *dk, *dv;
+  int nsink, csink, cwin;   // key tiles with sinks, and row chunks of those and of the other tiles
+};
+
+// ------------------------------------------------------------------ matrix instructions
+template <typename T> struct Mma;
+template <> struct Mma<bf16_t> {
+  typedef s8_t frag;
+  static constexpr int KS = 16;   // contraction depth of one fragment pair
+  __device__ __forceinline__ static f16_t mma(const frag& a, const frag& b, const f16_t& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bh8_t, a), __builtin_bit_cast(bh8_t, b), c, 0, 0, 0);
+  }
+  // accumulator registers of contraction step st (16 rows of the 32) as a fragment
+  __device__ __forceinline__ static frag pack(const f16_t& p, int st) {
+    union { uint32_t u[4]; frag f; } r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.u[i] = pack2bf(p[8 * st + 2 * i], p[8 * st + 2 * i + 1]);
+    return r.f;
+  }
+};
+template <> struct Mma<float> {
+  typedef f4_t frag;
+  static constexpr int KS = 8;
+  __device__ __forceinline__ static f16_t mma(const frag& a, const frag& b, f16_t c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  __device__ __forceinline__ static frag pack(const f16_t& p, int st) {
+    return frag{p[4 * st], p[4 * st + 1], p[4 * st + 2], p[4 * st + 3]};
+  }
+};
+
+// ------------------------------------------------------------------ LDS images
+// DP: head width rounded up to 32; the row pitch is 64 or 128 elements.
+template <typename T, int DP> struct Img {
+  static constexpr int ES = (int)sizeof(T);
+  static constexpr int PITCH = (DP <= 64 ? 64 : 128) * ES;
+  static constexpr int CPR = PITCH / 16;         // 16-byte chunks per row: 8, 16 or 32
+  static constexpr int ROWS = ES == 2 ? 64 : 32; // rows of a tile
+  static constexpr int BYTES = ROWS * PITCH;
+  static constexpr int NS = DP / Mma<T>::KS;     // fragments along the width
+  static constexpr int ND = DP / 32;             // 32-column blocks
+  // XOR of the chunk index: rows r .. r + 3 (one transposing read) and rows r .. r + 15 of one chunk
+  // (one 16-byte read phase) both spread over all banks
+  __device__ __forceinline__ static int swz(int row) {
+    return CPR == 8 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row & 3) << 2 | ((row >> 2) & 3);
+  }
+  __device__ __forceinline__ static const char* at(const char* img, int row, int chunk) {
+    return img + row * PITCH + ((chunk ^ swz(row)) << 4);
+  }
+  typedef typename Mma<T>::frag frag;
+  // fragment st along the width of row `row` (this lane's), columns KS st + (KS/2)(lane/32) ..
+  __device__ __forceinline__ static frag row_frag(const char* img, int row, int st, int lane) {
+    return *(const frag*)at(img, row, 2 * st + (lane >> 5));
+  }
+  // fragment of 32 columns d0 + (lane & 31) over the contraction rows of step st of rows r0 ..
+  __device__ __forceinline__ static frag col_frag(const char* img, int r0, int st, int d0, int lane) {
+    frag f;
+    if constexpr (ES == 2) {
+      const int i = lane & 15, row = r0 + 16 * st + 4 * (lane >> 5) + (i >> 2);
+      const int col = d0 + (lane & 16) + 4 * (i & 3), ch = col >> 3, sub = (col & 4) * 2;
+      const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at(img, row, ch) + sub));
+      const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at(img, row + 8, ch) + sub));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[e] = lo[e];
+        f[4 + e] = hi[e];
+      }
+    } else {
+      const int col = d0 + (lane & 31);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        f[e] = *(const float*)(at(img, r0 + 8 * st + 4 * (lane >> 5) + e, col >> 2) + (col & 3) * 4);
+    }
+    return f;
+  }
+};
+
+// ------------------------------------------------------------------ LDS-DMA
+// One instruction moves 64 x 16 bytes to consecutive LDS addresses.  Written in inline asm so that the
+// compiler does not drain it before the next LDS read; the kernels wait for their DMAs themselves.  An
+// offset past num_records reads zeros.  s_nop: the descriptor may come from a lane read (v_readfirstlane),
+// which needs five wait states before a memory instruction takes it.
+constexpr unsigned kOob = 0x80000000u;
+__device__ __forceinline__ i4_t make_rsrc(const void* base) {
+  const uint64_t p = (uint64_t)base;
+  i4_t r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xffffu));
+  r[2] = 0x7fffffff;
+  r[3] = 0x00020000;
+  return r;
+}
+__device__ __forceinline__ void dma16(const i4_t& rsrc, unsigned voff, const char* lds) {
+  const unsigned dst = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const __attribute__((address_space(3))) char*)lds);
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(voff), "s"(rsrc), "s"(dst)
+      : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// Key-row DMA of one wave: NI instructions of a tile shared by NW waves (NW == 1: the wave's own tile).
+template <typename T, int DP, int ROWS, int NW> struct KeyDma {
+  typedef Img<T, DP> I;
+  static constexpr int NI = ROWS * I::CPR / 64 / NW;
+  int row[NI];
+  unsigned chunk[NI];   // byte offset of the chunk within its row, or out of range
+  __device__ __forceinline__ void init(int wave, int lane, int D) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = (i * NW + wave) * 64 + lane;
+      row[i] = c / I::CPR;
+      const int ch = (c % I::CPR) ^ I::swz(row[i]);
+      chunk[i] = ch * 16 < D * I::ES ? (unsigned)ch * 16 : kOob;
+    }
+  }
+  // rows key0 + row of base; row valid if in [lo, hi) or below sl
+  __device__ __forceinline__ void issue(const char* base, int64_t stride, int key0, int lo, int hi, int sl, char* img,
+                                        int wave) const {
+    const i4_t rs = make_rsrc(base + (int64_t)key0 * stride);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int key = key0 + row[i];
+      const bool ok = (key >= lo && key < hi) || key < sl;
+      const unsigned off = (ok ? 0u : kOob) | (chunk[i] + (unsigned)row[i] * (unsigned)stride);
+      dma16(rs, (chunk[i] & kOob) | off, img + (i * NW + wave) * 1024);
+    }
+  }
+};
+
+// ------------------------------------------------------------------ masks
+struct RowMask {   // of this lane's row: visible(key) = key in [lo, lo + span] or key < sl
+  int lo;
+  unsigned span;
+  int sl;
+  __device__ __forceinline__ bool operator()(int key) const { return (unsigned)(key - lo) <= span || key < sl; }
+};
+struct Seq {       // of the workgroup's sequence
+  int len, off;    // valid keys; position of token 0
+};
+__device__ __forceinline__ Seq seq_of(const WArgs& a, int b) {
+  Seq s;
+  s.len = a.M;
+  if (a.lengths) s.len = min(max(a.lengths[b], 0), a.M);
+  s.off = a.cached ? s.len - a.T : 0;
+  return s;
+}
+__device__ __forceinline__ bool alive(const WArgs& a, const Seq& s, int r, int& p) {
+  p = dm_div(a.dmG, r) + s.off;
+  return r < a.R && p >= 0 && p < s.len;
+}
+__device__ __forceinline__ RowMask row_mask(const WArgs& a, const Seq& s, int r) {
+  int p;
+  RowMask m;
+  m.lo = 0x7fffffff;   // above every key
+  m.span = 0;
+  m.sl = 0;
+  if (alive(a, s, min(r, a.R - 1), p) && r < a.R) {
+    const int hi = a.causal ? p : min(p + a.window - 1, s.len - 1);
+    m.lo = p - a.window + 1;
+    m.span = (unsigned)(hi - m.lo);
+    m.sl = min(a.sinks, a.causal ? p + 1 : s.len);
+  }
+  return m;
+}
+// keys that the rows [r0, r1] see: [lo, hi) and [0, sl); pmin > pmax: none
+struct Span {
+  int pmin, pmax, lo, hi, sl;
+  bool cut;   // some of the rows are padding
+};
+__device__ __forceinline__ Span span_of(const WArgs& a, const Seq& s, int r0, int r1) {
+  Span v;
+  r1 = min(r1, a.R - 1);
+  const int first = dm_div(a.dmG, min(r0, a.R - 1)) + s.off, last = dm_div(a.dmG, r1) + s.off;
+  v.pmin = max(first, 0);
+  v.pmax = min(last, s.len - 1);
+  v.cut = first < 0 || last >= s.len;
+  if (r0 > r1 || v.pmin > v.pmax) {
+    v.pmin = 1;
+    v.pmax = 0;
+    v.lo = v.hi = v.sl = 0;
+    return v;
+  }
+  v.lo = max(v.pmin - a.window + 1, 0);
+  v.hi = a.causal ? v.pmax + 1 : min(v.pmax + a.window, s.len);
+  v.sl = min(a.sinks, a.causal ? v.pmax + 1 : s.len);
+  return v;
+}
+// does every row of the span see every key in [k0, k1)?  is there one that sees one?
+__device__ __forceinline__ bool sees_all(const WArgs& a, const Seq& s, const Span& v, int k0, int k1) {
+  if (v.cut || v.pmin > v.pmax || k1 > s.len || (a.causal && k1 - 1 > v.pmin)) return false;
+  if (k1 <= a.sinks) return true;
+  return v.pmax - k0 < a.window && (a.causal || k1 - 1 - v.pmin < a.window);
+}
+__device__ __forceinline__ bool sees_any(const Span& v, int k0, int k1) {
+  return v.pmin <= v.pmax && ((k0 < v.hi && k1 > v.lo) || k0 < v.sl);
+}
+// the key tiles of a span: sink tiles [0, ns), then window tiles [w0, w1)
+struct TileList {
+  int ns, w0, n;
+  __device__ __forceinline__ int operator[](int i) const { return i < ns ? i : w0 + i - ns; }
+};
+template <int KT> __device__ __forceinline__ TileList tiles_of(const Span& v) {
+  TileList t;
+  t.ns = (v.sl + KT - 1) / KT;
+  t.w0 = max(v.lo / KT, t.ns);
+  t.n = t.ns + max((v.hi + KT - 1) / KT - t.w0, 0);
+  return t;
+}
+
+// ------------------------------------------------------------------ softmax state of 32 rows (one per lane column)
+template <typename T, int DP> struct Online {
+  typedef Img<T, DP> I;
+  typedef typename I::frag frag;
+  float m, l;        // maximum (log2 units, lags by at most kGrow), this half's sum
+  f16_t o[I::ND];    // O^T: column = row of the tile, rows = head columns
+  __device__ __forceinline__ void init() {
+    m = kNegInf;
+    l = 0.f;
+#pragma unroll
+    for (int d = 0; d < I::ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  }
+  // NSUB blocks of 32 keys from key0, at LDS rows k0 ..
+  template <int NSUB, bool MASK>
+  __device__ __forceinline__ void step(const char* kimg, const char* vimg, int row0, int key0, const frag (&q)[I::NS],
+                                       float scale2, const RowMask& mask, int lane) {
+    f16_t s[NSUB];
+    float mx = kNegInf;
+#pragma unroll
+    for (int b = 0; b < NSUB; ++b) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
+#pragma unroll
+      for (int st = 0; st < I::NS; ++st)
+        s[b] = Mma<T>::mma(I::row_frag(kimg, row0 + 32 * b + (lane & 31), st, lane), q[st], s[b]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (MASK && !mask(key0 + 32 * b + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3))) s[b][e] = kNegInf;
+        mx = fmaxf(mx, s[b][e]);
+      }
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scale2;
+    if (__any(mx > m + kGrow || (m == kNegInf && mx > kNegInf))) {
+      const float mn = fmaxf(m, mx);
+      const float al = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < I::ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= al;
+      m = mn;
+    }
+    const float ms = m == kNegInf ? 0.f : m;
+#pragma unroll
+    for (int b = 0; b < NSUB; ++b) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[b][e] = __builtin_amdgcn_exp2f(fmaf(s[b][e], scale2, -ms));
+        l += s[b][e];
+      }
+#pragma unroll
+      for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+        const frag p = Mma<T>::pack(s[b], st);
+#pragma unroll
+        for (int d = 0; d < I::ND; ++d) o[d] = Mma<T>::mma(I::col_frag(vimg, row0 + 32 * b, st, 32 * d, lane), p, o[d]);
+      }
+    }
+  }
+};
+
+// this lane's row of a [token][head] tensor as fragments (rows past the end: zeros)
+template <typename T, int DP>
+__device__ __forceinline__ void load_frags(const char* row, bool ok, int D, int lane,
+                                           typename Mma<T>::frag (&f)[Img<T, DP>::NS]) {
+  constexpr int KS = Mma<T>::KS;
+#pragma unroll
+  for (int st = 0; st < Img<T, DP>::NS; ++st) {
+    const int d = KS * st + KS / 2 * (lane >> 5);
+#pragma unroll
+    for (int e = 0; e < (int)(sizeof(f[0]) / sizeof(f[0][0])); ++e) f[st][e] = 0;
+    if (ok && d < D) f[st] = *(const typename Mma<T>::frag*)(row + d * (int)sizeof(T));
+  }
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
+template <> __device__ __forceinline__ void store4<float>(float* p, float a, float b, float c, float d) {
+  *(float4*)p = make_float4(a, b, c, d);
+}
+template <> __device__ __forceinline__ void store4<bf16_t>(bf16_t* p, float a, float b, float c, float d) {
+  *(uint2*)p = make_uint2(pack2bf(a, b), pack2bf(c, d));
+}
+// column `lane & 31` of an accumulated [head column][row] tile to the row at p
+template <typename T, int ND>
+__device__ __forceinline__ void store_col(T* p, const f16_t (&o)[ND], float f, int D, int lane) {
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * d + 8 * g + 4 * (lane >> 5);
+      if (c < D) store4<T>(p + c, o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
+    }
+}
+
+// Row r's result of (part of) its keys: straight to o and lse, or to the split's partial.
+template <typename T, int DP>
+__device__ __forceinline__ void finish_row(const WArgs& a, int bh, int split, int r, const f16_t (&o)[DP / 32], float m,
+                                           float lsum, int lane) {
+  if (r >= a.R) return;
+  const float inv = lsum > 0.f ? 1.0f / lsum : (lsum == 0.f ? 0.f : lsum);   // NaN sums stay NaN
+  const float lse = lsum == 0.f ? kNegInf : m + __builtin_amdgcn_logf(lsum);
+  const int64_t row = (int64_t)bh * a.R + r, rows = (int64_t)a.B * a.Hk * a.R;
+  if (a.splits == 1) {
+    const int b = bh / a.Hk, hk = bh - b * a.Hk, t = dm_div(a.dmG, r), g = r - t * a.G;
+    T* p = (T*)a.o + (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
+    store_col<T, DP / 32>(p, o, inv, a.D, lane);
+    if (a.lse && lane < 32) a.lse[row] = lse;
+  } else {
+    store_col<float, DP / 32>(a.part + (split * rows + row) * a.D, o, inv, a.D, lane);
+    if (lane < 32) a.part[a.splits * rows * a.D + split * rows + row] = lse;
+  }
+}
+
+// ============================================================================ forward
+// 128 rows per workgroup, 32 per wave; key tiles double-buffered in LDS.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) wattn_fwd_kernel(const WArgs a) {
+  typedef Img<T, DP> I;
+  constexpr int KT = I::ROWS;
+  __shared__ __attribute__((aligned(16))) char smem[4 * I::BYTES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int L = xcd_remap(blockIdx.x, a.tiles * a.B * a.Hk * a.splits);
+  if (L < 0) return;
+  const int split = L % a.splits, tile = (L / a.splits) % a.tiles, bh = L / (a.splits * a.tiles);
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const Seq seq = seq_of(a, b);
+  const int r0 = tile * 128, rw = r0 + wave * 32;
+  const Span wg = span_of(a, seq, r0, r0 + 127), my = span_of(a, seq, rw, rw + 31);
+  const TileList tl = tiles_of<KT>(wg);
+  const int it0 = (int)((int64_t)tl.n * split / a.splits), it1 = (int)((int64_t)tl.n * (split + 1) / a.splits);
+
+  const char* kbase = (const char*)a.k + b * a.kb + hk * a.kh;
+  const char* vbase = (const char*)a.v + b * a.vb + hk * a.vh;
+  KeyDma<T, DP, KT, 4> dma;
+  dma.init(wave, lane, a.D);
+  const int r = rw + (lane & 31);
+  const RowMask mask = row_mask(a, seq, r);
+  typename I::frag q[I::NS];
+  {
+    const int t = dm_div(a.dmG, min(r, a.R - 1)), g = min(r, a.R - 1) - t * a.G;
+    load_frags<T, DP>((const char*)a.q + b * a.qb + t * a.qt + (hk * a.G + g) * a.qh, mask.lo != 0x7fffffff, a.D, lane, q);
+  }
+  Online<T, DP> st;
+  st.init();
+  if (it0 < it1) {
+    dma.issue(kbase, a.kt, tl[it0] * KT, wg.lo, wg.hi, wg.sl, smem, wave);
+    dma.issue(vbase, a.vt, tl[it0] * KT, wg.lo, wg.hi, wg.sl, smem + I::BYTES, wave);
+  }
+  for (int it = it0; it < it1; ++it) {
+    char* cur = smem + ((it - it0) & 1) * 2 * I::BYTES;
+    char* nxt = smem + ((it - it0 + 1) & 1) * 2 * I::BYTES;
+    if (it + 1 < it1) {
+      dma.issue(kbase, a.kt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt, wave);
+      dma.issue(vbase, a.vt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt + I::BYTES, wave);
+      wait_vm<2 * KeyDma<T, DP, KT, 4>::NI>();
+    } else {
+      wait_vm<0>();
+    }
+    lds_barrier();
+    const int key0 = tl[it] * KT;
+    if (sees_any(my, key0, key0 + KT)) {
+      if (sees_all(a, seq, my, key0, key0 + KT))
+        st.template step<KT / 32, false>(cur, cur + I::BYTES, 0, key0, q, a.scale2, mask, lane);
+      else
+        st.template step<KT / 32, true>(cur, cur + I::BYTES, 0, key0, q, a.scale2, mask, lane);
+    }
+    lds_barrier();   // every wave is done with this buffer before it is filled again
+  }
+  const float lsum = st.l + __shfl_xor(st.l, 32, 64);
+  finish_row<T, DP>(a, bh, split, r, st.o, st.m, lsum, lane);
+}
+
+// Few rows (at most 32 per tile): the four waves share the rows and split the keys, each with its own
+// LDS ring of 32-key tiles and no barrier in the loop; joined at the end.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
+  typedef Img<T, DP> I;
+  constexpr int KT = 32, IB = KT * I::PITCH;
+  constexpr int STG = IB <= 8192 ? 2 : 1;   // stages of K and V per wave (wide fp32: one fits)
+  constexpr int RING = STG * 2 * IB;
+  constexpr int OUT = 32 * (DP + 4) * 4;
+  constexpr int PER = RING > OUT ? RING : OUT;
+  __shared__ __attribute__((aligned(16))) char smem[4 * PER];
+  __shared__ float sm_m[4][32], sm_l[4][32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int L = xcd_remap(blockIdx.x, a.tiles * a.B * a.Hk * a.splits);
+  if (L < 0) return;
+  const int split = L % a.splits, tile = (L / a.splits) % a.tiles, bh = L / (a.splits * a.tiles);
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const Seq seq = seq_of(a, b);
+  const int r0 = tile * 32;
+  const Span my = span_of(a, seq, r0, r0 + 31);
+  const TileList tl = tiles_of<KT>(my);
+  const int it0 = (int)((int64_t)tl.n * split / a.splits) + wave, it1 = (int)((int64_t)tl.n * (split + 1) / a.splits);
+
+  const char* kbase = (const char*)a.k + b * a.kb + hk * a.kh;
+  const char* vbase = (const char*)a.v + b * a.vb + hk * a.vh;
+  char* ring = smem + wave * PER;
+  KeyDma<T, DP, KT, 1> dma;
+  dma.init(0, lane, a.D);
+  const int r = r0 + (lane & 31);
+  const RowMask mask = row_mask(a, seq, r);
+  typename I::frag q[I::NS];
+  {
+    const int t = dm_div(a.dmG, min(r, a.R - 1)), g = min(r, a.R - 1) - t * a.G;
+    load_frags<T, DP>((const char*)a.q + b * a.qb + t * a.qt + (hk * a.G + g) * a.qh, mask.lo != 0x7fffffff, a.D, lane, q);
+  }
+  Online<T, DP> st;
+  st.init();
+  if (it0 < it1) {
+    dma.issue(kbase, a.kt, tl[it0] * KT, my.lo, my.hi, my.sl, ring, 0);
+    dma.issue(vbase, a.vt, tl[it0] * KT, my.lo, my.hi, my.sl, ring + IB, 0);
+  }
+  int cur = 0;
+  for (int it = it0; it < it1; it += 4, cur = (cur + 1) % STG) {
+    char* c = ring + cur * 2 * IB;
+    char* n = ring + (cur + 1) % STG * 2 * IB;
+    if (STG == 2 && it + 4 < it1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the reads of the buffer filled next are done
+      dma.issue(kbase, a.kt, tl[it + 4] * KT, my.lo, my.hi, my.sl, n, 0);
+      dma.issue(vbase, a.vt, tl[it + 4] * KT, my.lo, my.hi, my.sl, n + IB, 0);
+      wait_vm<2 * KeyDma<T, DP, KT, 1>::NI>();
+    } else {
+      wait_vm<0>();
+    }
+    const int key0 = tl[it] * KT;
+    if (sees_all(a, seq, my, key0, key0 + KT))
+      st.template step<1, false>(c, c + IB, 0, key0, q, a.scale2, mask, lane);
+    else
+      st.template step<1, true>(c, c + IB, 0, key0, q, a.scale2, mask, lane);
+    if (STG == 1 && it + 4 < it1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      dma.issue(kbase, a.kt, tl[it + 4] * KT, my.lo, my.hi, my.sl, n, 0);
+      dma.issue(vbase, a.vt, tl[it + 4] * KT, my.lo, my.hi, my.sl, n + IB, 0);
+    }
+  }
+  // join: O of wave w at ring w as [row][DP + 4] floats
+  const float lsum = st.l + __shfl_xor(st.l, 32, 64);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  float* mine = (float*)ring + (lane & 31) * (DP + 4);
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *(float4*)(mine + 32 * d + 8 * g + 4 * (lane >> 5)) =
+          make_float4(st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]);
+  if (lane < 32) {
+    sm_m[wave][lane] = st.m;
+    sm_l[wave][lane] = lsum;
+  }
+  __syncthreads();
+  // 8 threads a row, DP / 8 columns each
+  const int row = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (DP / 8), rr = r0 + row;
+  if (rr >= a.R) return;
+  float mm = kNegInf;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm_m[w][row]);
+  float f[4], ls = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = mm == kNegInf ? (sm_l[w][row] == 0.f ? 0.f : sm_l[w][row]) : __builtin_amdgcn_exp2f(sm_m[w][row] - mm);
+    ls += f[w] * sm_l[w][row];
+  }
+  const float inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);
+  const float lse = ls == 0.f ? kNegInf : mm + __builtin_amdgcn_logf(ls);
+  const int64_t orow = (int64_t)bh * a.R + rr, rows = (int64_t)a.B * a.Hk * a.R;
+  const int t = dm_div(a.dmG, rr), g = rr - t * a.G;
+  T* po = (T*)a.o + (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
+  float* pp = a.splits == 1 ? nullptr : a.part + (split * rows + orow) * a.D;
+#pragma unroll
+  for (int c = 0; c < DP / 8; c += 4) {
+    if (c0 + c < a.D) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4 x = *(const float4*)((const float*)(smem + w * PER) + row * (DP + 4) + c0 + c);
+        s[0] += f[w] * x.x;
+        s[1] += f[w] * x.y;
+        s[2] += f[w] * x.z;
+        s[3] += f[w] * x.w;
+      }
+      if (pp) store4<float>(pp + c0 + c, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
+      else store4<T>(po + c0 + c, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
+    }
+  }
+  if ((threadIdx.x & 7) == 0) {
+    if (pp) a.part[a.splits * rows * a.D + split * rows + orow] = lse;
+    else if (a.lse) a.lse[orow] = lse;
+  }
+}
+
+// One row per 32 threads: the splits' results weighted by their sums, in split order.
+template <typename T>
+__global__ void __launch_bounds__(256) wattn_join_kernel(const WArgs a) {
+  const int64_t rows = (int64_t)a.B * a.Hk * a.R, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int c = (threadIdx.x & 31) * 4;
+  const float* lp = a.part + a.splits * rows * a.D + row;
+  float mm = kNegInf;
+  for (int z = 0; z < a.splits; ++z) mm = fmaxf(mm, lp[z * rows]);
+  float s[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
+  for (int z = 0; z < a.splits; ++z) {
+    const float lz = lp[z * rows];
+    const float f = lz == kNegInf ? 0.f : __builtin_amdgcn_exp2f(lz - mm);
+    ls += f;
+    if (c < a.D) {
+      const float4 x = *(const float4*)(a.part + (z * rows + row) * a.D + c);
+      s[0] += f * x.x;
+      s[1] += f * x.y;
+      s[2] += f * x.z;
+      s[3] += f * x.w;
+    }
+  }
+  const float inv = ls == 0.f ? 0.f : 1.0f / ls;
+  const int bh = (int)(row / a.R), r = (int)(row - (int64_t)bh * a.R);
+  const int b = bh / a.Hk, hk = bh - b * a.Hk, t = dm_div(a.dmG, r), g = r - t * a.G;
+  if (c < a.D)
+    store4<T>((T*)a.o + (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D + c, s[0] * inv, s[1] * inv, s[2] * inv,
+              s[3] * inv);
+  if (a.lse && (threadIdx.x & 31) == 0) a.lse[row] = ls == 0.f ? kNegInf : mm + __builtin_amdgcn_logf(ls);
+}
+
+// ============================================================================ backward: dQ
+// As the forward, with S and dP per key tile; also writes delta = dO . O for the key-major pass.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) wattn_dq_kernel(const WArgs a) {
+  typedef Img<T, DP> I;
+  typedef typename I::frag frag;
+  constexpr int KT = I::ROWS;
+  __shared__ __attribute__((aligned(16))) char smem[4 * I::BYTES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int L = xcd_remap(blockIdx.x, a.tiles * a.B * a.Hk);
+  if (L < 0) return;
+  const int tile = L % a.tiles, bh = L / a.tiles;
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const Seq seq = seq_of(a, b);
+  const int r0 = tile * 128, rw = r0 + wave * 32;
+  const Span wg = span_of(a, seq, r0, r0 + 127), my = span_of(a, seq, rw, rw + 31);
+  const TileList tl = tiles_of<KT>(wg);
+
+  const char* kbase = (const char*)a.k + b * a.kb + hk * a.kh;
+  const char* vbase = (const char*)a.v + b * a.vb + hk * a.vh;
+  KeyDma<T, DP, KT, 4> dma;
+  dma.init(wave, lane, a.D);
+  const int r = rw + (lane & 31);
+  const RowMask mask = row_mask(a, seq, r);
+  const bool live = mask.lo != 0x7fffffff;
+  const int t = dm_div(a.dmG, min(r, a.R - 1)), g = min(r, a.R - 1) - t * a.G;
+  const int64_t orow = (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
+  frag q[I::NS], dof[I::NS];
+  load_frags<T, DP>((const char*)a.q + b * a.qb + t * a.qt + (hk * a.G + g) * a.qh, live, a.D, lane, q);
+  load_frags<T, DP>((const char*)a.dO + b * a.ob + t * a.ot + (hk * a.G + g) * a.oh, live, a.D, lane, dof);
+  float dl = 0.f, lse = 0.f;
+  {
+    frag of[I::NS];
+    load_frags<T, DP>((const char*)((const T*)a.o + orow), live, a.D, lane, of);
+    constexpr int NE = sizeof(frag) / sizeof(T);
+#pragma unroll
+    for (int st = 0; st < I::NS; ++st)
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        if constexpr (sizeof(T) == 2) dl += bf2f((bf16_t)of[st][e]) * bf2f((bf16_t)dof[st][e]);
+        else dl += of[st][e] * dof[st][e];
+      }
+    dl += __shfl_xor(dl, 32, 64);
+    const int64_t row = (int64_t)bh * a.R + r;
+    if (live) lse = a.lse[row];
+    if (r < a.R && lane < 32) a.delta[row] = dl;
+  }
+  f16_t dq[I::ND];
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
+  if (tl.n > 0) {
+    dma.issue(kbase, a.kt, tl[0] * KT, wg.lo, wg.hi, wg.sl, smem, wave);
+    dma.issue(vbase, a.vt, tl[0] * KT, wg.lo, wg.hi, wg.sl, smem + I::BYTES, wave);
+  }
+  for (int it = 0; it < tl.n; ++it) {
+    char* cur = smem + (it & 1) * 2 * I::BYTES;
+    char* nxt = smem + ((it + 1) & 1) * 2 * I::BYTES;
+    if (it + 1 < tl.n) {
+      dma.issue(kbase, a.kt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt, wave);
+      dma.issue(vbase, a.vt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt + I::BYTES, wave);
+      wait_vm<2 * KeyDma<T, DP, KT, 4>::NI>();
+    } else {
+      wait_vm<0>();
+    }
+    lds_barrier();
+    const int key0 = tl[it] * KT;
+    if (sees_any(my, key0, key0 + KT)) {
+      const bool all = sees_all(a, seq, my, key0, key0 + KT);
+#pragma unroll
+      for (int kb = 0; kb < KT / 32; ++kb) {
+        f16_t s, dp;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < I::NS; ++st) {
+          s = Mma<T>::mma(I::row_frag(cur, 32 * kb + (lane & 31), st, lane), q[st], s);
+          dp = Mma<T>::mma(I::row_frag(cur + I::BYTES, 32 * kb + (lane & 31), st, lane), dof[st], dp);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse));
+          if (!all && !mask(key0 + 32 * kb + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3))) {
+            p = 0.f;
+            dp[e] = 0.f;
+          }
+          s[e] = p * (dp[e] - dl);
+        }
+#pragma unroll
+        for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+          const frag ds = Mma<T>::pack(s, st);
+#pragma unroll
+          for (int d = 0; d < I::ND; ++d) dq[d] = Mma<T>::mma(I::col_frag(cur, 32 * kb, st, 32 * d, lane), ds, dq[d]);
+        }
+      }
+    }
+    lds_barrier();
+  }
+  if (r < a.R) store_col<T, I::ND>((T*)a.dq + orow, dq, a.scale, a.D, lane);
+}
+
+// ============================================================================ backward: dK, dV
+// 128 keys per workgroup, 32 per wave (lane column = key); row tiles of Q and dO double-buffered in
+// LDS.  A key tile that holds sinks is seen by every later row: its rows are split over csink
+// workgroups (cwin for the others), whose fp32 parts wattn_dkv_join adds in order.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, 1) wattn_dkv_kernel(const WArgs a) {
+  typedef Img<T, DP> I;
+  typedef typename I::frag frag;
+  constexpr int RT = I::ROWS;
+  constexpr int NI = RT * I::CPR / 64 / 4;
+  __shared__ __attribute__((aligned(16))) char smem[4 * I::BYTES];
+  __shared__ __attribute__((aligned(16))) float s_l[2][RT], s_d[2][RT];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int items = a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin;
+  const int L = xcd_remap(blockIdx.x, items * a.B * a.Hk);
+  if (L < 0) return;
+  const int item = L % items, bh = L / items;
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const bool sink = item < a.nsink * a.csink;
+  const int nch = sink ? a.csink : a.cwin;
+  const int kt = sink ? item / a.csink : a.nsink + (item - a.nsink * a.csink) / a.cwin;
+  const int ch = sink ? item % a.csink : (item - a.nsink * a.csink) % a.cwin;
+  const Seq seq = seq_of(a, b);
+  const int k0 = kt * 128, k1 = min(k0 + 128, seq.len);
+
+  // rows that see one of the keys: positions [p0, p1]
+  int p0 = a.causal ? k0 : max(k0 - a.window + 1, 0), p1 = min(k1 - 1 + a.window - 1, seq.len - 1);
+  if (k0 < a.sinks) {
+    if (!a.causal) p0 = 0;
+    p1 = seq.len - 1;
+  }
+  int i0 = 0, i1 = 0;   // row tiles
+  const int rbeg = p0 * a.G, rend = (p1 + 1) * a.G;
+  if (k0 < k1 && p0 <= p1) {
+    i0 = rbeg / RT;
+    i1 = (rend + RT - 1) / RT;
+  }
+  const int n = i1 - i0;
+  const int c0 = i0 + (int)((int64_t)n * ch / nch), c1 = i0 + (int)((int64_t)n * (ch + 1) / nch);
+
+  const int kw = k0 + wave * 32, key = kw + (lane & 31);
+  const bool kok = key < seq.len;
+  frag kf[I::NS], vf[I::NS];
+  {
+    const int kk = min(key, a.M - 1);
+    load_frags<T, DP>((const char*)a.k + b * a.kb + (int64_t)kk * a.kt + hk * a.kh, kok, a.D, lane, kf);
+    load_frags<T, DP>((const char*)a.v + b * a.vb + (int64_t)kk * a.vt + hk * a.vh, kok, a.D, lane, vf);
+  }
+  // rows that see this lane's key: [vlo, vhi)
+  int vlo = 0x7fffffff, vhi = 0;
+  if (kok) {
+    vlo = a.causal ? key * a.G : max(key - a.window + 1, 0) * a.G;
+    vhi = (key + a.window) * a.G;
+    if (key < a.sinks) {
+      vhi = 0x7fffffff;
+      if (!a.causal) vlo = 0;
+    }
+  }
+  // rows that see all, or any, of the wave's keys
+  const int klast = kw + 31;
+  int alo = a.causal ? klast * a.G : max(klast - a.window + 1, 0) * a.G, ahi = (kw + a.window) * a.G;
+  int nlo = a.causal ? kw * a.G : max(kw - a.window + 1, 0) * a.G, nhi = (klast + a.window) * a.G;
+  if (klast < a.sinks) {
+    ahi = 0x7fffffff;
+    if (!a.causal) alo = 0;
+  }
+  if (kw < a.sinks) {
+    nhi = 0x7fffffff;
+    if (!a.causal) nlo = 0;
+  }
+  if (klast >= seq.len) alo = 0x7fffffff;
+  if (kw >= seq.len) nhi = 0;
+
+  int drow[NI];
+  unsigned dch[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = (i * 4 + wave) * 64 + lane;
+    drow[i] = c / I::CPR;
+    const int cc = (c % I::CPR) ^ I::swz(drow[i]);
+    dch[i] = cc * 16 < a.D * I::ES ? (unsigned)cc * 16 : kOob;
+  }
+  const char* qbase = (const char*)a.q + b * a.qb + hk * a.G * a.qh;
+  const char* obase = (const char*)a.dO + b * a.ob + hk * a.G * a.oh;
+  const int rlim = min(seq.len * a.G, a.R);   // live rows
+  auto issue = [&](int tile, char* img) {
+    const int r0 = tile * RT, t0 = dm_div(a.dmG, r0);
+    const i4_t rq = make_rsrc(qbase + t0 * a.qt), ro = make_rsrc(obase + t0 * a.ot);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = r0 + drow[i], t = dm_div(a.dmG, r), g = r - t * a.G;
+      const unsigned bad = (r < rlim ? 0u : kOob) | (dch[i] & kOob);
+      dma16(rq, bad | (dch[i] + (unsigned)((t - t0) * (int)a.qt + g * (int)a.qh)), img + (i * 4 + wave) * 1024);
+      dma16(ro, bad | (dch[i] + (unsigned)((t - t0) * (int)a.ot + g * (int)a.oh)), img + I::BYTES + (i * 4 + wave) * 1024);
+    }
+  };
+  const float* lbase = a.lse + (int64_t)bh * a.R;
+  const float* dbase = a.delta + (int64_t)bh * a.R;
+  auto stat = [&](int tile) {   // threads [0, RT): lse, [64, 64 + RT): delta
+    const int i = threadIdx.x & 63, r = tile * RT + i;
+    if (i >= RT || wave > 1) return 0.f;
+    if (wave == 0) return r < rlim ? lbase[r] : __builtin_inff();   // exp2(. - inf) = 0
+    return r < rlim ? dbase[r] : 0.f;
+  };
+  auto put = [&](float v, int buf) {
+    const int i = threadIdx.x & 63;
+    if (i < RT && wave == 0) s_l[buf][i] = v;
+    if (i < RT && wave == 1) s_d[buf][i] = v;
+  };
+  f16_t dk[I::ND], dv[I::ND];
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+
+  if (c0 < c1) {
+    put(stat(c0), 0);
+    issue(c0, smem);
+  }
+  for (int it = c0; it < c1; ++it) {
+    const int buf = (it - c0) & 1;
+    char* cur = smem + buf * 2 * I::BYTES;
+    float nx = 0.f;
+    const bool more = it + 1 < c1;
+    if (more) {
+      nx = stat(it + 1);
+      issue(it + 1, smem + (buf ^ 1) * 2 * I::BYTES);
+      wait_vm<2 * NI>();   // all but the DMAs just issued
+    } else {
+      wait_vm<0>();
+    }
+    lds_barrier();
+    const int r0 = it * RT;
+    if (r0 < nhi && r0 + RT > nlo) {
+      const bool all = r0 >= alo && r0 + RT <= ahi;
+#pragma unroll
+      for (int rb = 0; rb < RT / 32; ++rb) {
+        f16_t s, dp;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < I::NS; ++st) {
+          s = Mma<T>::mma(I::row_frag(cur, 32 * rb + (lane & 31), st, lane), kf[st], s);
+          dp = Mma<T>::mma(I::row_frag(cur + I::BYTES, 32 * rb + (lane & 31), st, lane), vf[st], dp);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int rr = 32 * rb + 8 * g + 4 * (lane >> 5);
+          const f4_t l4 = *(const f4_t*)&s_l[buf][rr], d4 = *(const f4_t*)&s_d[buf][rr];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = r0 + rr + e;
+            float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale2, -l4[e]));
+            float dd = dp[4 * g + e] - d4[e];
+            if (!all && (r < vlo || r >= vhi)) p = dd = 0.f;
+            s[4 * g + e] = p;
+            dp[4 * g + e] = p * dd;
+          }
+        }
+#pragma unroll
+        for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+          const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
+#pragma unroll
+          for (int d = 0; d < I::ND; ++d) {
+            dv[d] = Mma<T>::mma(I::col_frag(cur + I::BYTES, 32 * rb, st, 32 * d, lane), pf, dv[d]);
+            dk[d] = Mma<T>::mma(I::col_frag(cur, 32 * rb, st, 32 * d, lane), df, dk[d]);
+          }
+        }
+      }
+    }
+    if (more) put(nx, buf ^ 1);
+    lds_barrier();
+  }
+  if (key >= a.M) return;
+  if (nch == 1) {
+    const int64_t o = (((int64_t)b * a.M + key) * a.Hk + hk) * a.D;
+    store_col<T, I::ND>((T*)a.dk + o, dk, a.scale, a.D, lane);
+    store_col<T, I::ND>((T*)a.dv + o, dv, 1.f, a.D, lane);
+  } else {
+    float* p = a.part + (((int64_t)bh * items + item) * 128 + wave * 32 + (lane & 31)) * 2 * a.D;
+    store_col<float, I::ND>(p, dk, a.scale, a.D, lane);
+    store_col<float, I::ND>(p + a.D, dv, 1.f, a.D, lane);
+  }
+}
+
+// dK and dV of the key tiles whose rows were split: their chunks added in order.  One 4-column piece
+// of dK or dV per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) wattn_dkv_join_kernel(const WArgs a, int tile0, int ntile) {
+  const int q = 2 * a.D / 4;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (int64_t)ntile * 128 * q;
+  if (e >= per * a.B * a.Hk) return;
+  const int bh = (int)(e / per);
+  const int rem = (int)(e - bh * per), c = rem % q * 4, kl = rem / q % 128, kt = tile0 + rem / q / 128;
+  const int key = kt * 128 + kl;
+  if (key >= a.M) return;
+  const bool sink = kt < a.nsink;
+  const int nch = sink ? a.csink : a.cwin, items = a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin;
+  const int item = sink ? kt * a.csink : a.nsink * a.csink + (kt - a.nsink) * a.cwin;
+  const float* p = a.part + (((int64_t)bh * items + item) * 128 + kl) * 2 * a.D + c;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < nch; ++i) {
+    const float4 x = *(const float4*)(p + (int64_t)i * 128 * 2 * a.D);
+    s[0] += x.x;
+    s[1] += x.y;
+    s[2] += x.z;
+    s[3] += x.w;
+  }
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  T* dst = (T*)(c < a.D ? a.dk : a.dv) + (((int64_t)b * a.M + key) * a.Hk + hk) * a.D + (c < a.D ? c : c - a.D);
+  store4<T>(dst, s[0], s[1], s[2], s[3]);
+}
+
+// ============================================================================ host
+constexpr int kWgs = 512;   // workgroups that fill the card: two per CU
+
+bool fill(const dfcsa_wattn_desc* d, WArgs& a, bool backward) {
+  if (!d || (d->dtype != DFCSA_DT_F32 && d->dtype != DFCSA_DT_BF16)) return false;
+  if (d->B <= 0 || d->T <= 0 || d->M <= 0 || d->H <= 0 || d->Hk <= 0 || d->H > 65536 || d->H % d->Hk || d->D < 8 || d->D % 8 ||
+      d->D > 128 || d->window < 1 || d->sinks < 0 || !(d->scale > 0.f) || !d->q || !d->k || !d->v || !d->o)
+    return false;
+  if (!d->cached && d->T != d->M) return false;
+  if (d->cached && (!d->lengths || backward || !d->causal)) return false;
+  a.B = d->B; a.T = d->T; a.M = d->M; a.H = d->H; a.Hk = d->Hk; a.G = d->H / d->Hk; a.D = d->D;
+  const int64_t R = (int64_t)d->T * a.G;
+  // row and key arithmetic is 32 bits wide, up to (M + window) * G
+  if (R > (1 << 29) || (int64_t)d->M * a.G > (1 << 29) || (int64_t)d->B * d->Hk > (1 << 24)) return false;
+  a.R = (int)R;
+  a.window = std::min(d->window, d->M);   // a window of M keys hides nothing
+  a.sinks = std::min(d->sinks, d->M);
+  a.causal = d->causal != 0;
+  a.cached = d->cached != 0;
+  a.scale = d->scale;
+  a.scale2 = d->scale * kLog2e;
+  a.dmG = make_divmod(a.G);
+  const int es = d->dtype == DFCSA_DT_F32 ? 4 : 2;
+  const void* ptr[4] = {d->q, d->k, d->v, backward ? d->dout : nullptr};
+  const int64_t* str[4] = {d->q_stride, d->k_stride, d->v_stride, d->dout_stride};
+  for (int i = 0; i < (backward ? 4 : 3); ++i) {
+    if (!ptr[i] || (uintptr_t)ptr[i] % 16) return false;
+    for (int j = 0; j < 3; ++j)
+      if (str[i][j] < 0 || (str[i][j] * es) % 16) return false;
+    // offsets within one tile are 32 bits wide
+    if (str[i][1] * es >= (1 << 23) || str[i][2] * es * a.G >= (1 << 29)) return false;
+  }
+  a.q = d->q; a.k = d->k; a.v = d->v;
+  a.qb = d->q_stride[0] * es; a.qt = d->q_stride[1] * es; a.qh = d->q_stride[2] * es;
+  a.kb = d->k_stride[0] * es; a.kt = d->k_stride[1] * es; a.kh = d->k_stride[2] * es;
+  a.vb = d->v_stride[0] * es; a.vt = d->v_stride[1] * es; a.vh = d->v_stride[2] * es;
+  a.lengths = d->lengths;
+  a.o = d->o;
+  a.lse = d->lse;
+  a.part = d->work;
+  a.splits = 1;
+  a.dO = d->dout; a.ob = a.ot = a.oh = 0;
+  a.delta = d->delta;
+  a.dq = d->dq; a.dk = d->dk; a.dv = d->dv;
+  a.nsink = a.csink = a.cwin = a.tiles = 0;
+  if (backward) {
+    a.ob = d->dout_stride[0] * es; a.ot = d->dout_stride[1] * es; a.oh = d->dout_stride[2] * es;
+    if (!d->lse || !d->delta || !d->dq || !d->dk || !d->dv) return false;
+  }
+  return true;
+}
+
+// The forward's plan: few = the kernel whose waves split the keys of 32 rows; splits over the keys
+// where the row tiles alone do not fill the card.
+void plan_fwd(WArgs& a, bool& few) {
+  const int bh = a.B * a.Hk;
+  few = a.R <= 64;
+  a.tiles = few ? (a.R + 31) / 32 : (a.R + 127) / 128;
+  const int64_t base = (int64_t)a.tiles * bh;
+  // keys a row tile can see, whatever the lengths are
+  const int64_t tok = std::min<int64_t>(((few ? 32 : 128) + a.G - 1) / a.G + 1, a.T);
+  const int64_t span = std::min<int64_t>(a.M, (int64_t)a.window * (a.causal ? 1 : 2) + tok + a.sinks);
+  const int64_t step = few ? 128 : 64;   // keys of one round of the waves
+  int64_t s = (kWgs + base - 1) / base;
+  s = std::min(s, (span + step - 1) / step);
+  if (base * 2 > kWgs) s = 1;
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+}
+int64_t fwd_work(const WArgs& a) { return a.splits == 1 ? 0 : (int64_t)a.splits * a.B * a.Hk * a.R * (a.D + 1); }
+
+// The backward's key tiles, and the row chunks of those that many rows see: chunks of about the rows
+// that an ordinary tile has, more where the tiles alone do not fill the card.
+void plan_bwd(WArgs& a) {
+  a.tiles = (a.M + 127) / 128;
+  a.nsink = (a.sinks + 127) / 128;
+  const int bh = a.B * a.Hk;
+  const int rt = 32;
+  const int64_t win = std::min<int64_t>(a.M, (int64_t)a.window * (a.causal ? 1 : 2) + 127) * a.G;
+  const int64_t all = (int64_t)a.M * a.G;
+  const int64_t want = std::max<int64_t>(1, 256 / std::max(1, a.tiles * bh));
+  a.cwin = (int)std::max<int64_t>(1, std::min(want, win / (4 * rt)));
+  const int64_t rows = std::max<int64_t>(win / a.cwin, 4 * rt);
+  a.csink = (int)std::max<int64_t>(1, std::min<int64_t>((all + rows - 1) / rows, 256));
+}
+int64_t bwd_work(const WArgs& a) {
+  if (a.csink == 1 && a.cwin == 1) return 0;
+  return (int64_t)(a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin) * a.B * a.Hk * 128 * 2 * a.D;
+}
+
+#define BY_WIDTH(KERNEL, GRID, ...)                                                                      \
+  do {                                                                                                   \
+    if (a.D <= 32) hipLaunchKernelGGL((KERNEL<T, 32>), GRID, dim3(256), 0, st, __VA_ARGS__);             \
+    else if (a.D <= 64) hipLaunchKernelGGL((KERNEL<T, 64>), GRID, dim3(256), 0, st, __VA_ARGS__);        \
+    else if (a.D <= 96) hipLaunchKernelGGL((KERNEL<T, 96>), GRID, dim3(256), 0, st, __VA_ARGS__);        \
+    else hipLaunchKernelGGL((KERNEL<T, 128>), GRID, dim3(256), 0, st, __VA_ARGS__);                      \
+  } while (0)
+
+template <typename T>
+int run_fwd(const WArgs& a, bool few, hipStream_t st) {
+  const dim3 grid((unsigned)xcd_pad(a.tiles * a.B * a.Hk * a.splits));
+  if (few) BY_WIDTH(wattn_few_kernel, grid, a);
+  else BY_WIDTH(wattn_fwd_kernel, grid, a);
+  DFCSA_CHECK_LAUNCH();
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)a.B * a.Hk * a.R;
+    hipLaunchKernelGGL((wattn_join_kernel<T>), dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a);
+    DFCSA_CHECK_LAUNCH();
+  }
+  return 0;
+}
+template <typename T>
+int run_bwd(WArgs a, hipStream_t st) {
+  WArgs q = a;
+  q.tiles = (a.R + 127) / 128;
+  {
+    const WArgs& a = q;
+    BY_WIDTH(wattn_dq_kernel, dim3((unsigned)xcd_pad(a.tiles * a.B * a.Hk)), a);
+  }
+  DFCSA_CHECK_LAUNCH();
+  const int items = a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin;
+  BY_WIDTH(wattn_dkv_kernel, dim3((unsigned)xcd_pad(items * a.B * a.Hk)), a);
+  DFCSA_CHECK_LAUNCH();
+  const int t0 = a.csink > 1 ? 0 : a.nsink, t1 = a.cwin > 1 ? a.tiles : a.nsink;
+  if (t1 > t0) {
+    const int64_t e = (int64_t)(t1 - t0) * 128 * (2 * a.D / 4) * a.B * a.Hk;
+    hipLaunchKernelGGL((wattn_dkv_join_kernel<T>), dim3((unsigned)((e + 255) / 256)), dim3(256), 0, st, a, t0, t1 - t0);
+    DFCSA_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dfcsa_wattn_work_floats(const dfcsa_wattn_desc* d, int backward, int64_t* floats) {
+  WArgs a;
+  if (!floats || !fill(d, a, backward != 0)) return DFCSA_EINVAL;
+  if (backward) {
+    plan_bwd(a);
+    *floats = bwd_work(a);
+  } else {
+    bool few;
+    plan_fwd(a, few);
+    *floats = fwd_work(a);
+  }
+  return 0;
+}
+
+int dfcsa_wattn_fwd(const dfcsa_wattn_desc* d, void* stream) {
+  WArgs a;
+  if (!fill(d, a, false)) return DFCSA_EINVAL;
+  bool few;
+  plan_fwd(a, few);
+  if ((int64_t)a.tiles * a.B * a.Hk * a.splits > 0x7ffffff0) return DFCSA_EINVAL;
+  if (fwd_work(a) > 0 && (!d->work || d->work_floats < fwd_work(a))) return DFCSA_EINVAL;
+  return d->dtype == DFCSA_DT_F32 ? run_fwd<float>(a, few, (hipStream_t)stream) : run_fwd<bf16_t>(a, few, (hipStream_t)stream);
+}
+
+int dfcsa_wattn_bwd(const dfcsa_wattn_desc* d, void* stream) {
+  WArgs a;
+  if (!fill(d, a, true)) return DFCSA_EINVAL;
+  plan_bwd(a);
+  if ((int64_t)(a.nsink * a.csink + a.tiles * a.cwin) * a.B * a.Hk > 0x7ffffff0) return DFCSA_EINVAL;
+  if (bwd_work(a) > 0 && (!d->work || d->work_floats < bwd_work(a))) return DFCSA_EINVAL;
+  return d->dtype == DFCSA_DT_F32 ? run_bwd<float>(a, (hipStream_t)stream) : run_bwd<bf16_t>(a, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -119,6 +119,28 @@ class AugDesc(ctypes.Structure):
                 ("rotate", ctypes.c_int), ("flip", ctypes.c_int), ("mask_w", ctypes.c_int), ("pad", ctypes.c_int)]
 
 
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("B", ctypes.c_int), ("N", ctypes.c_int), ("D", ctypes.c_int),
+                ("npairs", ctypes.c_int), ("naxes", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("inverse", ctypes.c_int), ("heads", ctypes.c_int * 2), ("src", ctypes.c_void_p * 2),
+                ("dst", ctypes.c_void_p * 2), ("src_sb", ctypes.c_int64 * 2), ("src_sn", ctypes.c_int64 * 2),
+                ("src_sh", ctypes.c_int64 * 2), ("positions", ctypes.c_void_p), ("pos_sb", ctypes.c_int64),
+                ("pos_sn", ctypes.c_int64), ("pos_sa", ctypes.c_int64), ("turns", ctypes.c_void_p),
+                ("axis", ctypes.c_void_p), ("pos64", ctypes.c_int)]
+
+
+class WattnDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("B", ctypes.c_int), ("T", ctypes.c_int), ("M", ctypes.c_int),
+                ("H", ctypes.c_int), ("Hk", ctypes.c_int), ("D", ctypes.c_int), ("window", ctypes.c_int),
+                ("sinks", ctypes.c_int), ("causal", ctypes.c_int), ("cached", ctypes.c_int),
+                ("scale", ctypes.c_float), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+                ("lengths", ctypes.c_void_p), ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("work", ctypes.c_void_p), ("work_floats", ctypes.c_int64), ("dout", ctypes.c_void_p),
+                ("dout_stride", ctypes.c_int64 * 3), ("delta", ctypes.c_void_p), ("dq", ctypes.c_void_p),
+                ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(

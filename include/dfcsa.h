@@ -925,6 +925,84 @@ int dfcsa_prof_read(int kernel_class, double* total_ms, int64_t* launches, doubl
 int dfcsa_set_tuning(int knob, int value);
 int dfcsa_get_tuning(int knob);
 
+/* ------------------------------------------------------------------------------------------
+ * Token operators of a transformer block (dfcsa/token_ops.py).  They stand beside the LayerNorm,
+ * position-embedding and attention entry points above; the reference has no counterpart.
+ *
+ * RMS norm with the residual's addition: r = x + res in the stream's type, y = r * rstd * w with
+ * rstd = (mean_C r^2 + eps)^(-1/2).  (dtype, rdtype) of (x, y) and (res, r): (bf16, bf16), (bf16, f32)
+ * or (f32, f32); rows x C contiguous, C % 8 == 0, C <= 16384; w [C] and rstd [rows] fp32 (rstd may be
+ * NULL where no backward follows).
+ * fwd_q8: y8 = y / scale in e4m3 (nearest, ties to even), scales [rows][C / group], scale =
+ *   max(max |y| over the group, 1e-12) / 448; group 0 = the whole row, or 32, 64, 128 dividing C.
+ * bwd: d = rstd (u - xh mean(u xh)) + dr, u = dy w, xh = r rstd; dx (dtype), dres (rdtype) = d (each
+ *   may be NULL), dw [C] = sum over rows of dy xh (NULL: not formed).  dr may be NULL (zero).
+ *   work: dfcsa_rms_bwd_work_floats(rows, C) floats where dw is formed (fixed-order sums).
+ * dequant_q8: out (dtype) = y8 * scale. */
+int dfcsa_rms_fwd(int dtype, int rdtype, int rows, int C, const void* x, const void* res, const float* w, float eps,
+                  void* y, void* r, float* rstd, void* stream);
+int dfcsa_rms_fwd_q8(int dtype, int rdtype, int rows, int C, int group, const void* x, const void* res,
+                     const float* w, float eps, void* y8, float* scales, void* r, void* stream);
+int64_t dfcsa_rms_bwd_work_floats(int rows, int C);
+int dfcsa_rms_bwd(int dtype, int rdtype, int rows, int C, const void* dy, const void* dr, const void* r,
+                  const float* rstd, const float* w, void* dx, void* dres, float* dw, float* work,
+                  int64_t work_floats, void* stream);
+int dfcsa_dequant_q8(int dtype, int64_t rows, int C, int group, const void* y8, const float* scales, void* out,
+                     void* stream);
+/* Rotary positions with up to four axes: pair j of each head's channels -- (j, npairs + j), or
+ * (2j, 2j + 1) if interleaved -- turns by positions[axis[j]] * turns[j] full turns (inverse != 0:
+ * back, the gradient); channels from 2 npairs on are copied.  src/dst: two tensors (q and k; heads 0 =
+ * none) [B][N][heads][D], strides of src in elements (batch, token, head), channels contiguous, dst
+ * contiguous.  positions: int32 (pos64 == 0) or int64 on the device, strides in elements.  turns (in
+ * full turns per position) and axis are host arrays, read before the call returns. */
+#define DFCSA_ROTARY_MAX_PAIRS 256
+typedef struct {
+  int dtype, B, N, D, npairs, naxes, interleaved, inverse;
+  int heads[2];
+  const void* src[2];
+  void* dst[2];
+  int64_t src_sb[2], src_sn[2], src_sh[2];
+  const void* positions;
+  int64_t pos_sb, pos_sn, pos_sa;
+  const double* turns;
+  const unsigned char* axis;
+  int pos64;
+} dfcsa_rotary_desc;
+int dfcsa_rotary(const dfcsa_rotary_desc* d, void* stream);
+/* Attention with a sliding window and always-visible first tokens.  Key j is visible to the query at
+ * position p when j < length, j <= p (causal), and |p - j| < window or j < sinks; o = softmax over the
+ * visible keys of scale q.k, times v; zeros where nothing is visible.
+ * q, o [B][T][H][D], k, v [B][M][Hk][D] (H % Hk == 0, D % 8 == 0, D <= 128); strides in elements
+ * (batch, token, head) of q, k, v, dout: non-negative multiples of 16 bytes, token stride below 8 MiB,
+ * head stride times H / Hk below 512 MiB;
+ * o, dq, dk, dv contiguous.  lengths [B] int32 on the device (NULL: M; clamped to [0, M]).
+ * cached == 0: T == M, token t is at position t.  cached != 0 (causal, lengths required, forward
+ * only): token t is at position length - T + t.
+ * lse [B][Hk][T * H / Hk]: log2 of the rows' sums, written by fwd (may be NULL there), read by bwd;
+ * delta: scratch of the same size.  work: dfcsa_wattn_work_floats floats (0: may be NULL). */
+typedef struct {
+  int dtype, B, T, M, H, Hk, D, window, sinks, causal, cached;
+  float scale;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const int* lengths;
+  void* o;
+  float* lse;
+  float* work;
+  int64_t work_floats;
+  const void* dout;
+  int64_t dout_stride[3];
+  float* delta;
+  void* dq;
+  void* dk;
+  void* dv;
+} dfcsa_wattn_desc;
+int dfcsa_wattn_work_floats(const dfcsa_wattn_desc* d, int backward, int64_t* floats);
+int dfcsa_wattn_fwd(const dfcsa_wattn_desc* d, void* stream);
+int dfcsa_wattn_bwd(const dfcsa_wattn_desc* d, void* stream);
+
 const char* dfcsa_version(void);
 
 #ifdef __cplusplus

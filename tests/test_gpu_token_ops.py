@@ -1,0 +1,674 @@
+"""dfcsa.token_ops on the MI355X against plain 64-bit implementations.
+
+Tolerances are bounds on the rounding errors of the computed formulas: UT, half a step of the stored type
+(bf16 2^-8, fp32 2^-24); UP, the rounding of P and dS before the second products (bf16 inputs only); UF = 2^-24
+for each fp32 operation, a sum of n terms counting n of them; times 1.1 for the products of two errors."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+UF = 2.0 ** -24
+UT = {BF: 2.0 ** -8, F32: UF}
+SLACK = 1.1
+DEV = "cuda"
+
+
+def tk():
+    from dfcsa import token_ops
+    return token_ops
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def rand(g, *shape, type=F32):
+    return torch.randn(shape, generator=g, device=DEV).to(type)
+
+
+def within(got, want, bound, what):
+    got, want = got.detach().double(), want.detach()
+    err = (got - want).abs()
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    over = err - bound
+    i = int(over.argmax()) if over.numel() else 0
+    assert not over.numel() or float(over.max()) <= 0, (
+        f"{what}: off by {float(err.flatten()[i]):.3g}, allowed {float(bound.expand_as(err).flatten()[i]):.3g} "
+        f"(value {float(want.flatten()[i]):.3g}, {int((over > 0).sum())} of {over.numel()} over)")
+
+
+# ------------------------------------------------------------------ RMS norm
+TYPES = [(BF, BF), (BF, F32), (F32, F32)]
+
+
+def norm_ref(x, res, w, eps):
+    r = (x.float() + res.float()).to(res.dtype).double()
+    rstd = (r.square().mean(-1, keepdim=True) + eps).rsqrt()
+    return r, rstd, r * rstd * w.double()
+
+
+@pytest.mark.parametrize("ty,st", TYPES)
+@pytest.mark.parametrize("rows,C", [(1, 8), (3, 72), (5, 768), (4, 512), (7, 1032), (130, 2048), (9, 2056), (6, 4096),
+                                    (5000, 40), (3, 8200), (2, 16384), (4097, 1024)])
+def test_norm(rows, C, ty, st):
+    g, eps = gen(rows + C), 1e-6
+    x, res, w = rand(g, rows, C, type=ty), rand(g, rows, C, type=st) * 2, 1 + 0.3 * rand(g, C)
+    dy, dr = rand(g, rows, C, type=ty), rand(g, rows, C, type=st)
+    for t in (x, res, w):
+        t.requires_grad_(True)
+    y, r = tk().rms_norm_residual(x, res, w, eps)
+    assert y.dtype == ty and r.dtype == st
+    R, rstd, Y = norm_ref(x.detach(), res.detach(), w.detach(), eps)
+    assert torch.equal(r.detach(), (x.float() + res.float()).to(st).detach())
+    n = C + 20
+    within(y, Y, SLACK * (UT[ty] + n * UF) * Y.abs(), "y")
+    dx, dres, dw = torch.autograd.grad((y, r), (x, res, w), (dy, dr))
+    W, DY = w.detach().double(), dy.double()
+    xh, u = R * rstd, DY * W
+    m = (u * xh).mean(-1, keepdim=True)
+    D = rstd * (u - xh * m) + dr.double()
+    mag = rstd * (u.abs() + xh.abs() * (u * xh).abs().mean(-1, keepdim=True)) * 2 * n * UF + 2 * UF * D.abs()
+    within(dx, D, SLACK * (mag + UT[ty] * D.abs()), "dx")
+    within(dres, D, SLACK * (mag + UT[st] * D.abs()), "dres")
+    within(dw, (DY * xh).sum(0), SLACK * (rows + n) * UF * (DY * xh).abs().sum(0), "dw")
+
+
+def test_norm_missing_gradients_and_shapes():
+    g = gen(3)
+    x, res, w = rand(g, 2, 3, 64, type=BF).requires_grad_(), rand(g, 2, 3, 64).requires_grad_(), (1 + rand(g, 64) * .1).requires_grad_()
+    dy, dr = rand(g, 2, 3, 64, type=BF), rand(g, 2, 3, 64)
+    y, r = tk().rms_norm_residual(x, res, w)
+    assert y.shape == r.shape == (2, 3, 64)
+    a = torch.autograd.grad(y, (x, res, w), dy, retain_graph=True)
+    b = torch.autograd.grad(r, (x, res, w), dr, retain_graph=True, allow_unused=True)
+    c = torch.autograd.grad((y, r), (x, res, w), (dy, dr), retain_graph=True)
+    within(a[1] + b[1], c[1].double(), 4 * UF * (a[1].abs() + b[1].abs()).double(), "sum of both")
+    assert torch.equal(b[1], dr) and torch.equal(a[2], c[2]) and float(b[2].abs().max()) == 0
+    # one input at a time
+    only = torch.autograd.grad((y, r), (w,), (dy, dr))
+    assert torch.equal(only[0], c[2])
+    y2, r2 = tk().rms_norm_residual(x.detach(), res, w.detach())
+    assert torch.equal(torch.autograd.grad((y2, r2), res, (dy, dr))[0], c[1])
+    # no rows
+    e = torch.empty(0, 64, device=DEV, requires_grad=True)
+    y, r = tk().rms_norm_residual(e, e, w)
+    assert y.shape == (0, 64) and float(torch.autograd.grad(y.sum() + r.sum(), w)[0].abs().max()) == 0
+
+
+def test_norm_strides_and_offsets():
+    g = gen(4)
+    big = rand(g, 6, 3, 72, type=BF)
+    x, res = big[:, 1], big.transpose(0, 1)[2]          # rows apart, and the other way round
+    flat = rand(g, 6 * 72 + 1, type=BF)[1:].view(6, 72)  # two bytes off a 16-byte border
+    w = 1 + 0.1 * rand(g, 73)[1:]
+    for a, b in ((x, res), (flat, x), (x, flat)):
+        y, r = tk().rms_norm_residual(a, b, w)
+        y2, r2 = tk().rms_norm_residual(a.clone(), b.clone(), w.clone())
+        assert torch.equal(y, y2) and torch.equal(r, r2)
+
+
+def test_norm_gradient_by_differences():
+    g = gen(5)
+    x, res, w = rand(g, 3, 16).requires_grad_(), rand(g, 3, 16).requires_grad_(), (1 + rand(g, 16) * .1).requires_grad_()
+    dy, dr = rand(g, 3, 16), rand(g, 3, 16)
+
+    def f(x, res, w):
+        y, r = tk().rms_norm_residual(x, res, w)
+        return (y.double() * dy).sum() + (r.double() * dr).sum()
+
+    grads = torch.autograd.grad(f(x, res, w), (x, res, w))
+    h = 2.0 ** -7
+    for i, t in enumerate((x, res, w)):
+        d = rand(g, *t.shape)
+        up = [a.detach() + (h * d if j == i else 0) for j, a in enumerate((x, res, w))]
+        dn = [a.detach() - (h * d if j == i else 0) for j, a in enumerate((x, res, w))]
+        slope = float(f(*up) - f(*dn)) / (2 * h)
+        # central differences: h^2 times a third derivative of order one, and fp32 values of order 50 over 2 h
+        assert abs(slope - float((grads[i].double() * d).sum())) < 50 * h * h + 100 * UF / h
+
+
+@pytest.mark.parametrize("ty,st", TYPES)
+@pytest.mark.parametrize("rows,C,group", [(1, 8, 0), (4, 768, 0), (5, 96, 32), (33, 256, 64), (9, 2560, 128), (3, 384, 128),
+                                          (7, 8200, 0), (3, 16384, 32), (1000, 128, 128)])
+def test_norm_q8(rows, C, group, ty, st):
+    g, eps = gen(rows * 7 + C), 1e-6
+    x, res, w = rand(g, rows, C, type=ty), rand(g, rows, C, type=st), 1 + 0.3 * rand(g, C)
+    if rows > 2:
+        x[1], res[1] = 0, 0   # a row of zeros
+    y8, s, r = tk().rms_norm_residual_q8(x, res, w, eps, group)
+    assert y8.dtype == torch.float8_e4m3fn and s.shape == (rows, C // group if group else 1)
+    R, _, Y = norm_ref(x, res, w, eps)
+    assert torch.equal(r.double(), R)
+    G = group or C
+    amax = Y.view(rows, -1, G).abs().amax(-1)
+    within(s, amax.clamp(min=1e-12) / 448, SLACK * (C + 24) * UF * amax.clamp(min=1e-12) / 448, "scales")
+    S = s.double().repeat_interleave(G, -1)
+    # half a step of e4m3: 2^-4 of the value, or of the smallest normal 2^-6, plus fp32's part
+    half = torch.maximum(Y.abs() * 2.0 ** -4, S * 2.0 ** -10)
+    within(y8.float().double() * S, Y, SLACK * half, "y8")
+    assert float((y8.float().view(rows, -1, G).abs().amax(-1)[amax > 1e-9] - 448).abs().max()) == 0
+    for ot in (BF, F32):
+        out = tk().dequant_q8(y8, s, ot)
+        assert torch.equal(out, (y8.float() * s.repeat_interleave(G, -1)).to(ot))
+
+
+def test_norm_q8_rounds_to_nearest_even_and_keeps_nan():
+    # weight picks the values: r = 1 in all columns, so y = weight up to rstd; scale 1 by a column of 448
+    C = 64
+    w = torch.ones(C, device=DEV)
+    w[0] = 448.0
+    w[1:9] = torch.tensor([1.0625, 1.1875, 17.0, 19.0, 2.0 ** -10, 3 * 2.0 ** -10, 2.0 ** -7, -1.0625], device=DEV)
+    x, res = torch.full((2, C), 0.5, device=DEV), torch.full((2, C), 0.5, device=DEV)
+    x[1, 5] = float("nan")
+    y8, s, r = tk().rms_norm_residual_q8(x, res, w, 0.0)
+    assert float(s[0]) == 1.0
+    assert y8[0, :9].float().tolist() == [448.0, 1.0, 1.25, 16.0, 20.0, 0.0, 2 * 2.0 ** -9, 2.0 ** -7, -1.0]
+    assert torch.isnan(s[1]).all() and torch.isnan(y8[1].float()).all() and torch.isnan(r[1, 5])
+    x[1, 5] = 0.5
+    x[1] *= float("inf")
+    _, s, _ = tk().rms_norm_residual_q8(x, res, w, 0.0)
+    assert float(s[0]) == 1.0 and not torch.isfinite(s[1]).any()
+
+
+# ------------------------------------------------------------------ rotary
+def rotary_ref(x, pos, axes, base, shared, inter, sign):
+    P, out, j = sum(axes), x.double().clone(), 0
+    mag = torch.zeros_like(out)
+    pos = pos if pos.dim() == 3 else pos[None]
+    for a, n in enumerate(axes):
+        for i in range(n):
+            w = pos[..., a].double() * base ** -(j / P if shared else i / n)
+            c, s = w.cos()[..., None], w.sin()[..., None] * sign
+            ia, ib = (2 * j, 2 * j + 1) if inter else (j, P + j)
+            u, v = x[..., ia].double(), x[..., ib].double()
+            out[..., ia], out[..., ib] = u * c - v * s, u * s + v * c
+            mag[..., ia] = mag[..., ib] = u.abs() + v.abs()
+            j += 1
+    return out, mag
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("B,N,H,Hk,D,axes,shared,inter,far,wide", [
+    (1, 1, 1, 1, 8, (4,), False, False, 0, False), (2, 9, 3, 1, 64, (16, 16), False, False, 0, False),
+    (2, 17, 4, 2, 128, (16, 24, 24), True, False, 10 ** 6, False), (1, 300, 12, 12, 64, (16, 16), False, False, 0, True),
+    (3, 5, 5, 5, 24, (3, 5), False, False, 100, True), (2, 6, 2, 1, 80, (9, 8, 3), True, True, 10 ** 5, False),
+    (1, 33, 2, 2, 64, (4, 4, 4, 4), False, True, 10 ** 9, True), (1, 4, 1, 1, 10, (2, 1), False, False, 7, False),
+    (5, 1, 16, 4, 128, (32, 32), False, True, 10 ** 6, False), (1, 70, 1, 1, 512, (256,), False, False, 50, False)])
+def test_rotary(B, N, H, Hk, D, axes, shared, inter, far, wide, ty):
+    g = gen(B * N + D)
+    q, k = rand(g, B, N, H, D, type=ty).requires_grad_(), rand(g, B, N, Hk, D, type=ty).requires_grad_()
+    pos = torch.randint(-far // 2, far + 50, (B, N, len(axes)), generator=g, device=DEV).to(torch.int64 if wide else torch.int32)
+    gq, gk = rand(g, B, N, H, D, type=ty), rand(g, B, N, Hk, D, type=ty)
+    oq, ok = tk().rotary(q, k, pos, axes, 10000.0, shared, inter)
+    dq, dk = torch.autograd.grad((oq, ok), (q, k), (gq, gk))
+    # cos and sin: the fraction of the turn to fp32 (2 pi 2^-26), 2 ulp of sincospi; then three operations
+    for got, src, sign in ((oq, q, 1), (ok, k, 1), (dq, gq, -1), (dk, gk, -1)):
+        want, mag = rotary_ref(src.detach(), pos, axes, 10000.0, shared, inter, sign)
+        within(got, want, SLACK * (UT[ty] * want.abs() + 12 * UF * mag), "rotary")
+        assert torch.equal(got[..., 2 * sum(axes):], src[..., 2 * sum(axes):])
+
+
+def test_rotary_strides_shared_positions_and_missing_parts():
+    g = gen(11)
+    qkv = rand(g, 2, 7, 6 * 64, type=BF)
+    q, k = qkv[..., :256].view(2, 7, 4, 64), qkv[..., 256:320].view(2, 7, 1, 64)
+    pos = torch.randint(0, 99, (7, 2), generator=g, device=DEV).to(torch.int32)
+    want = tk().rotary(q.clone(), k.clone(), pos[None].expand(2, 7, 2).contiguous(), (16, 16))
+    head_major = q.transpose(1, 2).contiguous().transpose(1, 2)
+    odd = rand(g, 2 * 7 * 4 * 64 + 1, type=BF)[1:].view(2, 7, 4, 64)
+    odd.copy_(q)
+    channels_apart = torch.stack((q, q), -1)[..., 0]
+    for qq in (q, head_major, odd, channels_apart):
+        got = tk().rotary(qq, k, pos, (16, 16))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # positions stepping through memory
+    wide = torch.stack((pos, pos * 0 - 1), -1)[..., 0]
+    assert not wide.is_contiguous() and torch.equal(tk().rotary(q, k, wide, (16, 16))[0], want[0])
+    alone = tk().rotary(q, None, pos, (16, 16))
+    assert torch.equal(alone[0], want[0]) and alone[1] is None
+    qr, kr = q.clone().requires_grad_(), k.clone().requires_grad_()
+    a, b = tk().rotary(qr, kr, pos, (16, 16))
+    da = torch.autograd.grad(a.float().sum(), (qr, kr), retain_graph=True, allow_unused=True)
+    assert da[1] is None
+    (db,) = torch.autograd.grad(b.float().sum(), kr)
+    assert db.shape == k.shape
+    back, _ = tk().rotary(a.detach(), None, -pos, (16, 16))
+    # two turns, each rounded: (|a| + |b|) of the pair twice
+    pair = q.abs().view(2, 7, 4, 2, 32).sum(-2, keepdim=True).expand(2, 7, 4, 2, 32).reshape(q.shape)
+    within(back, q.double(), 3 * UT[BF] * pair.double(), "there and back")
+    e = torch.empty(2, 0, 4, 64, device=DEV)
+    assert tk().rotary(e, None, torch.empty(0, 2, dtype=torch.int32, device=DEV), (16, 16))[0].shape == e.shape
+
+
+# ------------------------------------------------------------------ attention
+def visible(T, M, length, off, window, sinks, causal):
+    p, j = torch.arange(T, device=DEV)[:, None] + off, torch.arange(M, device=DEV)[None]
+    m = (p >= 0) & (p < length) & (j < length) & (((p - j).abs() < window) | (j < sinks))
+    return m & (j <= p) if causal else m
+
+
+def attn_ref(q, k, v, do, mask, scale, ty):
+    """(o, dq, dk, dv) in 64 bits and the bounds of their errors; q [T, H, D], k, v [M, Hk, D], mask [T, M]."""
+    T, H, D = q.shape
+    M, Hk, _ = k.shape
+    G = H // Hk
+    up, ut = (2.0 ** -8, 2.0 ** -8) if ty == BF else (0.0, UF)
+    Q, K, V = q.double().transpose(0, 1), k.double().repeat_interleave(G, 1).transpose(0, 1), v.double().repeat_interleave(G, 1).transpose(0, 1)
+    s = scale * Q @ K.transpose(1, 2)
+    sm = s.masked_fill(~mask, -math.inf)
+    top = sm.amax(-1, keepdim=True).clamp(min=-1e300)
+    e = (sm - top).exp()
+    p = e / e.sum(-1, keepdim=True).clamp(min=1e-300)
+    o = p @ V
+    n = mask.sum(-1).double()[None, :, None]
+    es = UF * ((D + 8) * scale * Q.abs() @ K.abs().transpose(1, 2) + 8 * s.abs()).masked_fill(~mask, 0)
+    ep = 2 * es.amax(-1, keepdim=True) + (n + 32) * UF
+    eo = p @ V.abs() * (up + ep + n * UF) + ut * o.abs()
+    out = [o.transpose(0, 1)], [SLACK * eo.transpose(0, 1)]
+    if do is not None:
+        dO = do.double().transpose(0, 1)
+        dp = dO @ V.transpose(1, 2)
+        dl = (dO * o).sum(-1, keepdim=True)
+        ds = p * (dp - dl)
+        edp = D * UF * dO.abs() @ V.abs().transpose(1, 2)
+        edl = (dO.abs() * eo).sum(-1, keepdim=True) + D * UF * (dO * o).abs().sum(-1, keepdim=True)
+        eds = p * ((dp - dl).abs() * (ep + 8 * UF) + edp + edl) + up * ds.abs()
+
+        def groups(x):
+            return x.view(Hk, G, M, D).sum(1).transpose(0, 1)
+
+        dq, edq = scale * ds @ K, scale * (eds + (n + 8) * UF * ds.abs()) @ K.abs()
+        rows = T * G
+        dk = groups(scale * ds.transpose(1, 2) @ Q)
+        edk = groups(scale * (eds + (rows + 8) * UF * ds.abs()).transpose(1, 2) @ Q.abs())
+        dv = groups(p.transpose(1, 2) @ dO)
+        edv = groups((p * (up + ep + (rows + 8) * UF)).transpose(1, 2) @ dO.abs())
+        for want, bound in ((dq.transpose(0, 1), edq.transpose(0, 1)), (dk, edk), (dv, edv)):
+            out[0].append(want)
+            out[1].append(SLACK * (bound + ut * want.abs()))
+    return out
+
+
+def check_train(q, k, v, do, window, sinks, causal, lengths=None, scale=None):
+    B, N, H, D = q.shape
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    o = tk().window_attention(*leaves, window, sinks, causal=causal, lengths=n, scale=scale)
+    got = (o, *torch.autograd.grad(o, leaves, do))
+    plain = tk().window_attention(*(t.detach() for t in leaves), window, sinks, causal=causal, lengths=n, scale=scale)
+    assert torch.equal(plain, o)
+    for b in range(B):
+        L = N if lengths is None else min(max(lengths[b], 0), N)
+        mask = visible(N, N, L, 0, window, sinks, causal)
+        clean = [torch.where((torch.arange(N, device=DEV) < L)[:, None, None], t[b].detach(), torch.zeros_like(t[b])) for t in (*leaves, do)]
+        want, bound = attn_ref(*clean, mask, scale or 1 / math.sqrt(D), q.dtype)
+        for name, x, w, e in zip(("o", "dq", "dk", "dv"), got, want, bound):
+            within(x[b], w, e, f"{name}[{b}]")
+    return got
+
+
+CASES = [  # B, N, H, Hk, D, window, sinks, causal
+    (1, 1, 1, 1, 8, 1, 0, True), (1, 2, 2, 1, 16, 1, 1, True), (2, 31, 3, 3, 64, 5, 0, True),
+    (1, 33, 4, 2, 64, 33, 2, False), (2, 64, 2, 2, 128, 64, 0, True), (1, 65, 8, 1, 128, 9, 4, True),
+    (1, 127, 2, 1, 40, 40, 0, False), (1, 128, 3, 1, 80, 7, 70, True), (2, 129, 6, 2, 96, 129, 0, True),
+    (1, 200, 4, 4, 64, 57, 4, False), (1, 300, 5, 5, 32, 1, 300, True), (1, 257, 2, 2, 24, 64, 130, False),
+    (1, 700, 8, 2, 128, 100, 3, True), (1, 650, 3, 1, 112, 33, 200, False), (1, 1100, 2, 1, 64, 2000, 0, True),
+    (3, 385, 1, 1, 128, 128, 1, True)]
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("B,N,H,Hk,D,window,sinks,causal", CASES)
+def test_attention(B, N, H, Hk, D, window, sinks, causal, ty):
+    g = gen(N + D)
+    q, k, v, do = rand(g, B, N, H, D, type=ty), rand(g, B, N, Hk, D, type=ty), rand(g, B, N, Hk, D, type=ty), rand(g, B, N, H, D, type=ty)
+    check_train(q, k, v, do, window, sinks, causal)
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_padded_batch(ty, causal):
+    """Lengths of zero, one, inside a tile, at its border, whole and beyond; NaN and infinity in the padding."""
+    B, N, H, Hk, D = 7, 150, 4, 2, 64
+    lengths = [0, 1, 63, 64, 129, 150, 400]
+    g = gen(9)
+    q, k, v, do = rand(g, B, N, H, D, type=ty), rand(g, B, N, Hk, D, type=ty), rand(g, B, N, Hk, D, type=ty), rand(g, B, N, H, D, type=ty)
+    for b, n in enumerate(lengths):
+        for t, bad in ((q, math.nan), (k, math.inf), (v, math.nan), (do, -math.inf)):
+            t[b, n:] = bad
+    got = check_train(q, k, v, do, 20, 3, causal, lengths)
+    for b, n in enumerate(lengths):
+        for x in got:
+            assert float(x[b, n:].abs().sum()) == 0.0   # padding: zeros
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+def test_attention_strides(ty):
+    g = gen(21)
+    B, N, H, Hk, D = 2, 90, 4, 2, 64
+    qkv = rand(g, B, N, (H + 2 * Hk) * D, type=ty)
+    q, k, v = (x.view(B, N, -1, D) for x in qkv.split((H * D, Hk * D, Hk * D), -1))
+    do = rand(g, B, N, H, D, type=ty)
+    want = check_train(q, k, v, do, 17, 2, True)
+
+    def again(q, k, v, do):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = tk().window_attention(*leaves, 17, 2)
+        for a, b in zip((o, *torch.autograd.grad(o, leaves, do)), want):
+            assert torch.equal(a, b)
+
+    hm = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v, do)]
+    again(*hm)
+    again(*(t.permute(0, 1, 3, 2).contiguous().permute(0, 1, 3, 2) for t in (q, k, v, do)))   # channels apart
+    odd = rand(g, do.numel() + 1, type=ty)[1:].view(do.shape)
+    odd.copy_(do)
+    again(q, k, v, odd)
+    # a gradient that is one number for all
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    one = torch.autograd.grad(tk().window_attention(*leaves, 17, 2).sum(), leaves)
+    leaves2 = [t.detach().requires_grad_() for t in (q, k, v)]
+    two = torch.autograd.grad(tk().window_attention(*leaves2, 17, 2), leaves2, torch.ones_like(do))
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+    # one key head broadcast to all: its gradient is the sum over the copies
+    kb = k[:, :, :1].detach().requires_grad_()
+    o = tk().window_attention(q, kb.expand(B, N, Hk, D), v, 17, 2)
+    (dkb,) = torch.autograd.grad(o, kb, do)
+    full = k[:, :, :1].expand(B, N, Hk, D).contiguous().requires_grad_()
+    (dfull,) = torch.autograd.grad(tk().window_attention(q, full, v, 17, 2), full, do)
+    within(dkb, dfull.double().sum(2, keepdim=True), 2 * UT[ty] * dfull.double().abs().sum(2, keepdim=True), "broadcast")
+
+
+def test_attention_gradient_by_differences():
+    g = gen(31)
+    q, k, v, do = rand(g, 1, 40, 2, 16), rand(g, 1, 40, 1, 16), rand(g, 1, 40, 1, 16), rand(g, 1, 40, 2, 16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def f(*a):
+        return (tk().window_attention(*a, 9, 2).double() * do).sum()
+
+    grads = torch.autograd.grad(f(*leaves), leaves)
+    h = 2.0 ** -7
+    for i in range(3):
+        d = rand(g, *leaves[i].shape)
+        up = [t.detach() + (h * d if j == i else 0) for j, t in enumerate(leaves)]
+        dn = [t.detach() - (h * d if j == i else 0) for j, t in enumerate(leaves)]
+        slope = float(f(*up) - f(*dn)) / (2 * h)
+        # h^2 times a third derivative of order 1000 (1280 outputs of order one), fp32 values over 2 h
+        assert abs(slope - float((grads[i].double() * d).sum())) < 1000 * h * h
+
+
+def test_attention_large_scores():
+    """Scores of +-1000 (the running maximum moves by far more than its slack, and rows differ), one key taking all."""
+    g = gen(41)
+    for ty in (BF, F32):
+        q, k, v, do = (rand(g, 1, 260, 2, 64, type=ty) for _ in range(4))
+        k = (k * torch.linspace(0.1, 30, 260, device=DEV)[:, None, None]).to(ty)
+        o = tk().window_attention(q, k, v, 260)
+        want, bound = attn_ref(q[0], k[0], v[0], None, visible(260, 260, 260, 0, 260, 0, True), 0.125, ty)
+        within(o[0], want[0], bound[0], "o")
+
+
+CACHED = [  # B, T, cap, H, Hk, D, window, sinks, lengths
+    (1, 1, 1, 1, 1, 8, 1, 0, [1]), (3, 1, 40, 4, 2, 64, 7, 2, [0, 1, 40]), (2, 1, 700, 8, 1, 128, 100, 4, [700, 333]),
+    (2, 1, 4100, 2, 2, 64, 5000, 0, [4100, 77]), (1, 1, 3000, 32, 1, 128, 1000, 70, [2999]),
+    (3, 3, 200, 6, 3, 40, 50, 1, [2, 3, 150]), (2, 5, 300, 40, 8, 80, 300, 0, [299, 4]),
+    (1, 40, 500, 4, 2, 96, 64, 5, [450]), (2, 100, 900, 2, 1, 128, 200, 16, [900, 60]), (1, 70, 5000, 8, 8, 32, 6000, 0, [5000]),
+    (4, 1, 64, 3, 3, 16, 64, 0, [64, 65, 1000, -3])]
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("B,T,cap,H,Hk,D,window,sinks,lengths", CACHED)
+def test_attention_cached(B, T, cap, H, Hk, D, window, sinks, lengths, ty):
+    g = gen(cap + D)
+    q, k, v = rand(g, B, T, H, D, type=ty), rand(g, B, cap, Hk, D, type=ty), rand(g, B, cap, Hk, D, type=ty)
+    for b, n in enumerate(lengths):   # behind the end, and before the window of the first new token: not read
+        n = min(max(n, 0), cap)
+        k[b, n:], v[b, n:] = math.nan, math.inf
+        lo = n - T - window + 1
+        if lo > sinks:
+            k[b, sinks:lo], v[b, sinks:lo] = math.inf, math.nan
+    n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    o = tk().window_attention_cached(q, k, v, n, window, sinks)
+    for b in range(B):
+        L = min(max(lengths[b], 0), cap)
+        mask = visible(T, cap, L, L - T, window, sinks, True)
+        seen = mask.any(0)[:, None, None]
+        want, bound = attn_ref(q[b], torch.where(seen, k[b], 0), torch.where(seen, v[b], 0), None, mask, 1 / math.sqrt(D), ty)
+        within(o[b], want[0], bound[0], f"o[{b}]")
+
+
+def test_attention_cached_is_the_last_rows_of_the_whole():
+    g = gen(51)
+    q, k, v = rand(g, 2, 300, 8, 64, type=BF), rand(g, 2, 300, 2, 64, type=BF), rand(g, 2, 300, 2, 64, type=BF)
+    whole = tk().window_attention(q, k, v, 90, 4)
+    n = torch.tensor([300, 300], dtype=torch.int32, device=DEV)
+    for T in (1, 7, 130):
+        part = tk().window_attention_cached(q[:, 300 - T:], k, v, n, 90, 4)
+        # two roundings of P and two of the result
+        within(part, whole[:, 300 - T:].double(), 4 * UT[BF] * v.double().abs().amax() * torch.ones((), device=DEV, dtype=torch.float64), "part")
+
+
+def test_attention_long_cache_offsets():
+    """Keys further than 2^31 bytes and elements from the cache's start."""
+    cap, Hk, D = 2_200_000, 8, 128   # 4.5 GB each, 2.25e9 elements
+    g = gen(61)
+    k, v = torch.zeros(1, cap, Hk, D, dtype=BF, device=DEV), torch.zeros(1, cap, Hk, D, dtype=BF, device=DEV)
+    for t in (k, v):
+        t[0, -500:] = rand(g, 500, Hk, D, type=BF)
+        t[0, :8] = rand(g, 8, Hk, D, type=BF)
+    q = rand(g, 1, 1, 16, D, type=BF)
+    n = torch.tensor([cap], dtype=torch.int32, device=DEV)
+    o = tk().window_attention_cached(q, k, v, n, 400, 8)
+    keep = torch.cat((torch.arange(8, device=DEV), torch.arange(cap - 400, cap, device=DEV)))
+    want, bound = attn_ref(q[0], k[0, keep], v[0, keep], None, torch.ones(1, 408, dtype=torch.bool, device=DEV), 1 / math.sqrt(D), BF)
+    within(o[0], want[0], bound[0], "o")
+
+
+# ------------------------------------------------------------------ a block, streams, graphs
+def block(x, stream, w1, wq, wo, w2, pos, H, Hk, D, window, sinks, lengths):
+    """norm -> projection -> rotary -> windowed attention -> projection -> norm with the residual."""
+    t = tk()
+    B, N, C = x.shape
+    y, r = t.rms_norm_residual(x, stream, w1)
+    q, k, v = (y @ wq).split((H * D, Hk * D, Hk * D), -1)
+    q, k = t.rotary(q.view(B, N, H, D), k.view(B, N, Hk, D), pos, (D // 4, D // 4))
+    o = t.window_attention(q, k, v.view(B, N, Hk, D), window, sinks, causal=False, lengths=lengths)
+    return t.rms_norm_residual(o.reshape(B, N, H * D) @ wo, r, w2)
+
+
+def block_ref(x, stream, w1, wq, wo, w2, pos, H, Hk, D, window, sinks, lengths):
+    B, N, C = x.shape
+
+    def norm(a, b, w):
+        r = a + b
+        return r * (r.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w, r
+
+    y, r = norm(x, stream, w1)
+    q, k, v = (y @ wq).split((H * D, Hk * D, Hk * D), -1)
+
+    def turn(t):
+        P = D // 2
+        w = torch.cat([pos[..., a, None].double() * 10000.0 ** -(torch.arange(D // 4, device=DEV).double() / (D // 4)) for a in range(2)], -1)
+        c, s = w.cos()[:, None], w.sin()[:, None]
+        a, b = t[..., :P], t[..., P:]
+        return torch.cat((a * c - b * s, a * s + b * c), -1)
+
+    q, k, v = turn(q.view(B, N, H, D)), turn(k.view(B, N, Hk, D)), v.view(B, N, Hk, D)
+    k, v = k.repeat_interleave(H // Hk, 2), v.repeat_interleave(H // Hk, 2)
+    out = []
+    for b in range(B):
+        mask = visible(N, N, int(lengths[b]), 0, window, sinks, False)
+        s = (torch.einsum("nhd,mhd->hnm", q[b], k[b]) / math.sqrt(D)).masked_fill(~mask, -math.inf)
+        p = torch.where(mask.any(-1)[:, None], torch.softmax(s.masked_fill(~mask.any(-1)[:, None], 0), -1), torch.zeros_like(s))
+        out.append(torch.einsum("hnm,mhd->nhd", p, v[b]))
+    return norm(torch.stack(out).reshape(B, N, H * D) @ wo, r, w2)
+
+
+def block_inputs(ty):
+    g = gen(71)
+    B, N, C, H, Hk, D = 2, 90, 128, 4, 2, 32
+    x, stream = rand(g, B, N, C, type=ty), rand(g, B, N, C)
+    w1, w2 = 1 + 0.1 * rand(g, C), 1 + 0.1 * rand(g, C)
+    wq, wo = rand(g, C, (H + 2 * Hk) * D, type=ty) / math.sqrt(C), rand(g, H * D, C, type=ty) / math.sqrt(C)
+    n = torch.arange(N, device=DEV)
+    pos = torch.stack((n // 10, n % 10), -1).to(torch.int32)
+    lengths = torch.tensor([90, 71], dtype=torch.int32, device=DEV)
+    leaves = [t.detach().requires_grad_() for t in (x, stream, w1, wq, wo, w2)]
+    return leaves, (pos, H, Hk, D, 25, 3, lengths), (rand(g, B, N, C, type=ty), rand(g, B, N, C))
+
+
+@pytest.mark.parametrize("ty,tol", [(F32, 2e-5), (BF, 0.04)])
+def test_block(ty, tol):
+    """The operators together, values and all gradients.  Relative 2-norms: fp32, about 100 roundings in a row of a
+    few hundred terms each grow like their root; bf16, ten stored tensors at 2^-8 each, and as many in the gradients."""
+    leaves, rest, douts = block_inputs(ty)
+    got = block(*leaves, *rest)
+    grads = torch.autograd.grad(got, leaves, douts)
+    ref = [t.detach().double().requires_grad_() for t in leaves]
+    want = block_ref(*ref, *rest)
+    wgrads = torch.autograd.grad(want, ref, [d.double() for d in douts])
+    for a, b in zip((*got, *grads), (*want, *wgrads)):
+        assert float((a.double() - b).norm() / b.norm()) < tol
+
+
+def test_everything_twice_is_bitwise_the_same():
+    for ty in (BF, F32):
+        leaves, rest, douts = block_inputs(ty)
+        runs = []
+        for _ in range(2):
+            got = block(*leaves, *rest)
+            runs.append((*got, *torch.autograd.grad(got, leaves, douts)))
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_side_stream():
+    leaves, rest, douts = block_inputs(BF)
+    got = block(*leaves, *rest)
+    want = (*got, *torch.autograd.grad(got, leaves, douts))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = block(*leaves, *rest)
+        got = (*got, *torch.autograd.grad(got, leaves, douts))
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def token_calls():
+    """Every entry point's call of this package alone (no library product), on inputs that can be overwritten."""
+    t, g = tk(), gen(81)
+    x, st, w = rand(g, 50, 256, type=BF).requires_grad_(), rand(g, 50, 256).requires_grad_(), (1 + rand(g, 256) * .1).requires_grad_()
+    q, k, v = (rand(g, 1, 900, h, 64, type=BF).requires_grad_() for h in (4, 2, 2))
+    pos = torch.arange(1800, device=DEV).view(900, 2).to(torch.int32)
+    cq, ck, cv = rand(g, 2, 1, 8, 64, type=BF), rand(g, 2, 2000, 2, 64, type=BF), rand(g, 2, 2000, 2, 64, type=BF)
+    n = torch.tensor([2000, 700], dtype=torch.int32, device=DEV)
+    dy, dr, do = rand(g, 50, 256, type=BF), rand(g, 50, 256), rand(g, 1, 900, 4, 64, type=BF)
+
+    def run():
+        y, r = t.rms_norm_residual(x, st, w)
+        out = [y, r, *torch.autograd.grad((y, r), (x, st, w), (dy, dr))]
+        a, b = t.rotary(q, k, pos, (16, 16))
+        o = t.window_attention(a, b, v, 60, 3)
+        out += [o, *torch.autograd.grad(o, (q, k, v), do)]
+        with torch.no_grad():
+            y8, s, r = t.rms_norm_residual_q8(x, st, w, group=64)
+            out += [t.dequant_q8(y8, s), s, t.window_attention_cached(cq, ck, cv, n, 1500, 4)]
+        return [z.detach() for z in out]
+
+    return run, (x, st, q, k, v, cq, ck, cv, dy, do)
+
+
+def test_graph_capture_and_replay():
+    """Captured once (forward and backward), replayed with new inputs between eager calls: each replay is the eager result;
+    two graphs of the same calls do not share their workspaces."""
+    run, inputs = token_calls()
+    run()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            run()
+        torch.cuda.current_stream().wait_stream(s)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = run()
+        graphs.append((gr, out))
+    g = gen(91)
+    for turn in range(4):
+        with torch.no_grad():
+            for t in inputs:
+                t.copy_(rand(g, *t.shape))
+        want = run()
+        for gr, _ in graphs:
+            gr.replay()
+        again = run()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
+        assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+def test_saved_tensors_are_guarded_and_second_order_refused():
+    g = gen(95)
+    q, k, v = (rand(g, 1, 20, 2, 16).requires_grad_() for _ in range(3))
+    o = tk().window_attention(q, k, v, 5)
+    with torch.no_grad():
+        k.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    q2 = q.detach().requires_grad_()
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    for out in (tk().window_attention(q2, k, v, 5), tk().rms_norm_residual(q2, q, w)[0], tk().rotary(q2, None, torch.zeros(
+            20, 1, dtype=torch.int32, device=DEV), (4,))[0]):
+        with pytest.raises(RuntimeError, match="first order"):
+            torch.autograd.grad(out.sum(), q2, create_graph=True)
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals():
+    t, g = tk(), gen(99)
+    x, w = rand(g, 4, 64), torch.ones(64, device=DEV)
+    b = x.to(BF)
+    for bad, e in ((lambda: t.rms_norm_residual(x, x[:2], w), ValueError), (lambda: t.rms_norm_residual(x[:, :12], x[:, :12], w[:12]), ValueError),
+                   (lambda: t.rms_norm_residual(x, b, w), TypeError), (lambda: t.rms_norm_residual(x.half(), x, w), TypeError),
+                   (lambda: t.rms_norm_residual(x, x, w.to(BF)), TypeError), (lambda: t.rms_norm_residual(x, x, w[:8]), ValueError),
+                   (lambda: t.rms_norm_residual(x, x, w, eps=-1), ValueError), (lambda: t.rms_norm_residual(x, x, w, eps=math.nan), ValueError),
+                   (lambda: t.rms_norm_residual(x, x.cpu(), w), RuntimeError),
+                   (lambda: t.rms_norm_residual_q8(x, x, w, group=16), ValueError), (lambda: t.rms_norm_residual_q8(x, x, w, group=128), ValueError),
+                   (lambda: t.dequant_q8(x, torch.ones(4, 1, device=DEV)), TypeError),
+                   (lambda: t.dequant_q8(x.to(t.E4M3), torch.ones(4, 3, device=DEV)), ValueError),
+                   (lambda: t.dequant_q8(x.to(t.E4M3), torch.ones(3, 1, device=DEV)), ValueError),
+                   (lambda: t.dequant_q8(x.to(t.E4M3), torch.ones(4, 1, device=DEV), torch.float16), TypeError)):
+        with pytest.raises(e):
+            bad()
+    q, pos = rand(g, 2, 5, 4, 16), torch.zeros(5, 2, dtype=torch.int32, device=DEV)
+    for bad, e in ((lambda: t.rotary(q[0], None, pos, (4, 4)), ValueError), (lambda: t.rotary(q, q[:, :4], pos, (4, 4)), ValueError),
+                   (lambda: t.rotary(q, q.to(BF), pos, (4, 4)), TypeError), (lambda: t.rotary(q.half(), None, pos, (4, 4)), TypeError),
+                   (lambda: t.rotary(q, q, pos, (4, 5)), ValueError), (lambda: t.rotary(q, q, pos, (4, 0)), ValueError),
+                   (lambda: t.rotary(q, q, pos, ()), ValueError), (lambda: t.rotary(q, q, pos, (1,) * 5), ValueError),
+                   (lambda: t.rotary(q, q, pos, (8,)), ValueError), (lambda: t.rotary(q, q, pos.float(), (4, 4)), TypeError),
+                   (lambda: t.rotary(q, q, pos[:4], (4, 4)), ValueError), (lambda: t.rotary(q, q, pos, (4, 4), base=0.5), ValueError),
+                   (lambda: t.rotary(q, q, pos.cpu(), (4, 4)), RuntimeError)):
+        with pytest.raises(e):
+            bad()
+    n = torch.tensor([5, 5], dtype=torch.int32, device=DEV)
+    for bad, e in ((lambda: t.window_attention(q, q, q, 0), ValueError), (lambda: t.window_attention(q, q, q, 2.5), ValueError),
+                   (lambda: t.window_attention(q, q, q, 2, -1), ValueError), (lambda: t.window_attention(q, q[:, :, :3], q[:, :, :3], 2), ValueError),
+                   (lambda: t.window_attention(q, q, q[:, :4], 2), ValueError), (lambda: t.window_attention(q, q[:, :4], q[:, :4], 2), ValueError),
+                   (lambda: t.window_attention(q[..., :12], q[..., :12], q[..., :12], 2), ValueError),
+                   (lambda: t.window_attention(rand(g, 1, 2, 1, 136), rand(g, 1, 2, 1, 136), rand(g, 1, 2, 1, 136), 2), ValueError),
+                   (lambda: t.window_attention(q, q.to(BF), q, 2), TypeError), (lambda: t.window_attention(q.half(), q.half(), q.half(), 2), TypeError),
+                   (lambda: t.window_attention(q, q, q, 2, scale=0.0), ValueError), (lambda: t.window_attention(q, q, q, 2, scale=math.inf), ValueError),
+                   (lambda: t.window_attention(q, q, q, 2, lengths=n.long()), TypeError), (lambda: t.window_attention(q, q, q, 2, lengths=n[:1]), ValueError),
+                   (lambda: t.window_attention(q, q, q, 2, lengths=n.cpu()), RuntimeError), (lambda: t.window_attention(q[0], q[0], q[0], 2), ValueError),
+                   (lambda: t.window_attention_cached(q, q, q, None, 2), TypeError), (lambda: t.window_attention_cached(q, q, q, n.float(), 2), TypeError)):
+        with pytest.raises(e):
+            bad()
+    e = torch.empty(1, 0, 2, 16, device=DEV, requires_grad=True)
+    assert torch.autograd.grad(t.window_attention(e, e, e, 3).sum(), e)[0].shape == e.shape
+    assert t.window_attention_cached(q, q[:, :0], q[:, :0], n, 3).abs().sum() == 0
