@@ -223,21 +223,28 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(int rows, int C, const T* 
   }
 }
 
-// out[c] = sum over n rows of part[.][c]: 32 columns per workgroup, 8 row slices of 32 threads, summed
-// over the slices in a fixed order
-__global__ void __launch_bounds__(256) rms_dw_kernel(int n, int C, const float* __restrict__ part,
-                                                     float* __restrict__ out) {
-  __shared__ float sm[8][32];
-  const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
-  float s = 0.f;
+// out[c] = sum over n rows of part[.][c]: 16 columns per workgroup, 64 row slices of 16 threads with four
+// loads in flight each, then the slices in a fixed order
+__global__ void __launch_bounds__(1024) rms_dw_kernel(int n, int C, const float* __restrict__ part,
+                                                      float* __restrict__ out) {
+  __shared__ float sm[64][17];
+  const int cl = threadIdx.x & 15, sl = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < C)
-    for (int i = sl; i < n; i += 8) s += part[(size_t)i * C + c];
-  sm[sl][cl] = s;
-  __syncthreads();
-  if (sl == 0 && c < C) {
+    for (int i = sl; i < n; i += 256)
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += sm[k][cl];
-    out[c] = s;
+      for (int k = 0; k < 4; ++k)
+        if (i + 64 * k < n) s[k] += part[(size_t)(i + 64 * k) * C + c];
+  sm[sl][cl] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (threadIdx.x < 64) {   // 4 slices of 16 each, then those four
+    const int q = threadIdx.x >> 4;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v += sm[q * 16 + k][cl];
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+    if (q == 0 && c < C) out[c] = v;
   }
 }
 
@@ -316,7 +323,7 @@ int launch_bwd(int rows, int C, const void* dy, const void* dr, const void* r, c
 #undef BWD
   DFCSA_CHECK_LAUNCH();
   if (dw) {
-    hipLaunchKernelGGL(rms_dw_kernel, dim3((C + 31) / 32), dim3(256), 0, st, n, C, part, dw);
+    hipLaunchKernelGGL(rms_dw_kernel, dim3((C + 15) / 16), dim3(1024), 0, st, n, C, part, dw);
     DFCSA_CHECK_LAUNCH();
   }
   return 0;

@@ -35,6 +35,8 @@
 namespace {
 
 typedef __bf16 bh8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bh2_t __attribute__((ext_vector_type(2)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef short s4_t __attribute__((ext_vector_type(4)));
 typedef short s8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
@@ -55,6 +57,7 @@ struct WArgs {
   int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh;   // bytes
   const int* lengths;
   void* o;
+  bf16_t* rest;          // training in bf16: what the rounding of o left, as bf16 (delta needs more than 8 bits of o)
   float* lse;            // [B][Hk][R], log2 of the sum of exp2(scale2 q.k)
   float* part;           // split results: O [splits][B*Hk*R][D], then lse [splits][B*Hk*R]
   int splits, tiles;     // row (or key) tiles per (batch, key head)
@@ -65,6 +68,11 @@ struct WArgs {
   void *dq, *dk, *dv;
   int nsink, csink, cwin;   // key tiles with sinks, and row chunks of those and of the other tiles
 };
+
+// two values to bf16 in one instruction
+__device__ __forceinline__ uint32_t cvt2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, bh2_t));
+}
 
 // ------------------------------------------------------------------ matrix instructions
 template <typename T> struct Mma;
@@ -78,7 +86,7 @@ template <> struct Mma<bf16_t> {
   __device__ __forceinline__ static frag pack(const f16_t& p, int st) {
     union { uint32_t u[4]; frag f; } r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.u[i] = pack2bf(p[8 * st + 2 * i], p[8 * st + 2 * i + 1]);
+    for (int i = 0; i < 4; ++i) r.u[i] = cvt2(p[8 * st + 2 * i], p[8 * st + 2 * i + 1]);
     return r.f;
   }
 };
@@ -110,32 +118,42 @@ template <typename T, int DP> struct Img {
   __device__ __forceinline__ static int swz(int row) {
     return CPR == 8 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row & 3) << 2 | ((row >> 2) & 3);
   }
-  __device__ __forceinline__ static const char* at(const char* img, int row, int chunk) {
-    return img + row * PITCH + ((chunk ^ swz(row)) << 4);
-  }
   typedef typename Mma<T>::frag frag;
-  // fragment st along the width of row `row` (this lane's), columns KS st + (KS/2)(lane/32) ..
-  __device__ __forceinline__ static frag row_frag(const char* img, int row, int st, int lane) {
-    return *(const frag*)at(img, row, 2 * st + (lane >> 5));
+  // A lane's byte offsets into an image for the two kinds of reads.  The swizzle touches only bits that
+  // the width step, the column block and the contraction step do not carry out of, so all reads of a tile
+  // are an XOR with a constant and a constant offset away from these two.
+  unsigned ra, ca;
+  __device__ __forceinline__ void init(int lane) {
+    const int row = lane & 31, h = lane >> 5;
+    ra = (unsigned)(row * PITCH + ((h ^ swz(row)) << 4));
+    if constexpr (ES == 2) {
+      const int i = lane & 15, r = 4 * h + (i >> 2), col = (lane & 16) + 4 * (i & 3);
+      ca = (unsigned)(r * PITCH + (((col >> 3) ^ swz(r)) << 4) + (col & 4) * 2);
+    } else {
+      ca = (unsigned)(4 * h * PITCH + (((row >> 2) ^ h) << 4) + (row & 3) * 4);
+    }
   }
-  // fragment of 32 columns d0 + (lane & 31) over the contraction rows of step st of rows r0 ..
-  __device__ __forceinline__ static frag col_frag(const char* img, int r0, int st, int d0, int lane) {
+  // fragment st along the width of row r0 + (lane & 31), columns KS st + (KS / 2)(lane / 32) ..
+  __device__ __forceinline__ frag row_frag(const char* img, int r0, int st) const {
+    return *(const frag*)(img + (ra ^ (unsigned)(st << 5)) + r0 * PITCH);
+  }
+  // fragment of 32 columns 32 db + (lane & 31) over the contraction rows of step st of rows r0 ..
+  __device__ __forceinline__ frag col_frag(const char* img, int r0, int st, int db) const {
     frag f;
     if constexpr (ES == 2) {
-      const int i = lane & 15, row = r0 + 16 * st + 4 * (lane >> 5) + (i >> 2);
-      const int col = d0 + (lane & 16) + 4 * (i & 3), ch = col >> 3, sub = (col & 4) * 2;
-      const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at(img, row, ch) + sub));
-      const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at(img, row + 8, ch) + sub));
+      const char* p = img + (r0 + 16 * st) * PITCH;
+      const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (ca ^ (unsigned)(db << 6))));
+      const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (ca ^ (unsigned)(db << 6 | 32)) + 8 * PITCH));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         f[e] = lo[e];
         f[4 + e] = hi[e];
       }
     } else {
-      const int col = d0 + (lane & 31);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        f[e] = *(const float*)(at(img, r0 + 8 * st + 4 * (lane >> 5) + e, col >> 2) + (col & 3) * 4);
+        f[e] = *(const float*)(img + (r0 + 8 * st + e) * PITCH +
+                               (ca ^ (unsigned)((db << 7) ^ (e << 6) ^ (((2 * st) & 3) << 4))));
     }
     return f;
   }
@@ -201,7 +219,16 @@ struct RowMask {   // of this lane's row: visible(key) = key in [lo, lo + span] 
   int lo;
   unsigned span;
   int sl;
-  __device__ __forceinline__ bool operator()(int key) const { return (unsigned)(key - lo) <= span || key < sl; }
+  // accumulator rows (keys key0 + 8 (e / 4) + e % 4) that the row does not see become `by`
+  __device__ __forceinline__ void hide(f16_t& s, int key0, float by) const {
+    const unsigned k = (unsigned)(key0 - lo);
+    const int left = sl - key0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int c = 8 * (e >> 2) + (e & 3);
+      s[e] = ((k + c <= span) | (c < left)) ? s[e] : by;
+    }
+  }
 };
 struct Seq {       // of the workgroup's sequence
   int len, off;    // valid keys; position of token 0
@@ -276,6 +303,13 @@ template <int KT> __device__ __forceinline__ TileList tiles_of(const Span& v) {
   return t;
 }
 
+__device__ __forceinline__ f16_t zero16() {
+  f16_t z;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  return z;
+}
+
 // ------------------------------------------------------------------ softmax state of 32 rows (one per lane column)
 template <typename T, int DP> struct Online {
   typedef Img<T, DP> I;
@@ -290,27 +324,30 @@ template <typename T, int DP> struct Online {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   }
-  // NSUB blocks of 32 keys from key0, at LDS rows k0 ..
-  template <int NSUB, bool MASK>
-  __device__ __forceinline__ void step(const char* kimg, const char* vimg, int row0, int key0, const frag (&q)[I::NS],
-                                       float scale2, const RowMask& mask, int lane) {
+  // NSUB blocks of 32 keys from key0
+  template <int NSUB>
+  __device__ __forceinline__ void step(const I& im, const char* kimg, const char* vimg, int key0, const frag (&q)[I::NS],
+                                       float scale2, bool masked, const RowMask& mask, int lane) {
     f16_t s[NSUB];
     float mx = kNegInf;
 #pragma unroll
     for (int b = 0; b < NSUB; ++b) {
+      s[b] = zero16();
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
-#pragma unroll
-      for (int st = 0; st < I::NS; ++st)
-        s[b] = Mma<T>::mma(I::row_frag(kimg, row0 + 32 * b + (lane & 31), st, lane), q[st], s[b]);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (MASK && !mask(key0 + 32 * b + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3))) s[b][e] = kNegInf;
-        mx = fmaxf(mx, s[b][e]);
-      }
+      for (int st = 0; st < I::NS; ++st) s[b] = Mma<T>::mma(im.row_frag(kimg, 32 * b, st), q[st], s[b]);
     }
+    if (masked) {
+      asm volatile("");   // a branch around the selects, not selects every time
+#pragma unroll
+      for (int b = 0; b < NSUB; ++b) mask.hide(s[b], key0 + 32 * b + 4 * (lane >> 5), kNegInf);
+    }
+#pragma unroll
+    for (int b = 0; b < NSUB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scale2;
     if (__any(mx > m + kGrow || (m == kNegInf && mx > kNegInf))) {
+      asm volatile("");   // keeps this a branch: as selects, the 16 ND products would run every time
       const float mn = fmaxf(m, mx);
       const float al = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= al;
@@ -332,7 +369,7 @@ template <typename T, int DP> struct Online {
       for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
         const frag p = Mma<T>::pack(s[b], st);
 #pragma unroll
-        for (int d = 0; d < I::ND; ++d) o[d] = Mma<T>::mma(I::col_frag(vimg, row0 + 32 * b, st, 32 * d, lane), p, o[d]);
+        for (int d = 0; d < I::ND; ++d) o[d] = Mma<T>::mma(im.col_frag(vimg, 32 * b, st, d), p, o[d]);
       }
     }
   }
@@ -356,7 +393,7 @@ template <> __device__ __forceinline__ void store4<float>(float* p, float a, flo
   *(float4*)p = make_float4(a, b, c, d);
 }
 template <> __device__ __forceinline__ void store4<bf16_t>(bf16_t* p, float a, float b, float c, float d) {
-  *(uint2*)p = make_uint2(pack2bf(a, b), pack2bf(c, d));
+  *(uint2*)p = make_uint2(cvt2(a, b), cvt2(c, d));
 }
 // column `lane & 31` of an accumulated [head column][row] tile to the row at p
 template <typename T, int ND>
@@ -370,6 +407,21 @@ __device__ __forceinline__ void store_col(T* p, const f16_t (&o)[ND], float f, i
     }
 }
 
+// what the rounding of four values to bf16 left, as bf16
+__device__ __forceinline__ void store4_rest(bf16_t* p, float a, float b, float c, float d) {
+  store4<bf16_t>(p, a - bf2f(f2bf(a)), b - bf2f(f2bf(b)), c - bf2f(f2bf(c)), d - bf2f(f2bf(d)));
+}
+template <int ND>
+__device__ __forceinline__ void store_col_rest(bf16_t* p, const f16_t (&o)[ND], float f, int D, int lane) {
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * d + 8 * g + 4 * (lane >> 5);
+      if (c < D) store4_rest(p + c, o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
+    }
+}
+
 // Row r's result of (part of) its keys: straight to o and lse, or to the split's partial.
 template <typename T, int DP>
 __device__ __forceinline__ void finish_row(const WArgs& a, int bh, int split, int r, const f16_t (&o)[DP / 32], float m,
@@ -380,8 +432,9 @@ __device__ __forceinline__ void finish_row(const WArgs& a, int bh, int split, in
   const int64_t row = (int64_t)bh * a.R + r, rows = (int64_t)a.B * a.Hk * a.R;
   if (a.splits == 1) {
     const int b = bh / a.Hk, hk = bh - b * a.Hk, t = dm_div(a.dmG, r), g = r - t * a.G;
-    T* p = (T*)a.o + (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
-    store_col<T, DP / 32>(p, o, inv, a.D, lane);
+    const int64_t at = (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
+    store_col<T, DP / 32>((T*)a.o + at, o, inv, a.D, lane);
+    if (sizeof(T) == 2 && a.rest) store_col_rest<DP / 32>(a.rest + at, o, inv, a.D, lane);
     if (a.lse && lane < 32) a.lse[row] = lse;
   } else {
     store_col<float, DP / 32>(a.part + (split * rows + row) * a.D, o, inv, a.D, lane);
@@ -392,7 +445,7 @@ __device__ __forceinline__ void finish_row(const WArgs& a, int bh, int split, in
 // ============================================================================ forward
 // 128 rows per workgroup, 32 per wave; key tiles double-buffered in LDS.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) wattn_fwd_kernel(const WArgs a) {
+__global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wattn_fwd_kernel(const WArgs a) {
   typedef Img<T, DP> I;
   constexpr int KT = I::ROWS;
   __shared__ __attribute__((aligned(16))) char smem[4 * I::BYTES];
@@ -418,6 +471,8 @@ __global__ void __launch_bounds__(256) wattn_fwd_kernel(const WArgs a) {
     const int t = dm_div(a.dmG, min(r, a.R - 1)), g = min(r, a.R - 1) - t * a.G;
     load_frags<T, DP>((const char*)a.q + b * a.qb + t * a.qt + (hk * a.G + g) * a.qh, mask.lo != 0x7fffffff, a.D, lane, q);
   }
+  I im;
+  im.init(lane);
   Online<T, DP> st;
   st.init();
   if (it0 < it1) {
@@ -436,12 +491,8 @@ __global__ void __launch_bounds__(256) wattn_fwd_kernel(const WArgs a) {
     }
     lds_barrier();
     const int key0 = tl[it] * KT;
-    if (sees_any(my, key0, key0 + KT)) {
-      if (sees_all(a, seq, my, key0, key0 + KT))
-        st.template step<KT / 32, false>(cur, cur + I::BYTES, 0, key0, q, a.scale2, mask, lane);
-      else
-        st.template step<KT / 32, true>(cur, cur + I::BYTES, 0, key0, q, a.scale2, mask, lane);
-    }
+    if (sees_any(my, key0, key0 + KT))
+      st.template step<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane);
     lds_barrier();   // every wave is done with this buffer before it is filled again
   }
   const float lsum = st.l + __shfl_xor(st.l, 32, 64);
@@ -483,6 +534,8 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
     const int t = dm_div(a.dmG, min(r, a.R - 1)), g = min(r, a.R - 1) - t * a.G;
     load_frags<T, DP>((const char*)a.q + b * a.qb + t * a.qt + (hk * a.G + g) * a.qh, mask.lo != 0x7fffffff, a.D, lane, q);
   }
+  I im;
+  im.init(lane);
   Online<T, DP> st;
   st.init();
   if (it0 < it1) {
@@ -502,10 +555,7 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
       wait_vm<0>();
     }
     const int key0 = tl[it] * KT;
-    if (sees_all(a, seq, my, key0, key0 + KT))
-      st.template step<1, false>(c, c + IB, 0, key0, q, a.scale2, mask, lane);
-    else
-      st.template step<1, true>(c, c + IB, 0, key0, q, a.scale2, mask, lane);
+    st.template step<1>(im, c, c + IB, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane);
     if (STG == 1 && it + 4 < it1) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       dma.issue(kbase, a.kt, tl[it + 4] * KT, my.lo, my.hi, my.sl, n, 0);
@@ -543,7 +593,8 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
   const float lse = ls == 0.f ? kNegInf : mm + __builtin_amdgcn_logf(ls);
   const int64_t orow = (int64_t)bh * a.R + rr, rows = (int64_t)a.B * a.Hk * a.R;
   const int t = dm_div(a.dmG, rr), g = rr - t * a.G;
-  T* po = (T*)a.o + (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
+  const int64_t at = (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
+  T* po = (T*)a.o + at;
   float* pp = a.splits == 1 ? nullptr : a.part + (split * rows + orow) * a.D;
 #pragma unroll
   for (int c = 0; c < DP / 8; c += 4) {
@@ -557,8 +608,12 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
         s[2] += f[w] * x.z;
         s[3] += f[w] * x.w;
       }
-      if (pp) store4<float>(pp + c0 + c, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
-      else store4<T>(po + c0 + c, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
+      if (pp) {
+        store4<float>(pp + c0 + c, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
+      } else {
+        store4<T>(po + c0 + c, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
+        if (sizeof(T) == 2 && a.rest) store4_rest(a.rest + at + c0 + c, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
+      }
     }
   }
   if ((threadIdx.x & 7) == 0) {
@@ -567,41 +622,54 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
   }
 }
 
-// One row per 32 threads: the splits' results weighted by their sums, in split order.
+// One row per 32 threads: the splits' results weighted by their sums, in split order.  At most 64
+// splits; their 2 x 32 sums are read at once, then four results are in flight at a time.
 template <typename T>
 __global__ void __launch_bounds__(256) wattn_join_kernel(const WArgs a) {
   const int64_t rows = (int64_t)a.B * a.Hk * a.R, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const int c = (threadIdx.x & 31) * 4;
+  const int i = threadIdx.x & 31, c = i * 4;
   const float* lp = a.part + a.splits * rows * a.D + row;
-  float mm = kNegInf;
-  for (int z = 0; z < a.splits; ++z) mm = fmaxf(mm, lp[z * rows]);
+  const float l0 = i < a.splits ? lp[i * rows] : kNegInf, l1 = i + 32 < a.splits ? lp[(i + 32) * rows] : kNegInf;
+  float mm = fmaxf(l0, l1);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 32));
+  // a NaN sum has to reach the result: the maximum drops it, its weight does not
+  const float f0 = l0 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(l0 - mm);
+  const float f1 = l1 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(l1 - mm);
   float s[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
-  for (int z = 0; z < a.splits; ++z) {
-    const float lz = lp[z * rows];
-    const float f = lz == kNegInf ? 0.f : __builtin_amdgcn_exp2f(lz - mm);
-    ls += f;
-    if (c < a.D) {
-      const float4 x = *(const float4*)(a.part + (z * rows + row) * a.D + c);
-      s[0] += f * x.x;
-      s[1] += f * x.y;
-      s[2] += f * x.z;
-      s[3] += f * x.w;
+  const float* p = a.part + row * a.D + (c < a.D ? c : 0);
+  for (int z0 = 0; z0 < a.splits; z0 += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = *(const float4*)(p + (int64_t)min(z0 + k, a.splits - 1) * rows * a.D);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int z = z0 + k;
+      const float f = z < a.splits ? __shfl(z < 32 ? f0 : f1, z & 31, 32) : 0.f;
+      if (f == 0.f) continue;   // a split that saw nothing
+      ls += f;
+      s[0] += f * x[k].x;
+      s[1] += f * x[k].y;
+      s[2] += f * x[k].z;
+      s[3] += f * x[k].w;
     }
   }
   const float inv = ls == 0.f ? 0.f : 1.0f / ls;
   const int bh = (int)(row / a.R), r = (int)(row - (int64_t)bh * a.R);
   const int b = bh / a.Hk, hk = bh - b * a.Hk, t = dm_div(a.dmG, r), g = r - t * a.G;
-  if (c < a.D)
-    store4<T>((T*)a.o + (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D + c, s[0] * inv, s[1] * inv, s[2] * inv,
-              s[3] * inv);
-  if (a.lse && (threadIdx.x & 31) == 0) a.lse[row] = ls == 0.f ? kNegInf : mm + __builtin_amdgcn_logf(ls);
+  if (c < a.D) {
+    const int64_t at = (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D + c;
+    store4<T>((T*)a.o + at, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
+    if (sizeof(T) == 2 && a.rest) store4_rest(a.rest + at, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
+  }
+  if (a.lse && i == 0) a.lse[row] = ls == 0.f ? kNegInf : mm + __builtin_amdgcn_logf(ls);
 }
 
 // ============================================================================ backward: dQ
 // As the forward, with S and dP per key tile; also writes delta = dO . O for the key-major pass.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) wattn_dq_kernel(const WArgs a) {
+__global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wattn_dq_kernel(const WArgs a) {
   typedef Img<T, DP> I;
   typedef typename I::frag frag;
   constexpr int KT = I::ROWS;
@@ -633,6 +701,14 @@ __global__ void __launch_bounds__(256) wattn_dq_kernel(const WArgs a) {
     frag of[I::NS];
     load_frags<T, DP>((const char*)((const T*)a.o + orow), live, a.D, lane, of);
     constexpr int NE = sizeof(frag) / sizeof(T);
+    if (sizeof(T) == 2 && a.rest) {
+      frag rf[I::NS];
+      load_frags<T, DP>((const char*)(a.rest + orow), live, a.D, lane, rf);
+#pragma unroll
+      for (int st = 0; st < I::NS; ++st)
+#pragma unroll
+        for (int e = 0; e < NE; ++e) dl += bf2f((bf16_t)rf[st][e]) * bf2f((bf16_t)dof[st][e]);
+    }
 #pragma unroll
     for (int st = 0; st < I::NS; ++st)
 #pragma unroll
@@ -647,9 +723,31 @@ __global__ void __launch_bounds__(256) wattn_dq_kernel(const WArgs a) {
   }
   f16_t dq[I::ND];
 #pragma unroll
-  for (int d = 0; d < I::ND; ++d)
+  for (int d = 0; d < I::ND; ++d) dq[d] = zero16();
+  I im;
+  im.init(lane);
+  auto body = [&](const char* cur, int key0, bool masked) {
+#pragma unroll 1   // one 32 x 32 block's registers at a time; the other wave of the SIMD fills the gaps
+    for (int kb = 0; kb < KT / 32; ++kb) {
+      f16_t s = zero16(), dp = zero16();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
+      for (int st = 0; st < I::NS; ++st) s = Mma<T>::mma(im.row_frag(cur, 32 * kb, st), q[st], s);
+#pragma unroll
+      for (int st = 0; st < I::NS; ++st) dp = Mma<T>::mma(im.row_frag(cur + I::BYTES, 32 * kb, st), dof[st], dp);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - dl);
+      if (masked) {
+        asm volatile("");
+        mask.hide(s, key0 + 32 * kb + 4 * (lane >> 5), 0.f);
+      }
+#pragma unroll
+      for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+        const frag ds = Mma<T>::pack(s, st);
+#pragma unroll
+        for (int d = 0; d < I::ND; ++d) dq[d] = Mma<T>::mma(im.col_frag(cur, 32 * kb, st, d), ds, dq[d]);
+      }
+    }
+  };
   if (tl.n > 0) {
     dma.issue(kbase, a.kt, tl[0] * KT, wg.lo, wg.hi, wg.sl, smem, wave);
     dma.issue(vbase, a.vt, tl[0] * KT, wg.lo, wg.hi, wg.sl, smem + I::BYTES, wave);
@@ -666,35 +764,7 @@ __global__ void __launch_bounds__(256) wattn_dq_kernel(const WArgs a) {
     }
     lds_barrier();
     const int key0 = tl[it] * KT;
-    if (sees_any(my, key0, key0 + KT)) {
-      const bool all = sees_all(a, seq, my, key0, key0 + KT);
-#pragma unroll
-      for (int kb = 0; kb < KT / 32; ++kb) {
-        f16_t s, dp;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-#pragma unroll
-        for (int st = 0; st < I::NS; ++st) {
-          s = Mma<T>::mma(I::row_frag(cur, 32 * kb + (lane & 31), st, lane), q[st], s);
-          dp = Mma<T>::mma(I::row_frag(cur + I::BYTES, 32 * kb + (lane & 31), st, lane), dof[st], dp);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse));
-          if (!all && !mask(key0 + 32 * kb + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3))) {
-            p = 0.f;
-            dp[e] = 0.f;
-          }
-          s[e] = p * (dp[e] - dl);
-        }
-#pragma unroll
-        for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
-          const frag ds = Mma<T>::pack(s, st);
-#pragma unroll
-          for (int d = 0; d < I::ND; ++d) dq[d] = Mma<T>::mma(I::col_frag(cur, 32 * kb, st, 32 * d, lane), ds, dq[d]);
-        }
-      }
-    }
+    if (sees_any(my, key0, key0 + KT)) body(cur, key0, !sees_all(a, seq, my, key0, key0 + KT));
     lds_barrier();
   }
   if (r < a.R) store_col<T, I::ND>((T*)a.dq + orow, dq, a.scale, a.D, lane);
@@ -705,12 +775,15 @@ __global__ void __launch_bounds__(256) wattn_dq_kernel(const WArgs a) {
 // LDS.  A key tile that holds sinks is seen by every later row: its rows are split over csink
 // workgroups (cwin for the others), whose fp32 parts wattn_dkv_join adds in order.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, 1) wattn_dkv_kernel(const WArgs a) {
+__global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wattn_dkv_kernel(const WArgs a) {
   typedef Img<T, DP> I;
   typedef typename I::frag frag;
-  constexpr int RT = I::ROWS;
+  // bf16 heads wider than 64: K (32 registers) stays in LDS and row tiles are 32 high, so that two
+  // waves fit on a SIMD beside the 128 accumulators
+  constexpr bool KLDS = sizeof(T) == 2 && DP > 64;
+  constexpr int RT = KLDS ? 32 : I::ROWS, RB = RT * I::PITCH;
   constexpr int NI = RT * I::CPR / 64 / 4;
-  __shared__ __attribute__((aligned(16))) char smem[4 * I::BYTES];
+  __shared__ __attribute__((aligned(256))) char smem[4 * RB + (KLDS ? 128 * I::PITCH : 0)];
   __shared__ __attribute__((aligned(16))) float s_l[2][RT], s_d[2][RT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int items = a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin;
@@ -742,10 +815,17 @@ __global__ void __launch_bounds__(256, 1) wattn_dkv_kernel(const WArgs a) {
 
   const int kw = k0 + wave * 32, key = kw + (lane & 31);
   const bool kok = key < seq.len;
-  frag kf[I::NS], vf[I::NS];
+  frag kf[KLDS ? 1 : I::NS], vf[I::NS];
+  const char* kimg = smem + 4 * RB;
   {
     const int kk = min(key, a.M - 1);
-    load_frags<T, DP>((const char*)a.k + b * a.kb + (int64_t)kk * a.kt + hk * a.kh, kok, a.D, lane, kf);
+    if constexpr (KLDS) {
+      KeyDma<T, DP, 128, 4> dma;
+      dma.init(wave, lane, a.D);
+      if (k0 < seq.len) dma.issue((const char*)a.k + b * a.kb + hk * a.kh, a.kt, k0, 0, seq.len, 0, smem + 4 * RB, wave);
+    } else {
+      load_frags<T, DP>((const char*)a.k + b * a.kb + (int64_t)kk * a.kt + hk * a.kh, kok, a.D, lane, kf);
+    }
     load_frags<T, DP>((const char*)a.v + b * a.vb + (int64_t)kk * a.vt + hk * a.vh, kok, a.D, lane, vf);
   }
   // rows that see this lane's key: [vlo, vhi)
@@ -793,7 +873,7 @@ __global__ void __launch_bounds__(256, 1) wattn_dkv_kernel(const WArgs a) {
       const int r = r0 + drow[i], t = dm_div(a.dmG, r), g = r - t * a.G;
       const unsigned bad = (r < rlim ? 0u : kOob) | (dch[i] & kOob);
       dma16(rq, bad | (dch[i] + (unsigned)((t - t0) * (int)a.qt + g * (int)a.qh)), img + (i * 4 + wave) * 1024);
-      dma16(ro, bad | (dch[i] + (unsigned)((t - t0) * (int)a.ot + g * (int)a.oh)), img + I::BYTES + (i * 4 + wave) * 1024);
+      dma16(ro, bad | (dch[i] + (unsigned)((t - t0) * (int)a.ot + g * (int)a.oh)), img + RB + (i * 4 + wave) * 1024);
     }
   };
   const float* lbase = a.lse + (int64_t)bh * a.R;
@@ -811,9 +891,54 @@ __global__ void __launch_bounds__(256, 1) wattn_dkv_kernel(const WArgs a) {
   };
   f16_t dk[I::ND], dv[I::ND];
 #pragma unroll
-  for (int d = 0; d < I::ND; ++d)
+  for (int d = 0; d < I::ND; ++d) dk[d] = dv[d] = zero16();
+  I im;
+  im.init(lane);
+  auto body = [&](const char* cur, int buf, int r0, bool masked) {
+#pragma unroll 1
+    for (int rb = 0; rb < RT / 32; ++rb) {
+      f16_t s = zero16(), dp = zero16();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+      for (int st = 0; st < I::NS; ++st) {
+        frag kk;
+        if constexpr (KLDS) kk = im.row_frag(kimg + wave * 32 * I::PITCH, 0, st);
+        else kk = kf[st];
+        s = Mma<T>::mma(im.row_frag(cur, 32 * rb, st), kk, s);
+      }
+#pragma unroll
+      for (int st = 0; st < I::NS; ++st) dp = Mma<T>::mma(im.row_frag(cur + RB, 32 * rb, st), vf[st], dp);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int rr = 32 * rb + 8 * g + 4 * (lane >> 5);
+        const f4_t l4 = *(const f4_t*)&s_l[buf][rr], d4 = *(const f4_t*)&s_d[buf][rr];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale2, -l4[e]));
+          dp[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - d4[e]);
+        }
+      }
+      if (masked) {
+        asm volatile("");
+        const int rr = r0 + 32 * rb + 4 * (lane >> 5), ge = vlo - rr, lt = vhi - rr;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int c = 8 * (e >> 2) + (e & 3);
+          const bool see = (c >= ge) & (c < lt);
+          s[e] = see ? s[e] : 0.f;
+          dp[e] = see ? dp[e] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+        const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
+#pragma unroll
+        for (int d = 0; d < I::ND; ++d) {
+          dv[d] = Mma<T>::mma(im.col_frag(cur + RB, 32 * rb, st, d), pf, dv[d]);
+          dk[d] = Mma<T>::mma(im.col_frag(cur, 32 * rb, st, d), df, dk[d]);
+        }
+      }
+    }
+  };
 
   if (c0 < c1) {
     put(stat(c0), 0);
@@ -821,12 +946,12 @@ __global__ void __launch_bounds__(256, 1) wattn_dkv_kernel(const WArgs a) {
   }
   for (int it = c0; it < c1; ++it) {
     const int buf = (it - c0) & 1;
-    char* cur = smem + buf * 2 * I::BYTES;
+    char* cur = smem + buf * 2 * RB;
     float nx = 0.f;
     const bool more = it + 1 < c1;
     if (more) {
       nx = stat(it + 1);
-      issue(it + 1, smem + (buf ^ 1) * 2 * I::BYTES);
+      issue(it + 1, smem + (buf ^ 1) * 2 * RB);
       wait_vm<2 * NI>();   // all but the DMAs just issued
     } else {
       wait_vm<0>();
@@ -834,41 +959,7 @@ __global__ void __launch_bounds__(256, 1) wattn_dkv_kernel(const WArgs a) {
     lds_barrier();
     const int r0 = it * RT;
     if (r0 < nhi && r0 + RT > nlo) {
-      const bool all = r0 >= alo && r0 + RT <= ahi;
-#pragma unroll
-      for (int rb = 0; rb < RT / 32; ++rb) {
-        f16_t s, dp;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-#pragma unroll
-        for (int st = 0; st < I::NS; ++st) {
-          s = Mma<T>::mma(I::row_frag(cur, 32 * rb + (lane & 31), st, lane), kf[st], s);
-          dp = Mma<T>::mma(I::row_frag(cur + I::BYTES, 32 * rb + (lane & 31), st, lane), vf[st], dp);
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int rr = 32 * rb + 8 * g + 4 * (lane >> 5);
-          const f4_t l4 = *(const f4_t*)&s_l[buf][rr], d4 = *(const f4_t*)&s_d[buf][rr];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = r0 + rr + e;
-            float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale2, -l4[e]));
-            float dd = dp[4 * g + e] - d4[e];
-            if (!all && (r < vlo || r >= vhi)) p = dd = 0.f;
-            s[4 * g + e] = p;
-            dp[4 * g + e] = p * dd;
-          }
-        }
-#pragma unroll
-        for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
-          const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
-#pragma unroll
-          for (int d = 0; d < I::ND; ++d) {
-            dv[d] = Mma<T>::mma(I::col_frag(cur + I::BYTES, 32 * rb, st, 32 * d, lane), pf, dv[d]);
-            dk[d] = Mma<T>::mma(I::col_frag(cur, 32 * rb, st, 32 * d, lane), df, dk[d]);
-          }
-        }
-      }
+      body(cur, buf, r0, r0 < alo || r0 + RT > ahi);
     }
     if (more) put(nx, buf ^ 1);
     lds_barrier();
@@ -951,6 +1042,7 @@ bool fill(const dfcsa_wattn_desc* d, WArgs& a, bool backward) {
   a.vb = d->v_stride[0] * es; a.vt = d->v_stride[1] * es; a.vh = d->v_stride[2] * es;
   a.lengths = d->lengths;
   a.o = d->o;
+  a.rest = d->dtype == DFCSA_DT_BF16 ? (bf16_t*)d->o_rest : nullptr;
   a.lse = d->lse;
   a.part = d->work;
   a.splits = 1;

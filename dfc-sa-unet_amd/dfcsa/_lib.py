@@ -138,7 +138,7 @@ class WattnDesc(ctypes.Structure):
                 ("lengths", ctypes.c_void_p), ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p),
                 ("work", ctypes.c_void_p), ("work_floats", ctypes.c_int64), ("dout", ctypes.c_void_p),
                 ("dout_stride", ctypes.c_int64 * 3), ("delta", ctypes.c_void_p), ("dq", ctypes.c_void_p),
-                ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p)]
+                ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p), ("o_rest", ctypes.c_void_p)]
 
 
 def _load():

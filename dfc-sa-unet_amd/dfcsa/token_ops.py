@@ -63,8 +63,8 @@ def _dtype(t, what):
 
 def _launch(dev, name, *args):
     """The entry point on the current stream of `dev`, whichever device is current."""
-    s = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-    if dev.index == torch.cuda.current_device():
+    s = torch._C._cuda_getCurrentRawStream(dev.index)
+    if dev.index == torch._C._cuda_getDevice():
         return call(name, *args, s)
     with torch.cuda.device(dev):
         return call(name, *args, s)
@@ -380,10 +380,12 @@ def _workspace(d, backward, dev):
     return work
 
 
-def _attend(dev, ty, q, k, v, window, sinks, causal, cached, scale, lengths, lse):
+def _attend(dev, ty, q, k, v, window, sinks, causal, cached, scale, lengths, lse, rest=None):
     """o; q, k, v as _strided gives them, lengths contiguous."""
     o = torch.empty(q.shape, dtype=q.dtype, device=dev)
     d = _desc(ty, q, k, v, window, sinks, causal, cached, scale, lengths, o, lse)
+    if rest is not None:
+        d.o_rest = rest.data_ptr()
     work = _workspace(d, False, dev)
     _launch(dev, "dfcsa_wattn_fwd", ctypes.addressof(d))
     del work
@@ -396,21 +398,24 @@ class _WindowAttention(torch.autograd.Function):
         dev, ty, window, sinks, causal, scale = meta
         B, T, H, _ = q.shape
         lse = torch.empty(B * T * H, dtype=torch.float32, device=dev)
-        o = _attend(dev, ty, q, k, v, window, sinks, causal, False, scale, lengths, lse)
-        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        # bf16: the backward's dO . O needs more of O than its 8 bits, so what the rounding left is kept too
+        rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if ty == _lib.DT_BF16 else None
+        o = _attend(dev, ty, q, k, v, window, sinks, causal, False, scale, lengths, lse, rest)
+        ctx.save_for_backward(q, k, v, o, lse, lengths, rest)
         ctx.meta = meta
         return o
 
     @staticmethod
     @_first_order
     def backward(ctx, do):
-        q, k, v, o, lse, lengths = ctx.saved_tensors
+        q, k, v, o, lse, lengths, rest = ctx.saved_tensors
         dev, ty, window, sinks, causal, scale = ctx.meta
         do = _strided(do, q.shape[2] // k.shape[2])
         dq, delta = torch.empty(q.shape, dtype=q.dtype, device=dev), torch.empty_like(lse)
         dk, dv = torch.empty(k.shape, dtype=k.dtype, device=dev), torch.empty(v.shape, dtype=v.dtype, device=dev)
         d = _desc(ty, q, k, v, window, sinks, causal, False, scale, lengths, o, lse)
         d.dout, d.dout_stride[:] = do.data_ptr(), do.stride()[:3]
+        d.o_rest = None if rest is None else rest.data_ptr()
         d.delta, d.dq, d.dk, d.dv = delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         work = _workspace(d, True, dev)
         _launch(dev, "dfcsa_wattn_bwd", ctypes.addressof(d))

@@ -979,7 +979,8 @@ int dfcsa_rotary(const dfcsa_rotary_desc* d, void* stream);
  * cached == 0: T == M, token t is at position t.  cached != 0 (causal, lengths required, forward
  * only): token t is at position length - T + t.
  * lse [B][Hk][T * H / Hk]: log2 of the rows' sums, written by fwd (may be NULL there), read by bwd;
- * delta: scratch of the same size.  work: dfcsa_wattn_work_floats floats (0: may be NULL). */
+ * delta: scratch of the same size.  o_rest (bf16, may be NULL): [B][T][H][D] bf16, what the rounding of
+ * o left, written by fwd, read by bwd for delta = dO . O.  work: dfcsa_wattn_work_floats floats (0: may be NULL). */
 typedef struct {
   int dtype, B, T, M, H, Hk, D, window, sinks, causal, cached;
   float scale;
@@ -998,6 +999,7 @@ typedef struct {
   void* dq;
   void* dk;
   void* dv;
+  void* o_rest;
 } dfcsa_wattn_desc;
 int dfcsa_wattn_work_floats(const dfcsa_wattn_desc* d, int backward, int64_t* floats);
 int dfcsa_wattn_fwd(const dfcsa_wattn_desc* d, void* stream);
