@@ -83,6 +83,15 @@ template <> struct Mma<bf16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bh8_t, a), __builtin_bit_cast(bh8_t, b), c, 0, 0, 0);
   }
   // accumulator registers of contraction step st (16 rows of the 32) as a fragment
+  // a sum plus a fragment's elements
+  __device__ __forceinline__ static float add(const frag& f, float l) {
+    union { frag f; uint32_t u[4]; } x;
+    x.f = f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bh2_t, x.u[i]), (bh2_t){(__bf16)1.0f, (__bf16)1.0f}, l, false);
+    return l;
+  }
   __device__ __forceinline__ static frag pack(const f16_t& p, int st) {
     union { uint32_t u[4]; frag f; } r;
 #pragma unroll
@@ -98,6 +107,7 @@ template <> struct Mma<float> {
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
     return c;
   }
+  __device__ __forceinline__ static float add(const frag& f, float l) { return l + ((f[0] + f[1]) + (f[2] + f[3])); }
   __device__ __forceinline__ static frag pack(const f16_t& p, int st) {
     return frag{p[4 * st], p[4 * st + 1], p[4 * st + 2], p[4 * st + 3]};
   }
@@ -162,8 +172,7 @@ template <typename T, int DP> struct Img {
 // ------------------------------------------------------------------ LDS-DMA
 // One instruction moves 64 x 16 bytes to consecutive LDS addresses.  Written in inline asm so that the
 // compiler does not drain it before the next LDS read; the kernels wait for their DMAs themselves.  An
-// offset past num_records reads zeros.  s_nop: the descriptor may come from a lane read (v_readfirstlane),
-// which needs five wait states before a memory instruction takes it.
+// offset past num_records reads zeros.
 constexpr unsigned kOob = 0x80000000u;
 __device__ __forceinline__ i4_t make_rsrc(const void* base) {
   const uint64_t p = (uint64_t)base;
@@ -172,15 +181,20 @@ __device__ __forceinline__ i4_t make_rsrc(const void* base) {
   r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xffffu));
   r[2] = 0x7fffffff;
   r[3] = 0x00020000;
+  // a scalar register that a lane read wrote needs five wait states before a memory instruction takes it
+  asm volatile("s_nop 4" : "+s"(r));
   return r;
 }
-__device__ __forceinline__ void dma16(const i4_t& rsrc, unsigned voff, const char* lds) {
-  const unsigned dst = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(const __attribute__((address_space(3))) char*)lds);
+__device__ __forceinline__ unsigned lds_addr(const char* p) {
+  return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p;
+}
+// lds: wave-uniform
+__device__ __forceinline__ void dma16(const i4_t& rsrc, unsigned voff, unsigned lds) {
   unsigned keep;
   asm volatile(
-      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
       : "=&s"(keep)
-      : "v"(voff), "s"(rsrc), "s"(dst)
+      : "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds))
       : "memory");
 }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
@@ -200,16 +214,22 @@ template <typename T, int DP, int ROWS, int NW> struct KeyDma {
       chunk[i] = ch * 16 < D * I::ES ? (unsigned)ch * 16 : kOob;
     }
   }
-  // rows key0 + row of base; row valid if in [lo, hi) or below sl
-  __device__ __forceinline__ void issue(const char* base, int64_t stride, int key0, int lo, int hi, int sl, char* img,
+  // rows key0 + row of base into the image at lds; a row is valid if in [lo, hi) or below sl
+  __device__ __forceinline__ void issue(const char* base, int64_t stride, int key0, int lo, int hi, int sl, unsigned lds,
                                         int wave) const {
     const i4_t rs = make_rsrc(base + (int64_t)key0 * stride);
+    if (key0 + ROWS <= sl || (key0 >= lo && key0 + ROWS <= hi)) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int key = key0 + row[i];
-      const bool ok = (key >= lo && key < hi) || key < sl;
-      const unsigned off = (ok ? 0u : kOob) | (chunk[i] + (unsigned)row[i] * (unsigned)stride);
-      dma16(rs, (chunk[i] & kOob) | off, img + (i * NW + wave) * 1024);
+      for (int i = 0; i < NI; ++i)
+        dma16(rs, chunk[i] + (unsigned)row[i] * (unsigned)stride, lds + (i * NW + wave) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int key = key0 + row[i];
+        const bool ok = (key >= lo && key < hi) || key < sl;
+        dma16(rs, (ok ? 0u : kOob) | (chunk[i] & kOob) | (chunk[i] + (unsigned)row[i] * (unsigned)stride),
+              lds + (i * NW + wave) * 1024);
+      }
     }
   }
 };
@@ -361,13 +381,11 @@ template <typename T, int DP> struct Online {
 #pragma unroll
     for (int b = 0; b < NSUB; ++b) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[b][e] = __builtin_amdgcn_exp2f(fmaf(s[b][e], scale2, -ms));
-        l += s[b][e];
-      }
+      for (int e = 0; e < 16; ++e) s[b][e] = __builtin_amdgcn_exp2f(fmaf(s[b][e], scale2, -ms));
 #pragma unroll
       for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
         const frag p = Mma<T>::pack(s[b], st);
+        l = Mma<T>::add(p, l);   // of P as it is multiplied
 #pragma unroll
         for (int d = 0; d < I::ND; ++d) o[d] = Mma<T>::mma(im.col_frag(vimg, 32 * b, st, d), p, o[d]);
       }
@@ -403,7 +421,7 @@ __device__ __forceinline__ void store_col(T* p, const f16_t (&o)[ND], float f, i
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int c = 32 * d + 8 * g + 4 * (lane >> 5);
-      if (c < D) store4<T>(p + c, o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
+      if (32 * ND == D || c < D) store4<T>(p + c, o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
     }
 }
 
@@ -418,7 +436,7 @@ __device__ __forceinline__ void store_col_rest(bf16_t* p, const f16_t (&o)[ND], 
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int c = 32 * d + 8 * g + 4 * (lane >> 5);
-      if (c < D) store4_rest(p + c, o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
+      if (32 * ND == D || c < D) store4_rest(p + c, o[d][4 * g] * f, o[d][4 * g + 1] * f, o[d][4 * g + 2] * f, o[d][4 * g + 3] * f);
     }
 }
 
@@ -476,24 +494,21 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
   Online<T, DP> st;
   st.init();
   if (it0 < it1) {
-    dma.issue(kbase, a.kt, tl[it0] * KT, wg.lo, wg.hi, wg.sl, smem, wave);
-    dma.issue(vbase, a.vt, tl[it0] * KT, wg.lo, wg.hi, wg.sl, smem + I::BYTES, wave);
+    dma.issue(kbase, a.kt, tl[it0] * KT, wg.lo, wg.hi, wg.sl, lds_addr(smem), wave);
+    dma.issue(vbase, a.vt, tl[it0] * KT, wg.lo, wg.hi, wg.sl, lds_addr(smem) + I::BYTES, wave);
   }
   for (int it = it0; it < it1; ++it) {
     char* cur = smem + ((it - it0) & 1) * 2 * I::BYTES;
-    char* nxt = smem + ((it - it0 + 1) & 1) * 2 * I::BYTES;
+    const unsigned nxt = lds_addr(smem) + ((it - it0 + 1) & 1) * 2 * I::BYTES;
+    wait_vm<0>();
+    lds_barrier();   // this tile is there, and every wave is done with the other buffer
     if (it + 1 < it1) {
       dma.issue(kbase, a.kt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt, wave);
       dma.issue(vbase, a.vt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt + I::BYTES, wave);
-      wait_vm<2 * KeyDma<T, DP, KT, 4>::NI>();
-    } else {
-      wait_vm<0>();
     }
-    lds_barrier();
     const int key0 = tl[it] * KT;
     if (sees_any(my, key0, key0 + KT))
       st.template step<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane);
-    lds_barrier();   // every wave is done with this buffer before it is filled again
   }
   const float lsum = st.l + __shfl_xor(st.l, 32, 64);
   finish_row<T, DP>(a, bh, split, r, st.o, st.m, lsum, lane);
@@ -539,13 +554,13 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
   Online<T, DP> st;
   st.init();
   if (it0 < it1) {
-    dma.issue(kbase, a.kt, tl[it0] * KT, my.lo, my.hi, my.sl, ring, 0);
-    dma.issue(vbase, a.vt, tl[it0] * KT, my.lo, my.hi, my.sl, ring + IB, 0);
+    dma.issue(kbase, a.kt, tl[it0] * KT, my.lo, my.hi, my.sl, lds_addr(ring), 0);
+    dma.issue(vbase, a.vt, tl[it0] * KT, my.lo, my.hi, my.sl, lds_addr(ring) + IB, 0);
   }
   int cur = 0;
   for (int it = it0; it < it1; it += 4, cur = (cur + 1) % STG) {
     char* c = ring + cur * 2 * IB;
-    char* n = ring + (cur + 1) % STG * 2 * IB;
+    const unsigned n = lds_addr(ring) + (cur + 1) % STG * 2 * IB;
     if (STG == 2 && it + 4 < it1) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the reads of the buffer filled next are done
       dma.issue(kbase, a.kt, tl[it + 4] * KT, my.lo, my.hi, my.sl, n, 0);
@@ -749,52 +764,54 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
     }
   };
   if (tl.n > 0) {
-    dma.issue(kbase, a.kt, tl[0] * KT, wg.lo, wg.hi, wg.sl, smem, wave);
-    dma.issue(vbase, a.vt, tl[0] * KT, wg.lo, wg.hi, wg.sl, smem + I::BYTES, wave);
+    dma.issue(kbase, a.kt, tl[0] * KT, wg.lo, wg.hi, wg.sl, lds_addr(smem), wave);
+    dma.issue(vbase, a.vt, tl[0] * KT, wg.lo, wg.hi, wg.sl, lds_addr(smem) + I::BYTES, wave);
   }
   for (int it = 0; it < tl.n; ++it) {
     char* cur = smem + (it & 1) * 2 * I::BYTES;
-    char* nxt = smem + ((it + 1) & 1) * 2 * I::BYTES;
+    const unsigned nxt = lds_addr(smem) + ((it + 1) & 1) * 2 * I::BYTES;
+    wait_vm<0>();
+    lds_barrier();
     if (it + 1 < tl.n) {
       dma.issue(kbase, a.kt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt, wave);
       dma.issue(vbase, a.vt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt + I::BYTES, wave);
-      wait_vm<2 * KeyDma<T, DP, KT, 4>::NI>();
-    } else {
-      wait_vm<0>();
     }
-    lds_barrier();
     const int key0 = tl[it] * KT;
     if (sees_any(my, key0, key0 + KT)) body(cur, key0, !sees_all(a, seq, my, key0, key0 + KT));
-    lds_barrier();
   }
   if (r < a.R) store_col<T, I::ND>((T*)a.dq + orow, dq, a.scale, a.D, lane);
 }
 
 // ============================================================================ backward: dK, dV
 // 128 keys per workgroup, 32 per wave (lane column = key); row tiles of Q and dO double-buffered in
-// LDS.  A key tile that holds sinks is seen by every later row: its rows are split over csink
+// LDS.  bf16: eight waves, two for each 32 keys, which take the two 32-row halves of a tile and add up
+// at the end through LDS.  A key tile that holds sinks is seen by every later row: its rows are split over csink
 // workgroups (cwin for the others), whose fp32 parts wattn_dkv_join adds in order.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wattn_dkv_kernel(const WArgs a) {
+__global__ void __launch_bounds__(sizeof(T) == 2 ? 512 : 256, sizeof(T) == 4 && DP > 64 ? 1 : 2) wattn_dkv_kernel(const WArgs a) {
   typedef Img<T, DP> I;
   typedef typename I::frag frag;
-  // bf16 heads wider than 64: K (32 registers) stays in LDS and row tiles are 32 high, so that two
-  // waves fit on a SIMD beside the 128 accumulators
+  // bf16 heads wider than 64: K (32 registers) stays in LDS, so that two waves fit on a SIMD beside the
+  // 128 accumulators
   constexpr bool KLDS = sizeof(T) == 2 && DP > 64;
-  constexpr int RT = KLDS ? 32 : I::ROWS, RB = RT * I::PITCH;
-  constexpr int NI = RT * I::CPR / 64 / 4;
-  __shared__ __attribute__((aligned(256))) char smem[4 * RB + (KLDS ? 128 * I::PITCH : 0)];
+  constexpr int NW = sizeof(T) == 2 ? 8 : 4;
+  constexpr int RT = I::ROWS, RB = RT * I::PITCH;
+  constexpr int NI = RT * I::CPR / 64 / NW;
+  constexpr int OUT = NW == 8 ? 4 * 64 * (DP / 2) * 4 : 0;   // one wave's dK or dV, four times
+  constexpr int MAIN = 4 * RB + (KLDS ? 128 * I::PITCH : 0);
+  __shared__ __attribute__((aligned(256))) char smem[MAIN > OUT ? MAIN : OUT];
   __shared__ __attribute__((aligned(16))) float s_l[2][RT], s_d[2][RT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int items = a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin;
-  const int L = xcd_remap(blockIdx.x, items * a.B * a.Hk);
+  // the tiles without sinks come first: they are the longest, and the others' short chunks fill the end
+  const int nwin = (a.tiles - a.nsink) * a.cwin, nsnk = a.nsink * a.csink, items = nwin + nsnk;
+  const int BH = a.B * a.Hk, id = blockIdx.x < xcd_pad(nwin * BH) ? 0 : 1;
+  const int L = xcd_remap(blockIdx.x - (id ? xcd_pad(nwin * BH) : 0), (id ? nsnk : nwin) * BH);
   if (L < 0) return;
-  const int item = L % items, bh = L / items;
+  const bool sink = id == 1;
+  const int nch = sink ? a.csink : a.cwin, of = sink ? nsnk : nwin;
+  const int bh = L / of, kt = (L % of) / nch + (sink ? 0 : a.nsink), ch = (L % of) % nch;
+  const int item = L % of + (sink ? nwin : 0);
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
-  const bool sink = item < a.nsink * a.csink;
-  const int nch = sink ? a.csink : a.cwin;
-  const int kt = sink ? item / a.csink : a.nsink + (item - a.nsink * a.csink) / a.cwin;
-  const int ch = sink ? item % a.csink : (item - a.nsink * a.csink) % a.cwin;
   const Seq seq = seq_of(a, b);
   const int k0 = kt * 128, k1 = min(k0 + 128, seq.len);
 
@@ -813,16 +830,17 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
   const int n = i1 - i0;
   const int c0 = i0 + (int)((int64_t)n * ch / nch), c1 = i0 + (int)((int64_t)n * (ch + 1) / nch);
 
-  const int kw = k0 + wave * 32, key = kw + (lane & 31);
+  const int kb = wave & 3, half = wave >> 2;
+  const int kw = k0 + kb * 32, key = kw + (lane & 31);
   const bool kok = key < seq.len;
   frag kf[KLDS ? 1 : I::NS], vf[I::NS];
   const char* kimg = smem + 4 * RB;
   {
     const int kk = min(key, a.M - 1);
     if constexpr (KLDS) {
-      KeyDma<T, DP, 128, 4> dma;
+      KeyDma<T, DP, 128, NW> dma;
       dma.init(wave, lane, a.D);
-      if (k0 < seq.len) dma.issue((const char*)a.k + b * a.kb + hk * a.kh, a.kt, k0, 0, seq.len, 0, smem + 4 * RB, wave);
+      if (k0 < seq.len) dma.issue((const char*)a.k + b * a.kb + hk * a.kh, a.kt, k0, 0, seq.len, 0, lds_addr(smem) + 4 * RB, wave);
     } else {
       load_frags<T, DP>((const char*)a.k + b * a.kb + (int64_t)kk * a.kt + hk * a.kh, kok, a.D, lane, kf);
     }
@@ -857,7 +875,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
   unsigned dch[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int c = (i * 4 + wave) * 64 + lane;
+    const int c = (i * NW + wave) * 64 + lane;
     drow[i] = c / I::CPR;
     const int cc = (c % I::CPR) ^ I::swz(drow[i]);
     dch[i] = cc * 16 < a.D * I::ES ? (unsigned)cc * 16 : kOob;
@@ -865,15 +883,15 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
   const char* qbase = (const char*)a.q + b * a.qb + hk * a.G * a.qh;
   const char* obase = (const char*)a.dO + b * a.ob + hk * a.G * a.oh;
   const int rlim = min(seq.len * a.G, a.R);   // live rows
-  auto issue = [&](int tile, char* img) {
+  auto issue = [&](int tile, unsigned img) {
     const int r0 = tile * RT, t0 = dm_div(a.dmG, r0);
     const i4_t rq = make_rsrc(qbase + t0 * a.qt), ro = make_rsrc(obase + t0 * a.ot);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = r0 + drow[i], t = dm_div(a.dmG, r), g = r - t * a.G;
       const unsigned bad = (r < rlim ? 0u : kOob) | (dch[i] & kOob);
-      dma16(rq, bad | (dch[i] + (unsigned)((t - t0) * (int)a.qt + g * (int)a.qh)), img + (i * 4 + wave) * 1024);
-      dma16(ro, bad | (dch[i] + (unsigned)((t - t0) * (int)a.ot + g * (int)a.oh)), img + RB + (i * 4 + wave) * 1024);
+      dma16(rq, bad | (dch[i] + (unsigned)((t - t0) * (int)a.qt + g * (int)a.qh)), img + (i * NW + wave) * 1024);
+      dma16(ro, bad | (dch[i] + (unsigned)((t - t0) * (int)a.ot + g * (int)a.oh)), img + RB + (i * NW + wave) * 1024);
     }
   };
   const float* lbase = a.lse + (int64_t)bh * a.R;
@@ -894,14 +912,14 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
   for (int d = 0; d < I::ND; ++d) dk[d] = dv[d] = zero16();
   I im;
   im.init(lane);
-  auto body = [&](const char* cur, int buf, int r0, bool masked) {
-#pragma unroll 1
-    for (int rb = 0; rb < RT / 32; ++rb) {
+  auto body = [&](const char* cur, int buf, int r0, bool masked) {   // rows r0 .. r0 + 31, image row 32 half
+    const int rb = NW == 8 ? half : 0;
+    {
       f16_t s = zero16(), dp = zero16();
 #pragma unroll
       for (int st = 0; st < I::NS; ++st) {
         frag kk;
-        if constexpr (KLDS) kk = im.row_frag(kimg + wave * 32 * I::PITCH, 0, st);
+        if constexpr (KLDS) kk = im.row_frag(kimg + kb * 32 * I::PITCH, 0, st);
         else kk = kf[st];
         s = Mma<T>::mma(im.row_frag(cur, 32 * rb, st), kk, s);
       }
@@ -919,7 +937,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
       }
       if (masked) {
         asm volatile("");
-        const int rr = r0 + 32 * rb + 4 * (lane >> 5), ge = vlo - rr, lt = vhi - rr;
+        const int rr = r0 + 4 * (lane >> 5), ge = vlo - rr, lt = vhi - rr;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int c = 8 * (e >> 2) + (e & 3);
@@ -942,27 +960,52 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
 
   if (c0 < c1) {
     put(stat(c0), 0);
-    issue(c0, smem);
+    issue(c0, lds_addr(smem));
   }
   for (int it = c0; it < c1; ++it) {
     const int buf = (it - c0) & 1;
     char* cur = smem + buf * 2 * RB;
+    wait_vm<0>();
+    lds_barrier();
     float nx = 0.f;
     const bool more = it + 1 < c1;
     if (more) {
       nx = stat(it + 1);
-      issue(it + 1, smem + (buf ^ 1) * 2 * RB);
-      wait_vm<2 * NI>();   // all but the DMAs just issued
-    } else {
-      wait_vm<0>();
+      issue(it + 1, lds_addr(smem) + (buf ^ 1) * 2 * RB);
     }
-    lds_barrier();
-    const int r0 = it * RT;
-    if (r0 < nhi && r0 + RT > nlo) {
-      body(cur, buf, r0, r0 < alo || r0 + RT > ahi);
-    }
+    const int r0 = it * RT + (NW == 8 ? 32 * half : 0);
+    if (r0 < nhi && r0 + 32 > nlo) body(cur, buf, r0, r0 < alo || r0 + 32 > ahi);
     if (more) put(nx, buf ^ 1);
-    lds_barrier();
+  }
+  wait_vm<0>();   // K's DMA, where no row tile waited for it
+  __syncthreads();
+  if constexpr (NW == 8) {
+    // the second half's sums: [register group of 4][lane] in LDS, dK then dV
+    float* x = (float*)smem + kb * 64 * (DP / 2) + lane * 4;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      f16_t(&acc)[I::ND] = pass ? dv : dk;
+      if (half == 1)
+#pragma unroll
+        for (int d = 0; d < I::ND; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *(float4*)(x + (d * 4 + g) * 256) = make_float4(acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]);
+      __syncthreads();
+      if (half == 0)
+#pragma unroll
+        for (int d = 0; d < I::ND; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 v = *(const float4*)(x + (d * 4 + g) * 256);
+            acc[d][4 * g] += v.x;
+            acc[d][4 * g + 1] += v.y;
+            acc[d][4 * g + 2] += v.z;
+            acc[d][4 * g + 3] += v.w;
+          }
+      __syncthreads();
+    }
+    if (half == 1) return;
   }
   if (key >= a.M) return;
   if (nch == 1) {
@@ -970,7 +1013,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
     store_col<T, I::ND>((T*)a.dk + o, dk, a.scale, a.D, lane);
     store_col<T, I::ND>((T*)a.dv + o, dv, 1.f, a.D, lane);
   } else {
-    float* p = a.part + (((int64_t)bh * items + item) * 128 + wave * 32 + (lane & 31)) * 2 * a.D;
+    float* p = a.part + (((int64_t)bh * items + item) * 128 + kb * 32 + (lane & 31)) * 2 * a.D;
     store_col<float, I::ND>(p, dk, a.scale, a.D, lane);
     store_col<float, I::ND>(p + a.D, dv, 1.f, a.D, lane);
   }
@@ -988,8 +1031,8 @@ __global__ void __launch_bounds__(256) wattn_dkv_join_kernel(const WArgs a, int 
   const int key = kt * 128 + kl;
   if (key >= a.M) return;
   const bool sink = kt < a.nsink;
-  const int nch = sink ? a.csink : a.cwin, items = a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin;
-  const int item = sink ? kt * a.csink : a.nsink * a.csink + (kt - a.nsink) * a.cwin;
+  const int nwin = (a.tiles - a.nsink) * a.cwin, nch = sink ? a.csink : a.cwin, items = nwin + a.nsink * a.csink;
+  const int item = sink ? nwin + kt * a.csink : (kt - a.nsink) * a.cwin;
   const float* p = a.part + (((int64_t)bh * items + item) * 128 + kl) * 2 * a.D + c;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < nch; ++i) {
@@ -1075,38 +1118,53 @@ void plan_fwd(WArgs& a, bool& few) {
 }
 int64_t fwd_work(const WArgs& a) { return a.splits == 1 ? 0 : (int64_t)a.splits * a.B * a.Hk * a.R * (a.D + 1); }
 
-// The backward's key tiles, and the row chunks of those that many rows see: chunks of about the rows
-// that an ordinary tile has, more where the tiles alone do not fill the card.
-void plan_bwd(WArgs& a) {
+// The backward's key tiles, and how many chunks their rows are split into.  A tile without sinks has
+// `win` rows; more chunks than workgroups that run at once cost a second round of them all, too few
+// leave CUs idle, and more than one chunk costs the fp32 parts' way to memory and back.  Estimated in
+// microseconds: a row tile is 2 (bf16, width 128; 64 x 128 pairs) or 8 (fp32, 32 x 128), a workgroup
+// starts and ends in 4 of them, the parts move at 5 TB/s behind a 4 us launch.  Measured at 8192 tokens,
+// 16 / 4 heads of 128, window 1024, 4 sinks: 63 x 4 long workgroups in one round.
+// A tile with sinks has all rows, but only the waves with sinks work on most of them: shorter chunks.
+void plan_bwd(WArgs& a, bool f32) {
   a.tiles = (a.M + 127) / 128;
   a.nsink = (a.sinks + 127) / 128;
-  const int bh = a.B * a.Hk;
-  const int rt = 32;
+  const int64_t bh = (int64_t)a.B * a.Hk, rt = f32 ? 32 : 64;
+  const int slots = f32 && a.D <= 64 ? 512 : 256;
+  const double tile = (f32 ? 8.0 : 2.0) * std::max(a.D, 32) / 128;
   const int64_t win = std::min<int64_t>(a.M, (int64_t)a.window * (a.causal ? 1 : 2) + 127) * a.G;
-  const int64_t all = (int64_t)a.M * a.G;
-  const int64_t want = std::max<int64_t>(1, 256 / std::max(1, a.tiles * bh));
-  a.cwin = (int)std::max<int64_t>(1, std::min(want, win / (4 * rt)));
-  const int64_t rows = std::max<int64_t>(win / a.cwin, 4 * rt);
-  a.csink = (int)std::max<int64_t>(1, std::min<int64_t>((all + rows - 1) / rows, 256));
+  const int64_t wt = (win + rt - 1) / rt, all = ((int64_t)a.M * a.G + rt - 1) / rt;
+  double best = 0;
+  a.cwin = 1;
+  for (int c = 1; c <= 8 && c <= std::max<int64_t>(1, wt / 2); ++c) {
+    const double rounds = (double)(((int64_t)std::max(1, a.tiles - a.nsink) * bh * c + slots - 1) / slots);
+    double t = rounds * ((double)((wt + c - 1) / c) + 4) * tile;
+    if (c > 1) t += 4 + (double)c * a.M * bh * a.D * 16 / 5e6;
+    if (c == 1 || t < best) {
+      best = t;
+      a.cwin = c;
+    }
+  }
+  const int64_t rows = std::max<int64_t>((wt / a.cwin + 3) / 4, 4);
+  a.csink = all <= wt ? a.cwin : (int)std::min<int64_t>((all + rows - 1) / rows, 256);
 }
 int64_t bwd_work(const WArgs& a) {
   if (a.csink == 1 && a.cwin == 1) return 0;
   return (int64_t)(a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin) * a.B * a.Hk * 128 * 2 * a.D;
 }
 
-#define BY_WIDTH(KERNEL, GRID, ...)                                                                      \
-  do {                                                                                                   \
-    if (a.D <= 32) hipLaunchKernelGGL((KERNEL<T, 32>), GRID, dim3(256), 0, st, __VA_ARGS__);             \
-    else if (a.D <= 64) hipLaunchKernelGGL((KERNEL<T, 64>), GRID, dim3(256), 0, st, __VA_ARGS__);        \
-    else if (a.D <= 96) hipLaunchKernelGGL((KERNEL<T, 96>), GRID, dim3(256), 0, st, __VA_ARGS__);        \
-    else hipLaunchKernelGGL((KERNEL<T, 128>), GRID, dim3(256), 0, st, __VA_ARGS__);                      \
+#define BY_WIDTH(KERNEL, GRID, THREADS, ARGS)                                                        \
+  do {                                                                                               \
+    if (a.D <= 32) hipLaunchKernelGGL((KERNEL<T, 32>), GRID, dim3(THREADS), 0, st, ARGS);            \
+    else if (a.D <= 64) hipLaunchKernelGGL((KERNEL<T, 64>), GRID, dim3(THREADS), 0, st, ARGS);       \
+    else if (a.D <= 96) hipLaunchKernelGGL((KERNEL<T, 96>), GRID, dim3(THREADS), 0, st, ARGS);       \
+    else hipLaunchKernelGGL((KERNEL<T, 128>), GRID, dim3(THREADS), 0, st, ARGS);                     \
   } while (0)
 
 template <typename T>
 int run_fwd(const WArgs& a, bool few, hipStream_t st) {
   const dim3 grid((unsigned)xcd_pad(a.tiles * a.B * a.Hk * a.splits));
-  if (few) BY_WIDTH(wattn_few_kernel, grid, a);
-  else BY_WIDTH(wattn_fwd_kernel, grid, a);
+  if (few) BY_WIDTH(wattn_few_kernel, grid, 256, a);
+  else BY_WIDTH(wattn_fwd_kernel, grid, 256, a);
   DFCSA_CHECK_LAUNCH();
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.B * a.Hk * a.R;
@@ -1121,11 +1179,11 @@ int run_bwd(WArgs a, hipStream_t st) {
   q.tiles = (a.R + 127) / 128;
   {
     const WArgs& a = q;
-    BY_WIDTH(wattn_dq_kernel, dim3((unsigned)xcd_pad(a.tiles * a.B * a.Hk)), a);
+    BY_WIDTH(wattn_dq_kernel, dim3((unsigned)xcd_pad(a.tiles * a.B * a.Hk)), 256, a);
   }
   DFCSA_CHECK_LAUNCH();
-  const int items = a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin;
-  BY_WIDTH(wattn_dkv_kernel, dim3((unsigned)xcd_pad(items * a.B * a.Hk)), a);
+  const int bh = a.B * a.Hk;
+  BY_WIDTH(wattn_dkv_kernel, dim3((unsigned)(xcd_pad((a.tiles - a.nsink) * a.cwin * bh) + xcd_pad(a.nsink * a.csink * bh))), sizeof(T) == 2 ? 512 : 256, a);
   DFCSA_CHECK_LAUNCH();
   const int t0 = a.csink > 1 ? 0 : a.nsink, t1 = a.cwin > 1 ? a.tiles : a.nsink;
   if (t1 > t0) {
@@ -1144,7 +1202,7 @@ int dfcsa_wattn_work_floats(const dfcsa_wattn_desc* d, int backward, int64_t* fl
   WArgs a;
   if (!floats || !fill(d, a, backward != 0)) return DFCSA_EINVAL;
   if (backward) {
-    plan_bwd(a);
+    plan_bwd(a, d->dtype == DFCSA_DT_F32);
     *floats = bwd_work(a);
   } else {
     bool few;
@@ -1167,7 +1225,7 @@ int dfcsa_wattn_fwd(const dfcsa_wattn_desc* d, void* stream) {
 int dfcsa_wattn_bwd(const dfcsa_wattn_desc* d, void* stream) {
   WArgs a;
   if (!fill(d, a, true)) return DFCSA_EINVAL;
-  plan_bwd(a);
+  plan_bwd(a, d->dtype == DFCSA_DT_F32);
   if ((int64_t)(a.nsink * a.csink + a.tiles * a.cwin) * a.B * a.Hk > 0x7ffffff0) return DFCSA_EINVAL;
   if (bwd_work(a) > 0 && (!d->work || d->work_floats < bwd_work(a))) return DFCSA_EINVAL;
   return d->dtype == DFCSA_DT_F32 ? run_bwd<float>(a, (hipStream_t)stream) : run_bwd<bf16_t>(a, (hipStream_t)stream);

@@ -51,6 +51,13 @@ def test_serving_forms_refuse_gradients():
         tk.window_attention_cached(q, q, q, torch.ones(1, dtype=torch.int32), 2)
 
 
+@pytest.mark.parametrize("axes,base", [((), 1e4), ((1,) * 5, 1e4), ((4, 0), 1e4), ((300,), 1e4), ((200, 200), 1e4),
+                                       ((4.5,), 1e4), ((4,), 0.5), ((4,), float("inf")), ((4,), float("nan"))])
+def test_rotary_table_refusals(axes, base):
+    with pytest.raises(ValueError):
+        tk._turn_table(axes, base, False)
+
+
 P16 = 1 << 20   # an aligned address that nothing reads: every call below is refused before a launch
 
 
@@ -76,7 +83,7 @@ def test_norm_backward_needs_its_workspace():
 
 
 def rotary_desc(**over):
-    turns, axis = tk._turn_table((4, 4), 10000.0, False)
+    turns, axis = (ctypes.c_double * 8)(*[0.1] * 8), (ctypes.c_ubyte * 8)(*[0] * 4 + [1] * 4)
     d = _lib.RotaryDesc(dtype=1, B=1, N=4, D=16, npairs=8, naxes=2, positions=P16, pos_sb=8, pos_sn=2, pos_sa=1,
                         turns=ctypes.addressof(turns), axis=ctypes.addressof(axis))
     d.keep = (turns, axis)
