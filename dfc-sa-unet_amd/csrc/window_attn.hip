@@ -66,12 +66,19 @@ struct WArgs {
   int64_t ob, ot, oh;    // dO strides, bytes
   float* delta;
   void *dq, *dk, *dv;
-  int nsink, csink, cwin;   // key tiles with sinks, and row chunks of those and of the other tiles
+  int nsink, cwin;       // key tiles with sinks; row chunks of a key tile
+  int far32, cfar;       // blocks of 32 sinks, and chunks of the rows beyond the window that see them (0: none)
 };
 
 // two values to bf16 in one instruction
 __device__ __forceinline__ uint32_t cvt2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, bh2_t));
+}
+
+// the far rows' parts lie behind the window's (floats)
+__device__ __host__ __forceinline__ int64_t far_at(const WArgs& a) {
+  const int64_t items = a.cwin > 1 ? (int64_t)a.tiles * a.cwin : (a.cfar ? a.nsink : 0);
+  return items * a.B * a.Hk * 128 * 2 * a.D;
 }
 
 // ------------------------------------------------------------------ matrix instructions
@@ -822,17 +829,29 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
 
 // ============================================================================ backward: dK, dV
 // 128 keys per workgroup, 32 per wave (lane column = key); row tiles of Q and dO double-buffered in
-// LDS.  bf16: eight waves, two for each 32 keys, which take the two 32-row halves of a tile and add up
-// at the end through LDS.  A key tile that holds sinks is seen by every later row: its rows are split over csink
-// workgroups (cwin for the others), whose fp32 parts wattn_dkv_join adds in order.
+// LDS.  bf16 wider than 64: eight waves, two for each 32 keys, which take the two 32-row halves of a
+// tile and add up at the end through LDS (one such workgroup fills a CU: measured 284 -> 225 us at 8192
+// tokens, 16 / 4 heads of 128, window 1024, against four waves with one tile per CU).
+// A workgroup takes the rows whose window reaches its keys, or one of cwin chunks of them; the rows
+// further away that see sinks are wattn_far_kernel's.  fp32 parts are added in order by wattn_dkv_join.
+__device__ __forceinline__ void key_rows(const WArgs& a, const Seq& seq, int kt, int rt, int& i0, int& i1) {
+  const int k0 = kt * 128, k1 = min(k0 + 128, seq.len);
+  const int p0 = a.causal ? k0 : max(k0 - a.window + 1, 0), p1 = min(k1 - 1 + a.window - 1, seq.len - 1);
+  i0 = i1 = 0;   // tiles of rt rows
+  if (k0 < k1 && p0 <= p1) {
+    i0 = p0 * a.G / rt;
+    i1 = ((p1 + 1) * a.G + rt - 1) / rt;
+  }
+}
+template <typename T, int DP> constexpr int dkv_waves() { return sizeof(T) == 2 && DP > 64 ? 8 : 4; }
 template <typename T, int DP>
-__global__ void __launch_bounds__(sizeof(T) == 2 ? 512 : 256, sizeof(T) == 4 && DP > 64 ? 1 : 2) wattn_dkv_kernel(const WArgs a) {
+__global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && DP > 64 ? 1 : 2) wattn_dkv_kernel(const WArgs a) {
   typedef Img<T, DP> I;
   typedef typename I::frag frag;
   // bf16 heads wider than 64: K (32 registers) stays in LDS, so that two waves fit on a SIMD beside the
   // 128 accumulators
   constexpr bool KLDS = sizeof(T) == 2 && DP > 64;
-  constexpr int NW = sizeof(T) == 2 ? 8 : 4;
+  constexpr int NW = dkv_waves<T, DP>();
   constexpr int RT = I::ROWS, RB = RT * I::PITCH;
   constexpr int NI = RT * I::CPR / 64 / NW;
   constexpr int OUT = NW == 8 ? 4 * 64 * (DP / 2) * 4 : 0;   // one wave's dK or dV, four times
@@ -840,33 +859,16 @@ __global__ void __launch_bounds__(sizeof(T) == 2 ? 512 : 256, sizeof(T) == 4 && 
   __shared__ __attribute__((aligned(256))) char smem[MAIN > OUT ? MAIN : OUT];
   __shared__ __attribute__((aligned(16))) float s_l[2][RT], s_d[2][RT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // the tiles without sinks come first: they are the longest, and the others' short chunks fill the end
-  const int nwin = (a.tiles - a.nsink) * a.cwin, nsnk = a.nsink * a.csink, items = nwin + nsnk;
-  const int BH = a.B * a.Hk, id = blockIdx.x < xcd_pad(nwin * BH) ? 0 : 1;
-  const int L = xcd_remap(blockIdx.x - (id ? xcd_pad(nwin * BH) : 0), (id ? nsnk : nwin) * BH);
+  const int L = xcd_remap(blockIdx.x, a.tiles * a.cwin * a.B * a.Hk);
   if (L < 0) return;
-  const bool sink = id == 1;
-  const int nch = sink ? a.csink : a.cwin, of = sink ? nsnk : nwin;
-  const int bh = L / of, kt = (L % of) / nch + (sink ? 0 : a.nsink), ch = (L % of) % nch;
-  const int item = L % of + (sink ? nwin : 0);
+  const int bh = L / (a.tiles * a.cwin), item = L % (a.tiles * a.cwin), kt = item / a.cwin, ch = item % a.cwin;
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const Seq seq = seq_of(a, b);
-  const int k0 = kt * 128, k1 = min(k0 + 128, seq.len);
-
-  // rows that see one of the keys: positions [p0, p1]
-  int p0 = a.causal ? k0 : max(k0 - a.window + 1, 0), p1 = min(k1 - 1 + a.window - 1, seq.len - 1);
-  if (k0 < a.sinks) {
-    if (!a.causal) p0 = 0;
-    p1 = seq.len - 1;
-  }
-  int i0 = 0, i1 = 0;   // row tiles
-  const int rbeg = p0 * a.G, rend = (p1 + 1) * a.G;
-  if (k0 < k1 && p0 <= p1) {
-    i0 = rbeg / RT;
-    i1 = (rend + RT - 1) / RT;
-  }
+  const int k0 = kt * 128;
+  int i0, i1;
+  key_rows(a, seq, kt, RT, i0, i1);
   const int n = i1 - i0;
-  const int c0 = i0 + (int)((int64_t)n * ch / nch), c1 = i0 + (int)((int64_t)n * (ch + 1) / nch);
+  const int c0 = i0 + (int)((int64_t)n * ch / a.cwin), c1 = i0 + (int)((int64_t)n * (ch + 1) / a.cwin);
 
   const int kb = wave & 3, half = wave >> 2;
   const int kw = k0 + kb * 32, key = kw + (lane & 31);
@@ -950,8 +952,7 @@ __global__ void __launch_bounds__(sizeof(T) == 2 ? 512 : 256, sizeof(T) == 4 && 
   for (int d = 0; d < I::ND; ++d) dk[d] = dv[d] = zero16();
   I im;
   im.init(lane);
-  auto body = [&](const char* cur, int buf, int r0, bool masked) {   // rows r0 .. r0 + 31, image row 32 half
-    const int rb = NW == 8 ? half : 0;
+  auto body = [&](const char* cur, int buf, int r0, int rb, bool masked) {   // rows r0 .., image rows 32 rb ..
     {
       f16_t s = zero16(), dp = zero16();
 #pragma unroll
@@ -1011,8 +1012,11 @@ __global__ void __launch_bounds__(sizeof(T) == 2 ? 512 : 256, sizeof(T) == 4 && 
       nx = stat(it + 1);
       issue(it + 1, lds_addr(smem) + (buf ^ 1) * 2 * RB);
     }
-    const int r0 = it * RT + (NW == 8 ? 32 * half : 0);
-    if (r0 < nhi && r0 + 32 > nlo) body(cur, buf, r0, r0 < alo || r0 + 32 > ahi);
+#pragma unroll 1
+    for (int rb = NW == 8 ? half : 0; rb < RT / 32; rb += NW == 8 ? 2 : 1) {
+      const int r0 = it * RT + 32 * rb;
+      if (r0 < nhi && r0 + 32 > nlo) body(cur, buf, r0, rb, r0 < alo || r0 + 32 > ahi);
+    }
     if (more) put(nx, buf ^ 1);
   }
   wait_vm<0>();   // K's DMA, where no row tile waited for it
@@ -1045,7 +1049,7 @@ __global__ void __launch_bounds__(sizeof(T) == 2 ? 512 : 256, sizeof(T) == 4 && 
     }
     if (half == 1) return;
   }
-  if (nch == 1) {
+  if (a.cwin == 1 && !(kt < a.nsink && a.cfar)) {
     char* lds = smem + kb * 32 * out_pitch<DP>();
     auto at = [&](void* p) {
       return [&, p](int i) { return kw + i < a.M ? (T*)p + (((int64_t)b * a.M + kw + i) * a.Hk + hk) * a.D : nullptr; };
@@ -1053,34 +1057,174 @@ __global__ void __launch_bounds__(sizeof(T) == 2 ? 512 : 256, sizeof(T) == 4 && 
     store_rows<T, DP, false>(lds, dk, a.scale, a.D, lane, at(a.dk));
     store_rows<T, DP, false>(lds, dv, 1.f, a.D, lane, at(a.dv));
   } else if (key < a.M) {
+    const int items = a.cwin > 1 ? a.tiles * a.cwin : a.nsink;   // as in the join
     float* p = a.part + (((int64_t)bh * items + item) * 128 + kb * 32 + (lane & 31)) * 2 * a.D;
     store_col<float, I::ND>(p, dk, a.scale, a.D, lane);
     store_col<float, I::ND>(p + a.D, dv, 1.f, a.D, lane);
   }
 }
 
-// dK and dV of the key tiles whose rows were split: their chunks added in order.  One 4-column piece
-// of dK or dV per thread.
+// Rows beyond the window of the sinks' key tiles: they see `sinks` keys only.  A workgroup has one block
+// of 32 sink keys (a.far32 of them) and one of cfar chunks of the rows; each wave runs through its own
+// row blocks with its own LDS ring, without barriers; the waves' sums are added at the end into part.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
+  typedef Img<T, DP> I;
+  typedef typename I::frag frag;
+  constexpr int RB = 32 * I::PITCH, STG = RB <= 8192 ? 2 : 1, RING = STG * 2 * RB;
+  constexpr int NI = RB / 1024;
+  static_assert(RING >= 64 * DP * 4, "the sums fit a wave's ring");
+  constexpr int RT = I::ROWS;   // as wattn_dkv_kernel
+  __shared__ __attribute__((aligned(256))) char smem[4 * RING];
+  __shared__ __attribute__((aligned(16))) float s_st[4][64];   // lse, delta of the block
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int L = xcd_remap(blockIdx.x, a.far32 * a.cfar * a.B * a.Hk);
+  if (L < 0) return;
+  const int ch = L % a.cfar, sb = L / a.cfar % a.far32, bh = L / (a.cfar * a.far32);
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const Seq seq = seq_of(a, b);
+  const int rlim = min(seq.len * a.G, a.R);   // live rows
+  int i0, i1;
+  key_rows(a, seq, sb / 4, RT, i0, i1);
+  // row blocks [0, nlo) (causal: those rows come before the keys) and [hi0, hi0 + nhi)
+  const int kw = sb * 32, key = kw + (lane & 31);
+  const int nlo = a.causal || i0 == i1 ? 0 : i0 * (RT / 32);
+  const int hi0 = i1 * (RT / 32), nhi = i0 == i1 ? 0 : max((rlim + 31) / 32 - hi0, 0);
+  const int nb = kw < seq.len ? nlo + nhi : 0;
+  const int c0 = (int)((int64_t)nb * ch / a.cfar) + wave, c1 = (int)((int64_t)nb * (ch + 1) / a.cfar);
+  const bool kok = key < seq.len && key < a.sinks;
+
+  frag kf[I::NS], vf[I::NS];
+  {
+    const int kk = min(key, a.M - 1);
+    load_frags<T, DP>((const char*)a.k + b * a.kb + (int64_t)kk * a.kt + hk * a.kh, kok, a.D, lane, kf);
+    load_frags<T, DP>((const char*)a.v + b * a.vb + (int64_t)kk * a.vt + hk * a.vh, kok, a.D, lane, vf);
+  }
+  const char* qbase = (const char*)a.q + b * a.qb + hk * a.G * a.qh;
+  const char* obase = (const char*)a.dO + b * a.ob + hk * a.G * a.oh;
+  char* ring = smem + wave * RING;
+  auto row_of = [&](int i) { return (i < nlo ? i : hi0 + i - nlo) * 32; };
+  float st_v = 0.f;   // lanes [0, 32): lse of the block in flight, [32, 64): delta
+  auto issue = [&](int i, unsigned img) {
+    const int r0 = row_of(i), t0 = dm_div(a.dmG, r0);
+    const int rs = r0 + (lane & 31);
+    st_v = lane < 32 ? __builtin_inff() : 0.f;   // exp2(. - inf) = 0
+    if (rs < rlim) st_v = (lane < 32 ? a.lse : a.delta)[(int64_t)bh * a.R + rs];
+    const i4_t rq = make_rsrc(qbase + t0 * a.qt), ro = make_rsrc(obase + t0 * a.ot);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int c = j * 64 + lane, row = c / I::CPR, cc = (c % I::CPR) ^ I::swz(row);
+      const int r = r0 + row, t = dm_div(a.dmG, r), g = r - t * a.G;
+      const unsigned bad = r < rlim && cc * 16 < a.D * I::ES ? 0u : kOob;
+      dma16(rq, bad | (unsigned)(cc * 16 + (t - t0) * (int)a.qt + g * (int)a.qh), img + j * 1024);
+      dma16(ro, bad | (unsigned)(cc * 16 + (t - t0) * (int)a.ot + g * (int)a.oh), img + RB + j * 1024);
+    }
+  };
+  f16_t dk[I::ND], dv[I::ND];
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d) dk[d] = dv[d] = zero16();
+  I im;
+  im.init(lane);
+  if (c0 < c1) issue(c0, lds_addr(ring));
+  int cur = 0;
+  for (int i = c0; i < c1; i += 4, cur = (cur + 1) % STG) {
+    const char* q = ring + cur * 2 * RB;
+    const unsigned nx = lds_addr(ring) + (cur + 1) % STG * 2 * RB;
+    wait_vm<0>();   // this block is there (the wave has the other one in flight only from here on)
+    s_st[wave][lane] = st_v;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // and the reads of the buffer filled next are done
+    if (STG == 2 && i + 4 < c1) issue(i + 4, nx);
+    f16_t s = zero16(), dp = zero16();
+#pragma unroll
+    for (int st = 0; st < I::NS; ++st) s = Mma<T>::mma(im.row_frag(q, 0, st), kf[st], s);
+#pragma unroll
+    for (int st = 0; st < I::NS; ++st) dp = Mma<T>::mma(im.row_frag(q + RB, 0, st), vf[st], dp);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f4_t l4 = *(const f4_t*)&s_st[wave][8 * g + 4 * (lane >> 5)], d4 = *(const f4_t*)&s_st[wave][32 + 8 * g + 4 * (lane >> 5)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {   // every live row sees the lane's key if it is a sink: a select for the others
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale2, -l4[e]));
+        dp[4 * g + e] = kok ? p * (dp[4 * g + e] - d4[e]) : 0.f;
+        s[4 * g + e] = kok ? p : 0.f;
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+      const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
+#pragma unroll
+      for (int d = 0; d < I::ND; ++d) {
+        dv[d] = Mma<T>::mma(im.col_frag(q + RB, 0, st, d), pf, dv[d]);
+        dk[d] = Mma<T>::mma(im.col_frag(q, 0, st, d), df, dk[d]);
+      }
+    }
+    if (STG == 1 && i + 4 < c1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      issue(i + 4, nx);
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  float* x = (float*)ring + lane * 4;   // [dK, dV][register group of 4][lane]
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      *(float4*)(x + (d * 4 + g) * 256) = make_float4(dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]);
+      *(float4*)(x + ((I::ND + d) * 4 + g) * 256) = make_float4(dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]);
+    }
+  __syncthreads();
+  float* out = a.part + far_at(a) + ((int64_t)bh * a.far32 * a.cfar + sb * a.cfar + ch) * 32 * 2 * a.D;
+  for (int e = threadIdx.x; e < 2 * I::ND * 4 * 64; e += 256) {
+    const int ln = e & 63, grp = e >> 6, which = grp / (I::ND * 4), c = grp % (I::ND * 4) * 8 + 4 * (ln >> 5);
+    float4 v = *(const float4*)((const float*)smem + e * 4);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 y = *(const float4*)((const float*)(smem + w * RING) + e * 4);
+      v.x += y.x;
+      v.y += y.y;
+      v.z += y.z;
+      v.w += y.w;
+    }
+    const float f = which ? 1.f : a.scale;
+    if (c < a.D) *(float4*)(out + (ln & 31) * 2 * a.D + which * a.D + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+  }
+}
+
+// dK and dV of the key tiles in parts: the window's chunks, then the far rows' (sinks only), in order.
+// One 4-column piece of dK or dV per thread.
 template <typename T>
-__global__ void __launch_bounds__(256) wattn_dkv_join_kernel(const WArgs a, int tile0, int ntile) {
-  const int q = 2 * a.D / 4;
+__global__ void __launch_bounds__(256) wattn_dkv_join_kernel(const WArgs a) {
+  const int q = 2 * a.D / 4, ntile = a.cwin > 1 ? a.tiles : a.nsink, items = ntile * a.cwin;
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (int64_t)ntile * 128 * q;
   if (e >= per * a.B * a.Hk) return;
   const int bh = (int)(e / per);
-  const int rem = (int)(e - bh * per), c = rem % q * 4, kl = rem / q % 128, kt = tile0 + rem / q / 128;
-  const int key = kt * 128 + kl;
+  const int64_t rem = e - bh * per;
+  const int c = (int)(rem % q) * 4, key = (int)(rem / q);
   if (key >= a.M) return;
-  const bool sink = kt < a.nsink;
-  const int nwin = (a.tiles - a.nsink) * a.cwin, nch = sink ? a.csink : a.cwin, items = nwin + a.nsink * a.csink;
-  const int item = sink ? nwin + kt * a.csink : (kt - a.nsink) * a.cwin;
-  const float* p = a.part + (((int64_t)bh * items + item) * 128 + kl) * 2 * a.D + c;
+  const float* p = a.part + (((int64_t)bh * items + key / 128 * a.cwin) * 128 + key % 128) * 2 * a.D + c;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < nch; ++i) {
+  for (int i = 0; i < a.cwin; ++i) {
     const float4 x = *(const float4*)(p + (int64_t)i * 128 * 2 * a.D);
     s[0] += x.x;
     s[1] += x.y;
     s[2] += x.z;
     s[3] += x.w;
+  }
+  if (a.cfar && key < a.sinks) {
+    const float* f = a.part + far_at(a) + (((int64_t)bh * a.far32 + key / 32) * a.cfar * 32 + key % 32) * 2 * a.D + c;
+    for (int i = 0; i < a.cfar; i += 4) {   // four in flight
+      float4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = *(const float4*)(f + (int64_t)min(i + j, a.cfar - 1) * 32 * 2 * a.D);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i + j >= a.cfar) break;
+        s[0] += x[j].x;
+        s[1] += x[j].y;
+        s[2] += x[j].z;
+        s[3] += x[j].w;
+      }
+    }
   }
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   T* dst = (T*)(c < a.D ? a.dk : a.dv) + (((int64_t)b * a.M + key) * a.Hk + hk) * a.D + (c < a.D ? c : c - a.D);
@@ -1088,8 +1232,6 @@ __global__ void __launch_bounds__(256) wattn_dkv_join_kernel(const WArgs a, int 
 }
 
 // ============================================================================ host
-constexpr int kWgs = 512;   // workgroups that fill the card: two per CU
-
 bool fill(const dfcsa_wattn_desc* d, WArgs& a, bool backward) {
   if (!d || (d->dtype != DFCSA_DT_F32 && d->dtype != DFCSA_DT_BF16)) return false;
   if (d->B <= 0 || d->T <= 0 || d->M <= 0 || d->H <= 0 || d->Hk <= 0 || d->H > 65536 || d->H % d->Hk || d->D < 8 || d->D % 8 ||
@@ -1132,7 +1274,7 @@ bool fill(const dfcsa_wattn_desc* d, WArgs& a, bool backward) {
   a.dO = d->dout; a.ob = a.ot = a.oh = 0;
   a.delta = d->delta;
   a.dq = d->dq; a.dk = d->dk; a.dv = d->dv;
-  a.nsink = a.csink = a.cwin = a.tiles = 0;
+  a.nsink = a.cwin = a.far32 = a.cfar = a.tiles = 0;
   if (backward) {
     a.ob = d->dout_stride[0] * es; a.ot = d->dout_stride[1] * es; a.oh = d->dout_stride[2] * es;
     if (!d->lse || !d->delta || !d->dq || !d->dk || !d->dv) return false;
@@ -1141,8 +1283,11 @@ bool fill(const dfcsa_wattn_desc* d, WArgs& a, bool backward) {
 }
 
 // The forward's plan: few = the kernel whose waves split the keys of 32 rows; splits over the keys
-// where the row tiles alone do not fill the card.
-void plan_fwd(WArgs& a, bool& few) {
+// where the row tiles alone do not fill the card.  The estimate is in rounds of the waves (few: 128
+// keys, else a tile of 64 or 32), 3 of which a workgroup takes to start and end, and the join about as
+// long as 3: workgroups beyond one for each CU share it (wide and fp32 ones: the LDS or the matrix
+// unit is then full, so two take twice as long; else two run in 1.4 times the time of one).
+void plan_fwd(WArgs& a, bool f32, bool& few) {
   const int bh = a.B * a.Hk;
   few = a.R <= 64;
   a.tiles = few ? (a.R + 31) / 32 : (a.R + 127) / 128;
@@ -1150,33 +1295,39 @@ void plan_fwd(WArgs& a, bool& few) {
   // keys a row tile can see, whatever the lengths are
   const int64_t tok = std::min<int64_t>(((few ? 32 : 128) + a.G - 1) / a.G + 1, a.T);
   const int64_t span = std::min<int64_t>(a.M, (int64_t)a.window * (a.causal ? 1 : 2) + tok + a.sinks);
-  const int64_t step = few ? 128 : 64;   // keys of one round of the waves
-  int64_t s = (kWgs + base - 1) / base;
-  s = std::min(s, (span + step - 1) / step);
-  if (base * 2 > kWgs) s = 1;
-  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+  const int64_t step = few ? 128 : (f32 ? 32 : 64), rounds = (span + step - 1) / step;
+  const double two = few ? (a.D > 64 || f32 ? 2.0 : 1.4) : (f32 ? 2.0 : 1.4);
+  double best = 0;
+  a.splits = 1;
+  for (int s = 1; s <= 64 && s <= rounds; ++s) {
+    const int64_t per = (base * s + 255) / 256;   // workgroups of the fullest CU
+    const double load = per <= 1 ? 1.0 : two * (double)per / 2.0;
+    const double t = ((double)((rounds + s - 1) / s) + 3) * load + (s > 1 ? 3 + 0.05 * s : 0);
+    if (s == 1 || t < best) {
+      best = t;
+      a.splits = s;
+    }
+  }
 }
 int64_t fwd_work(const WArgs& a) { return a.splits == 1 ? 0 : (int64_t)a.splits * a.B * a.Hk * a.R * (a.D + 1); }
 
-// The backward's key tiles, and how many chunks their rows are split into.  A tile without sinks has
-// `win` rows; more chunks than workgroups that run at once cost a second round of them all, too few
-// leave CUs idle, and more than one chunk costs the fp32 parts' way to memory and back.  Estimated in
-// microseconds: a row tile is 2 (bf16, width 128; 64 x 128 pairs) or 8 (fp32, 32 x 128), a workgroup
-// starts and ends in 4 of them, the parts move at 5 TB/s behind a 4 us launch.  Measured at 8192 tokens,
-// 16 / 4 heads of 128, window 1024, 4 sinks: 63 x 4 long workgroups in one round.
-// A tile with sinks has all rows, but only the waves with sinks work on most of them: shorter chunks.
+// The backward's key tiles, and how many chunks their rows are split into.  A tile has `win` rows; more
+// workgroups than run at once cost a second round of them all, too few leave CUs idle, and more than
+// one chunk costs the fp32 parts' way to memory and back.  Estimated in microseconds: a row tile is 2
+// (bf16, width 128; 64 x 128 pairs) or 6 (fp32, 32 x 128), a workgroup starts and ends in 4 of them, the
+// parts move at 5 TB/s behind a 4 us launch.  The far rows are cut to a workgroup for each CU.
 void plan_bwd(WArgs& a, bool f32) {
   a.tiles = (a.M + 127) / 128;
   a.nsink = (a.sinks + 127) / 128;
   const int64_t bh = (int64_t)a.B * a.Hk, rt = f32 ? 32 : 64;
-  const int slots = f32 && a.D <= 64 ? 512 : 256;
-  const double tile = (f32 ? 8.0 : 2.0) * std::max(a.D, 32) / 128;
+  const int slots = a.D <= 64 ? 512 : 256;
+  const double tile = (f32 ? 6.0 : 2.0) * std::max(a.D, 32) / 128;
   const int64_t win = std::min<int64_t>(a.M, (int64_t)a.window * (a.causal ? 1 : 2) + 127) * a.G;
-  const int64_t wt = (win + rt - 1) / rt, all = ((int64_t)a.M * a.G + rt - 1) / rt;
+  const int64_t wt = (win + rt - 1) / rt;
   double best = 0;
   a.cwin = 1;
   for (int c = 1; c <= 8 && c <= std::max<int64_t>(1, wt / 2); ++c) {
-    const double rounds = (double)(((int64_t)std::max(1, a.tiles - a.nsink) * bh * c + slots - 1) / slots);
+    const double rounds = (double)((a.tiles * bh * c + slots - 1) / slots);
     double t = rounds * ((double)((wt + c - 1) / c) + 4) * tile;
     if (c > 1) t += 4 + (double)c * a.M * bh * a.D * 16 / 5e6;
     if (c == 1 || t < best) {
@@ -1184,13 +1335,18 @@ void plan_bwd(WArgs& a, bool f32) {
       a.cwin = c;
     }
   }
-  const int64_t rows = std::max<int64_t>((wt / a.cwin + 3) / 4, 4);
-  a.csink = all <= wt ? a.cwin : (int)std::min<int64_t>((all + rows - 1) / rows, 256);
+  // tokens beyond the window of the first sink tile, and (two-sided) before that of the last
+  const int64_t high = (int64_t)a.M - 127 - a.window;
+  const int64_t low = a.causal ? 0 : (int64_t)(a.nsink - 1) * 128 - a.window + 1;
+  const int64_t far = std::max<int64_t>(high, 0) + std::max<int64_t>(low, 0);
+  a.far32 = a.cfar = 0;
+  if (a.sinks > 0 && far > 0) {
+    a.far32 = (a.sinks + 31) / 32;
+    const int64_t blocks = (far * a.G + 31) / 32, base = bh * a.far32;
+    a.cfar = (int)std::max<int64_t>(1, std::min<int64_t>({(256 + base - 1) / base, blocks / 8, 64}));
+  }
 }
-int64_t bwd_work(const WArgs& a) {
-  if (a.csink == 1 && a.cwin == 1) return 0;
-  return (int64_t)(a.nsink * a.csink + (a.tiles - a.nsink) * a.cwin) * a.B * a.Hk * 128 * 2 * a.D;
-}
+int64_t bwd_work(const WArgs& a) { return far_at(a) + (int64_t)a.B * a.Hk * a.far32 * a.cfar * 32 * 2 * a.D; }
 
 #define BY_WIDTH(KERNEL, GRID, THREADS, ARGS)                                                        \
   do {                                                                                               \
@@ -1223,12 +1379,16 @@ int run_bwd(WArgs a, hipStream_t st) {
   }
   DFCSA_CHECK_LAUNCH();
   const int bh = a.B * a.Hk;
-  BY_WIDTH(wattn_dkv_kernel, dim3((unsigned)(xcd_pad((a.tiles - a.nsink) * a.cwin * bh) + xcd_pad(a.nsink * a.csink * bh))), sizeof(T) == 2 ? 512 : 256, a);
+  BY_WIDTH(wattn_dkv_kernel, dim3((unsigned)xcd_pad(a.tiles * a.cwin * bh)), sizeof(T) == 2 && a.D > 64 ? 512 : 256, a);
   DFCSA_CHECK_LAUNCH();
-  const int t0 = a.csink > 1 ? 0 : a.nsink, t1 = a.cwin > 1 ? a.tiles : a.nsink;
-  if (t1 > t0) {
-    const int64_t e = (int64_t)(t1 - t0) * 128 * (2 * a.D / 4) * a.B * a.Hk;
-    hipLaunchKernelGGL((wattn_dkv_join_kernel<T>), dim3((unsigned)((e + 255) / 256)), dim3(256), 0, st, a, t0, t1 - t0);
+  if (a.cfar) {
+    BY_WIDTH(wattn_far_kernel, dim3((unsigned)xcd_pad(a.far32 * a.cfar * bh)), 256, a);
+    DFCSA_CHECK_LAUNCH();
+  }
+  const int ntile = a.cwin > 1 ? a.tiles : (a.cfar ? a.nsink : 0);
+  if (ntile) {
+    const int64_t e = (int64_t)ntile * 128 * (2 * a.D / 4) * bh;
+    hipLaunchKernelGGL((wattn_dkv_join_kernel<T>), dim3((unsigned)((e + 255) / 256)), dim3(256), 0, st, a);
     DFCSA_CHECK_LAUNCH();
   }
   return 0;
@@ -1246,7 +1406,7 @@ int dfcsa_wattn_work_floats(const dfcsa_wattn_desc* d, int backward, int64_t* fl
     *floats = bwd_work(a);
   } else {
     bool few;
-    plan_fwd(a, few);
+    plan_fwd(a, d->dtype == DFCSA_DT_F32, few);
     *floats = fwd_work(a);
   }
   return 0;
@@ -1256,7 +1416,7 @@ int dfcsa_wattn_fwd(const dfcsa_wattn_desc* d, void* stream) {
   WArgs a;
   if (!fill(d, a, false)) return DFCSA_EINVAL;
   bool few;
-  plan_fwd(a, few);
+  plan_fwd(a, d->dtype == DFCSA_DT_F32, few);
   if ((int64_t)a.tiles * a.B * a.Hk * a.splits > 0x7ffffff0) return DFCSA_EINVAL;
   if (fwd_work(a) > 0 && (!d->work || d->work_floats < fwd_work(a))) return DFCSA_EINVAL;
   return d->dtype == DFCSA_DT_F32 ? run_fwd<float>(a, few, (hipStream_t)stream) : run_fwd<bf16_t>(a, few, (hipStream_t)stream);
@@ -1266,7 +1426,7 @@ int dfcsa_wattn_bwd(const dfcsa_wattn_desc* d, void* stream) {
   WArgs a;
   if (!fill(d, a, true)) return DFCSA_EINVAL;
   plan_bwd(a, d->dtype == DFCSA_DT_F32);
-  if ((int64_t)(a.nsink * a.csink + a.tiles * a.cwin) * a.B * a.Hk > 0x7ffffff0) return DFCSA_EINVAL;
+  if (((int64_t)a.tiles * a.cwin + (int64_t)a.far32 * a.cfar + (a.R + 127) / 128) * a.B * a.Hk > 0x7ffffff0) return DFCSA_EINVAL;
   if (bwd_work(a) > 0 && (!d->work || d->work_floats < bwd_work(a))) return DFCSA_EINVAL;
   return d->dtype == DFCSA_DT_F32 ? run_bwd<float>(a, (hipStream_t)stream) : run_bwd<bf16_t>(a, (hipStream_t)stream);
 }
