@@ -385,6 +385,7 @@ template <typename T, int DP> struct Online {
       m = mn;
     }
     const float ms = m == kNegInf ? 0.f : m;
+    __builtin_amdgcn_s_setprio(1);   // ahead of the SIMD's other waves while the matrix unit has work (113 -> 110 us)
 #pragma unroll
     for (int b = 0; b < NSUB; ++b) {
 #pragma unroll
@@ -397,6 +398,7 @@ template <typename T, int DP> struct Online {
         for (int d = 0; d < I::ND; ++d) o[d] = Mma<T>::mma(im.col_frag(vimg, 32 * b, st, d), p, o[d]);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
   }
 };
 
@@ -785,10 +787,12 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
 #pragma unroll 1   // one 32 x 32 block's registers at a time; the other wave of the SIMD fills the gaps
     for (int kb = 0; kb < KT / 32; ++kb) {
       f16_t s = zero16(), dp = zero16();
+      __builtin_amdgcn_s_setprio(1);   // 146 -> 142 us
 #pragma unroll
       for (int st = 0; st < I::NS; ++st) s = Mma<T>::mma(im.row_frag(cur, 32 * kb, st), q[st], s);
 #pragma unroll
       for (int st = 0; st < I::NS; ++st) dp = Mma<T>::mma(im.row_frag(cur + I::BYTES, 32 * kb, st), dof[st], dp);
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - dl);
       if (masked) {
@@ -836,7 +840,11 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
 // further away that see sinks are wattn_far_kernel's.  fp32 parts are added in order by wattn_dkv_join.
 __device__ __forceinline__ void key_rows(const WArgs& a, const Seq& seq, int kt, int rt, int& i0, int& i1) {
   const int k0 = kt * 128, k1 = min(k0 + 128, seq.len);
-  const int p0 = a.causal ? k0 : max(k0 - a.window + 1, 0), p1 = min(k1 - 1 + a.window - 1, seq.len - 1);
+  int p0 = a.causal ? k0 : max(k0 - a.window + 1, 0), p1 = min(k1 - 1 + a.window - 1, seq.len - 1);
+  if (k0 < a.sinks && !a.cfar) {   // few rows are further away: no pass of their own
+    p0 = a.causal ? k0 : 0;
+    p1 = seq.len - 1;
+  }
   i0 = i1 = 0;   // tiles of rt rows
   if (k0 < k1 && p0 <= p1) {
     i0 = p0 * a.G / rt;
@@ -855,9 +863,10 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
   constexpr int RT = I::ROWS, RB = RT * I::PITCH;
   constexpr int NI = RT * I::CPR / 64 / NW;
   constexpr int OUT = NW == 8 ? 4 * 64 * (DP / 2) * 4 : 0;   // one wave's dK or dV, four times
-  constexpr int MAIN = 4 * RB + (KLDS ? 128 * I::PITCH : 0);
+  constexpr int NB = 2;   // row tiles in LDS
+  constexpr int MAIN = 2 * NB * RB + (KLDS ? 128 * I::PITCH : 0);
   __shared__ __attribute__((aligned(256))) char smem[MAIN > OUT ? MAIN : OUT];
-  __shared__ __attribute__((aligned(16))) float s_l[2][RT], s_d[2][RT];
+  __shared__ __attribute__((aligned(16))) float s_l[NB][RT], s_d[NB][RT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int L = xcd_remap(blockIdx.x, a.tiles * a.cwin * a.B * a.Hk);
   if (L < 0) return;
@@ -874,13 +883,13 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
   const int kw = k0 + kb * 32, key = kw + (lane & 31);
   const bool kok = key < seq.len;
   frag kf[KLDS ? 1 : I::NS], vf[I::NS];
-  const char* kimg = smem + 4 * RB;
+  const char* kimg = smem + 2 * NB * RB;
   {
     const int kk = min(key, a.M - 1);
     if constexpr (KLDS) {
       KeyDma<T, DP, 128, NW> dma;
       dma.init(wave, lane, a.D);
-      if (k0 < seq.len) dma.issue((const char*)a.k + b * a.kb + hk * a.kh, a.kt, k0, 0, seq.len, 0, lds_addr(smem) + 4 * RB, wave);
+      if (k0 < seq.len) dma.issue((const char*)a.k + b * a.kb + hk * a.kh, a.kt, k0, 0, seq.len, 0, lds_addr(smem) + 2 * NB * RB, wave);
     } else {
       load_frags<T, DP>((const char*)a.k + b * a.kb + (int64_t)kk * a.kt + hk * a.kh, kok, a.D, lane, kf);
     }
@@ -952,49 +961,54 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
   for (int d = 0; d < I::ND; ++d) dk[d] = dv[d] = zero16();
   I im;
   im.init(lane);
-  auto body = [&](const char* cur, int buf, int r0, int rb, bool masked) {   // rows r0 .., image rows 32 rb ..
-    {
-      f16_t s = zero16(), dp = zero16();
+  // one 32 x 32 block in two phases: S and dP; then P, dS and the products with them
+  f16_t s, dp;
+  auto scores = [&](const char* cur, int rb) {
+    s = zero16();
+    dp = zero16();
 #pragma unroll
-      for (int st = 0; st < I::NS; ++st) {
-        frag kk;
-        if constexpr (KLDS) kk = im.row_frag(kimg + kb * 32 * I::PITCH, 0, st);
-        else kk = kf[st];
-        s = Mma<T>::mma(im.row_frag(cur, 32 * rb, st), kk, s);
-      }
+    for (int st = 0; st < I::NS; ++st) {
+      frag kk;
+      if constexpr (KLDS) kk = im.row_frag(kimg + kb * 32 * I::PITCH, 0, st);
+      else kk = kf[st];
+      s = Mma<T>::mma(im.row_frag(cur, 32 * rb, st), kk, s);
+    }
 #pragma unroll
-      for (int st = 0; st < I::NS; ++st) dp = Mma<T>::mma(im.row_frag(cur + RB, 32 * rb, st), vf[st], dp);
+    for (int st = 0; st < I::NS; ++st) dp = Mma<T>::mma(im.row_frag(cur + RB, 32 * rb, st), vf[st], dp);
+  };
+  auto products = [&](const char* cur, int buf, int r0, int rb, bool masked) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int rr = 32 * rb + 8 * g + 4 * (lane >> 5);
-        const f4_t l4 = *(const f4_t*)&s_l[buf][rr], d4 = *(const f4_t*)&s_d[buf][rr];
+    for (int g = 0; g < 4; ++g) {
+      const int rr = 32 * rb + 8 * g + 4 * (lane >> 5);
+      const f4_t l4 = *(const f4_t*)&s_l[buf][rr], d4 = *(const f4_t*)&s_d[buf][rr];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale2, -l4[e]));
-          dp[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - d4[e]);
-        }
-      }
-      if (masked) {
-        asm volatile("");
-        const int rr = r0 + 4 * (lane >> 5), ge = vlo - rr, lt = vhi - rr;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int c = 8 * (e >> 2) + (e & 3);
-          const bool see = (c >= ge) & (c < lt);
-          s[e] = see ? s[e] : 0.f;
-          dp[e] = see ? dp[e] : 0.f;
-        }
-      }
-#pragma unroll
-      for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
-        const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
-#pragma unroll
-        for (int d = 0; d < I::ND; ++d) {
-          dv[d] = Mma<T>::mma(im.col_frag(cur + RB, 32 * rb, st, d), pf, dv[d]);
-          dk[d] = Mma<T>::mma(im.col_frag(cur, 32 * rb, st, d), df, dk[d]);
-        }
+      for (int e = 0; e < 4; ++e) {
+        s[4 * g + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale2, -l4[e]));
+        dp[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - d4[e]);
       }
     }
+    if (masked) {
+      asm volatile("");
+      const int rr = r0 + 4 * (lane >> 5), ge = vlo - rr, lt = vhi - rr;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int c = 8 * (e >> 2) + (e & 3);
+        const bool see = (c >= ge) & (c < lt);
+        s[e] = see ? s[e] : 0.f;
+        dp[e] = see ? dp[e] : 0.f;
+      }
+    }
+    __builtin_amdgcn_s_setprio(1);   // 220 -> 215 us
+#pragma unroll
+    for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+      const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
+#pragma unroll
+      for (int d = 0; d < I::ND; ++d) {
+        dv[d] = Mma<T>::mma(im.col_frag(cur + RB, 32 * rb, st, d), pf, dv[d]);
+        dk[d] = Mma<T>::mma(im.col_frag(cur, 32 * rb, st, d), df, dk[d]);
+      }
+    }
+    __builtin_amdgcn_s_setprio(0);
   };
 
   if (c0 < c1) {
@@ -1012,10 +1026,13 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
       nx = stat(it + 1);
       issue(it + 1, lds_addr(smem) + (buf ^ 1) * 2 * RB);
     }
-#pragma unroll 1
+#pragma unroll 1   // one block's registers at a time; the other waves of the SIMD fill the gaps
     for (int rb = NW == 8 ? half : 0; rb < RT / 32; rb += NW == 8 ? 2 : 1) {
       const int r0 = it * RT + 32 * rb;
-      if (r0 < nhi && r0 + 32 > nlo) body(cur, buf, r0, rb, r0 < alo || r0 + 32 > ahi);
+      if (r0 < nhi && r0 + 32 > nlo) {
+        scores(cur, rb);
+        products(cur, buf, r0, rb, r0 < alo || r0 + 32 > ahi);
+      }
     }
     if (more) put(nx, buf ^ 1);
   }
@@ -1212,17 +1229,17 @@ __global__ void __launch_bounds__(256) wattn_dkv_join_kernel(const WArgs a) {
   }
   if (a.cfar && key < a.sinks) {
     const float* f = a.part + far_at(a) + (((int64_t)bh * a.far32 + key / 32) * a.cfar * 32 + key % 32) * 2 * a.D + c;
-    for (int i = 0; i < a.cfar; i += 4) {   // four in flight
-      float4 x[4];
+    for (int i = 0; i < a.cfar; i += 16) {   // sixteen in flight
+      float4 x[16];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = *(const float4*)(f + (int64_t)min(i + j, a.cfar - 1) * 32 * 2 * a.D);
+      for (int j = 0; j < 16; ++j) x[j] = *(const float4*)(f + (int64_t)min(i + j, a.cfar - 1) * 32 * 2 * a.D);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (i + j >= a.cfar) break;
-        s[0] += x[j].x;
-        s[1] += x[j].y;
-        s[2] += x[j].z;
-        s[3] += x[j].w;
+      for (int j = 0; j < 16; ++j) {
+        const float w = i + j < a.cfar ? 1.f : 0.f;
+        s[0] = fmaf(w, x[j].x, s[0]);
+        s[1] = fmaf(w, x[j].y, s[1]);
+        s[2] = fmaf(w, x[j].z, s[2]);
+        s[3] = fmaf(w, x[j].w, s[3]);
       }
     }
   }
@@ -1340,7 +1357,8 @@ void plan_bwd(WArgs& a, bool f32) {
   const int64_t low = a.causal ? 0 : (int64_t)(a.nsink - 1) * 128 - a.window + 1;
   const int64_t far = std::max<int64_t>(high, 0) + std::max<int64_t>(low, 0);
   a.far32 = a.cfar = 0;
-  if (a.sinks > 0 && far > 0) {
+  // a pass of their own costs two launches, about 12 us; without it the sinks' tiles take the far rows too
+  if (a.sinks > 0 && (double)(far * a.G / rt) * tile > 12) {
     a.far32 = (a.sinks + 31) / 32;
     const int64_t blocks = (far * a.G + 31) / 32, base = bh * a.far32;
     a.cfar = (int)std::max<int64_t>(1, std::min<int64_t>({(256 + base - 1) / base, blocks / 8, 64}));
