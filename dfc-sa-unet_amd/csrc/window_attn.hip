@@ -501,6 +501,132 @@ __device__ __forceinline__ void finish_rows(const WArgs& a, int bh, int split, i
   }
 }
 
+// ------------------------------------------------------------------ rows and keys one at a time
+// A product of matrix tiles multiplies every element of both: where a hidden key's P is 0 and its V (or K,
+// or a hidden row's Q or dO) is infinite or NaN, the 0 * inf reaches rows that do not see it.  Nothing is
+// tested for that in the loops; a wave whose results are not all finite forms them again here, from the
+// visible pairs alone, one row (or key) at a time with two columns per lane.
+__device__ __forceinline__ bool finite_all(const f16_t& v) {
+  bool ok = true;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) ok = ok && (__float_as_uint(v[e]) & 0x7f800000u) != 0x7f800000u;
+  return ok;
+}
+template <typename T> __device__ __forceinline__ float2 two(const void* row, int d, int D) {
+  if (d >= D) return make_float2(0.f, 0.f);
+  const T* p = (const T*)row + d;
+  return make_float2(ElemTraits<T>::to_f(p[0]), ElemTraits<T>::to_f(p[1]));
+}
+template <typename T> __device__ __forceinline__ void put_two(void* row, int d, int D, float x, float y) {
+  if (d >= D) return;
+  ((T*)row)[d] = ElemTraits<T>::from_f(x);
+  ((T*)row)[d + 1] = ElemTraits<T>::from_f(y);
+}
+struct At {   // a packed row's place
+  int t, g;
+};
+__device__ __forceinline__ At at_row(const WArgs& a, int r) {
+  At x;
+  x.t = dm_div(a.dmG, r);
+  x.g = r - x.t * a.G;
+  return x;
+}
+__device__ __forceinline__ bool sees(const RowMask& m, int key) { return (unsigned)(key - m.lo) <= m.span || key < m.sl; }
+
+// row r over the keys of tiles [it0, it1) of KT keys, to where finish_rows puts it
+template <typename T>
+__device__ __forceinline__ void exact_row(const WArgs& a, const Seq& seq, int bh, int split, int r, const TileList& tl, int it0,
+                                       int it1, int KT) {
+  const int lane = threadIdx.x & 63, d = 2 * lane, b = bh / a.Hk, hk = bh - b * a.Hk;
+  const At x = at_row(a, r);
+  const RowMask mask = row_mask(a, seq, r);
+  const bool live = mask.lo != 0x7fffffff;
+  const char* kb = (const char*)a.k + b * a.kb + hk * a.kh;
+  const char* vb = (const char*)a.v + b * a.vb + hk * a.vh;
+  float2 q = make_float2(0.f, 0.f);
+  if (live) q = two<T>((const char*)a.q + b * a.qb + x.t * a.qt + (hk * a.G + x.g) * a.qh, d, a.D);
+  float m = kNegInf, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int it = it0; it < it1; ++it)
+    for (int key = tl[it] * KT; key < (tl[it] + 1) * KT; ++key) {
+      if (!sees(mask, key)) continue;
+      const float2 k = two<T>(kb + (int64_t)key * a.kt, d, a.D), v = two<T>(vb + (int64_t)key * a.vt, d, a.D);
+      const float s = wave_sum(q.x * k.x + q.y * k.y) * a.scale2;
+      const float mn = fmaxf(m, s), ms = mn == kNegInf ? 0.f : mn;
+      const float al = __builtin_amdgcn_exp2f(m - ms), p = __builtin_amdgcn_exp2f(s - ms);
+      l = l * al + p;
+      o0 = o0 * al + p * v.x;
+      o1 = o1 * al + p * v.y;
+      m = mn;
+    }
+  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+  const float lse = l == 0.f ? kNegInf : m + __builtin_amdgcn_logf(l);
+  const int64_t row = (int64_t)bh * a.R + r, rows = (int64_t)a.B * a.Hk * a.R;
+  if (a.splits == 1) {
+    const int64_t at = (((int64_t)b * a.T + x.t) * a.H + hk * a.G + x.g) * a.D;
+    put_two<T>((T*)a.o + at, d, a.D, o0 * inv, o1 * inv);
+    if (sizeof(T) == 2 && a.rest)
+      put_two<bf16_t>(a.rest + at, d, a.D, o0 * inv - bf2f(f2bf(o0 * inv)), o1 * inv - bf2f(f2bf(o1 * inv)));
+    if (a.lse && lane == 0) a.lse[row] = lse;
+  } else {
+    put_two<float>(a.part + (split * rows + row) * a.D, d, a.D, o0 * inv, o1 * inv);
+    if (lane == 0) a.part[a.splits * rows * a.D + split * rows + row] = lse;
+  }
+}
+// dQ of row r
+template <typename T>
+__device__ __forceinline__ void exact_dq(const WArgs& a, const Seq& seq, int bh, int r, const TileList& tl, int KT, float lse,
+                                      float dl) {
+  const int lane = threadIdx.x & 63, d = 2 * lane, b = bh / a.Hk, hk = bh - b * a.Hk;
+  const At x = at_row(a, r);
+  const RowMask mask = row_mask(a, seq, r);
+  const char* kb = (const char*)a.k + b * a.kb + hk * a.kh;
+  const char* vb = (const char*)a.v + b * a.vb + hk * a.vh;
+  float2 q = make_float2(0.f, 0.f), g = q;
+  if (mask.lo != 0x7fffffff) {
+    q = two<T>((const char*)a.q + b * a.qb + x.t * a.qt + (hk * a.G + x.g) * a.qh, d, a.D);
+    g = two<T>((const char*)a.dO + b * a.ob + x.t * a.ot + (hk * a.G + x.g) * a.oh, d, a.D);
+  }
+  float d0 = 0.f, d1 = 0.f;
+  for (int it = 0; it < tl.n; ++it)
+    for (int key = tl[it] * KT; key < (tl[it] + 1) * KT; ++key) {
+      if (!sees(mask, key)) continue;
+      const float2 k = two<T>(kb + (int64_t)key * a.kt, d, a.D), v = two<T>(vb + (int64_t)key * a.vt, d, a.D);
+      const float s = wave_sum(q.x * k.x + q.y * k.y), dp = wave_sum(g.x * v.x + g.y * v.y);
+      const float ds = __builtin_amdgcn_exp2f(s * a.scale2 - lse) * (dp - dl);
+      d0 += ds * k.x;
+      d1 += ds * k.y;
+    }
+  put_two<T>((T*)a.dq + (((int64_t)b * a.T + x.t) * a.H + hk * a.G + x.g) * a.D, d, a.D, d0 * a.scale, d1 * a.scale);
+}
+// dK and dV of a key over rows [r0, r1) and [r2, r3), to outk and outv (type O)
+template <typename T, typename O>
+__device__ __forceinline__ void exact_key(const WArgs& a, const Seq& seq, int bh, int key, int r0, int r1, int r2, int r3,
+                                       O* outk, O* outv) {
+  const int lane = threadIdx.x & 63, d = 2 * lane, b = bh / a.Hk, hk = bh - b * a.Hk;
+  float2 k = make_float2(0.f, 0.f), v = k;
+  float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
+  if (key < seq.len) {
+    k = two<T>((const char*)a.k + b * a.kb + (int64_t)key * a.kt + hk * a.kh, d, a.D);
+    v = two<T>((const char*)a.v + b * a.vb + (int64_t)key * a.vt + hk * a.vh, d, a.D);
+    for (int r = r0; r < max(r1, r3); r = r + 1 == r1 && r2 < r3 && r2 > r ? r2 : r + 1) {
+      if (r >= a.R || (r >= r1 && (r < r2 || r >= r3))) continue;
+      if (!sees(row_mask(a, seq, r), key)) continue;
+      const At x = at_row(a, r);
+      const float2 q = two<T>((const char*)a.q + b * a.qb + x.t * a.qt + (hk * a.G + x.g) * a.qh, d, a.D);
+      const float2 g = two<T>((const char*)a.dO + b * a.ob + x.t * a.ot + (hk * a.G + x.g) * a.oh, d, a.D);
+      const float s = wave_sum(q.x * k.x + q.y * k.y), dp = wave_sum(g.x * v.x + g.y * v.y);
+      const float p = __builtin_amdgcn_exp2f(s * a.scale2 - a.lse[(int64_t)bh * a.R + r]);
+      const float ds = p * (dp - a.delta[(int64_t)bh * a.R + r]);
+      k0 += ds * q.x;
+      k1 += ds * q.y;
+      v0 += p * g.x;
+      v1 += p * g.y;
+    }
+  }
+  put_two<O>(outk, d, a.D, k0 * a.scale, k1 * a.scale);
+  put_two<O>(outv, d, a.D, v0, v1);
+}
+
 // ============================================================================ forward
 // 128 rows per workgroup, 32 per wave; key tiles double-buffered in LDS.
 template <typename T, int DP>
@@ -554,6 +680,13 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
   const float lsum = st.l + __shfl_xor(st.l, 32, 64);
   lds_barrier();   // the tiles are read
   finish_rows<T, DP>(a, bh, split, rw, st.o, st.m, lsum, smem + wave * 32 * out_pitch<DP>(), lane);
+  bool ok = true;
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(st.o[d]);
+  if (__any(!ok && r < a.R)) {
+#pragma unroll 1
+    for (int i = rw; i < min(rw + 32, a.R); ++i) exact_row<T>(a, seq, bh, split, i, tl, it0, it1, KT);
+  }
 }
 
 // Few rows (at most 32 per tile): the four waves share the rows and split the keys, each with its own
@@ -636,7 +769,7 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
   __syncthreads();
   // 8 threads a row, DP / 8 columns each
   const int row = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (DP / 8), rr = r0 + row;
-  if (rr >= a.R) return;
+  bool ok = true;
   float mm = kNegInf;
 #pragma unroll
   for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm_m[w][row]);
@@ -649,13 +782,13 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
   const float inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);
   const float lse = ls == 0.f ? kNegInf : mm + __builtin_amdgcn_logf(ls);
   const int64_t orow = (int64_t)bh * a.R + rr, rows = (int64_t)a.B * a.Hk * a.R;
-  const int t = dm_div(a.dmG, rr), g = rr - t * a.G;
+  const int t = dm_div(a.dmG, min(rr, a.R - 1)), g = rr - t * a.G;
   const int64_t at = (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
   T* po = (T*)a.o + at;
   float* pp = a.splits == 1 ? nullptr : a.part + (split * rows + orow) * a.D;
 #pragma unroll
   for (int c = 0; c < DP / 8; c += 4) {
-    if (c0 + c < a.D) {
+    if (rr < a.R && c0 + c < a.D) {
       float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -665,6 +798,8 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
         s[2] += f[w] * x.z;
         s[3] += f[w] * x.w;
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ok = ok && (__float_as_uint(s[e]) & 0x7f800000u) != 0x7f800000u;
       if (pp) {
         store4<float>(pp + c0 + c, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);
       } else {
@@ -673,9 +808,14 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
       }
     }
   }
-  if ((threadIdx.x & 7) == 0) {
+  if ((threadIdx.x & 7) == 0 && rr < a.R) {
     if (pp) a.part[a.splits * rows * a.D + split * rows + orow] = lse;
     else if (a.lse) a.lse[orow] = lse;
+  }
+  if (__syncthreads_or(!ok)) {   // (also the barrier between these stores and the ones that replace them)
+    const int f = (int)((int64_t)tl.n * split / a.splits);
+#pragma unroll 1
+    for (int i = r0 + wave; i < min(r0 + 32, a.R); i += 4) exact_row<T>(a, seq, bh, split, i, tl, f, it1, KT);
   }
 }
 
@@ -829,6 +969,14 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
     const int ti = dm_div(a.dmG, min(rw + i, a.R - 1)), gi = rw + i - ti * a.G;
     return rw + i < a.R ? (T*)a.dq + obase + ((int64_t)ti * a.H + gi) * a.D : nullptr;
   });
+  bool ok = true;
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(dq[d]);
+  if (__any(!ok && r < a.R)) {
+#pragma unroll 1
+    for (int i = 0; i < 32 && rw + i < a.R; ++i)
+      exact_dq<T>(a, seq, bh, rw + i, tl, KT, __shfl(lse, i, 64), __shfl(dl, i, 64));
+  }
 }
 
 // ============================================================================ backward: dK, dV
@@ -1066,6 +1214,9 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
     }
     if (half == 1) return;
   }
+  bool ok = true;
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(dk[d]) && finite_all(dv[d]);
   if (a.cwin == 1 && !(kt < a.nsink && a.cfar)) {
     char* lds = smem + kb * 32 * out_pitch<DP>();
     auto at = [&](void* p) {
@@ -1073,11 +1224,28 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
     };
     store_rows<T, DP, false>(lds, dk, a.scale, a.D, lane, at(a.dk));
     store_rows<T, DP, false>(lds, dv, 1.f, a.D, lane, at(a.dv));
-  } else if (key < a.M) {
+    if (__any(!ok)) {
+#pragma unroll 1
+      for (int i = 0; i < 32 && kw + i < a.M; ++i) {
+        const int64_t to = (((int64_t)b * a.M + kw + i) * a.Hk + hk) * a.D;
+        exact_key<T, T>(a, seq, bh, kw + i, c0 * RT, c1 * RT, 0, 0, (T*)a.dk + to, (T*)a.dv + to);
+      }
+    }
+    return;
+  }
+  if (key < a.M) {
     const int items = a.cwin > 1 ? a.tiles * a.cwin : a.nsink;   // as in the join
     float* p = a.part + (((int64_t)bh * items + item) * 128 + kb * 32 + (lane & 31)) * 2 * a.D;
     store_col<float, I::ND>(p, dk, a.scale, a.D, lane);
     store_col<float, I::ND>(p + a.D, dv, 1.f, a.D, lane);
+  }
+  if (__any(!ok)) {
+    const int items = a.cwin > 1 ? a.tiles * a.cwin : a.nsink;
+#pragma unroll 1
+    for (int i = 0; i < 32 && kw + i < a.M; ++i) {
+      float* p = a.part + (((int64_t)bh * items + item) * 128 + kb * 32 + i) * 2 * a.D;
+      exact_key<T, float>(a, seq, bh, kw + i, c0 * RT, c1 * RT, 0, 0, p, p + a.D);
+    }
   }
 }
 
@@ -1190,6 +1358,7 @@ __global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
       *(float4*)(x + ((I::ND + d) * 4 + g) * 256) = make_float4(dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]);
     }
   __syncthreads();
+  bool ok = true;
   float* out = a.part + far_at(a) + ((int64_t)bh * a.far32 * a.cfar + sb * a.cfar + ch) * 32 * 2 * a.D;
   for (int e = threadIdx.x; e < 2 * I::ND * 4 * 64; e += 256) {
     const int ln = e & 63, grp = e >> 6, which = grp / (I::ND * 4), c = grp % (I::ND * 4) * 8 + 4 * (ln >> 5);
@@ -1203,7 +1372,18 @@ __global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
       v.w += y.w;
     }
     const float f = which ? 1.f : a.scale;
+    const float t = v.x * 0.f + v.y * 0.f + v.z * 0.f + v.w * 0.f;   // NaN where one is not finite
+    ok = ok && t == 0.f;
     if (c < a.D) *(float4*)(out + (ln & 31) * 2 * a.D + which * a.D + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+  }
+  if (__syncthreads_or(!ok)) {
+    const int b0 = (int)((int64_t)nb * ch / a.cfar), l1 = min(c1, nlo), h0 = hi0 + max(b0 - nlo, 0), h1 = hi0 + c1 - nlo;
+#pragma unroll 1
+    for (int i = wave; i < 32; i += 4) {
+      float* p = out + i * 2 * a.D;
+      if (kw + i < min(a.sinks, seq.len))
+        exact_key<T, float>(a, seq, bh, kw + i, b0 * 32, l1 * 32, h0 * 32, h1 * 32, p, p + a.D);
+    }
   }
 }
 

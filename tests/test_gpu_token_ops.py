@@ -440,6 +440,66 @@ def test_attention_cached(B, T, cap, H, Hk, D, window, sinks, lengths, ty):
         within(o[b], want[0], bound[0], f"o[{b}]")
 
 
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("T,cap,window,n", [(1, 300, 40, 290), (5, 300, 40, 250), (40, 500, 64, 500), (90, 200, 30, 180)])
+def test_attention_cached_hidden_infinities(T, cap, window, n, ty):
+    """A key that some of the new tokens see and others do not: its NaN or infinity reaches those that see it only."""
+    g = gen(T + cap)
+    H, Hk, D = 4, 2, 64
+    q, k, v = rand(g, 1, T, H, D, type=ty), rand(g, 1, cap, Hk, D, type=ty), rand(g, 1, cap, Hk, D, type=ty)
+    lengths = torch.tensor([n], dtype=torch.int32, device=DEV)
+    want = tk().window_attention_cached(q, k, v, lengths, window, 2)
+    j = n - T // 2 - 1
+    for bad in (math.nan, math.inf):
+        v2 = v.clone()
+        v2[0, j] = bad
+        o = tk().window_attention_cached(q, k, v2, lengths, window, 2)
+        p = torch.arange(T, device=DEV) + n - T
+        sees = (p >= j) & (p - j < window)
+        assert not torch.isfinite(o[0, sees]).any()
+        # the rows formed again differ by the rounding of P and of the sums
+        within(o[0, ~sees], want[0, ~sees].double(), (4 * UT[ty] + 2000 * UF) * v.double().abs().amax().expand_as(want[0, ~sees]), "others")
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("N,H,Hk,D,window,sinks,causal", [(150, 4, 2, 64, 20, 3, True), (700, 2, 1, 128, 50, 4, True),
+                                                          (700, 3, 3, 40, 30, 40, False), (2500, 2, 2, 64, 100, 2, True)])
+def test_attention_hidden_infinities(N, H, Hk, D, window, sinks, causal, ty):
+    """NaN or infinity in a q, k, v or dO row: the results of the pairs that do not involve it stay."""
+    g = gen(N + D)
+    t = [rand(g, 1, N, h, D, type=ty) for h in (H, Hk, Hk, H)]
+    lens = torch.tensor([N - 3], dtype=torch.int32, device=DEV)
+
+    def run(q, k, v, do):
+        leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+        o = tk().window_attention(*leaves, window, sinks, causal=causal, lengths=lens)
+        return [o.detach()[0], *(x[0] for x in torch.autograd.grad(o, leaves, do))]
+
+    clean = run(*t)
+    mask = visible(N, N, N - 3, 0, window, sinks, causal)
+    at = N // 2
+    for which, bad in ((0, math.nan), (1, math.inf), (2, math.nan), (3, math.inf), (2, -math.inf)):
+        x = [y.clone() for y in t]
+        x[which][0, at] = bad
+        got = run(*x)
+        # what depends on the row: as a query (q, dO) or as a key (k, v), directly and through the rows that see it
+        if which in (0, 3):
+            rows = torch.zeros(N, dtype=torch.bool, device=DEV)
+            rows[at] = True
+        else:
+            rows = mask[:, at]
+        keys = mask[rows].any(0)
+        touched = (rows if which != 3 else torch.zeros_like(rows), rows, keys | False, keys | False)
+        for name, a, b, hit in zip(("o", "dq", "dk", "dv"), got, clean, touched):
+            free = ~hit
+            assert torch.isfinite(a[free]).all(), (which, name)
+            # formed again in another order, P and dS unrounded: rounding of both sides
+            scale = b.double().abs().amax()
+            within(a[free], b[free].double(), (6 * UT[ty] + 4 * N * UF) * scale.expand_as(b[free]), f"{which} {name}")
+        assert not torch.isfinite(got[0][rows]).all() or which == 3
+        assert not torch.isfinite(got[1][rows]).all()
+
+
 def test_attention_cached_is_the_last_rows_of_the_whole():
     g = gen(51)
     q, k, v = rand(g, 2, 300, 8, 64, type=BF), rand(g, 2, 300, 2, 64, type=BF), rand(g, 2, 300, 2, 64, type=BF)
