@@ -15,6 +15,7 @@ namespace {
 // A row is held by WAVES waves of one workgroup (1: C <= 2048, four rows per workgroup; 4: wider
 // rows), NC chunks of 8 columns per lane.
 constexpr int kNormMaxC = 16384;
+constexpr int kNormMaxRows = 0x7fff0000;   // a row index plus a grid's rows stays an int
 constexpr float kE4m3Max = 448.0f;
 
 template <int WAVES>
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(int n, int C, const float*
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) dequant_kernel(int64_t n8, int C8, DivMod dmc, int gsh, int ng,
+__global__ void __launch_bounds__(256) dequant_kernel(int64_t n8, int C8, int gsh, int ng,
                                                       const uint2* __restrict__ y8, const float* __restrict__ scales,
                                                       T* __restrict__ out) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -329,7 +330,7 @@ int launch_bwd(int rows, int C, const void* dy, const void* dr, const void* r, c
   return 0;
 }
 
-bool norm_shape_ok(int rows, int C) { return rows > 0 && C >= 8 && C % 8 == 0 && C <= kNormMaxC; }
+bool norm_shape_ok(int rows, int C) { return rows > 0 && rows <= kNormMaxRows && C >= 8 && C % 8 == 0 && C <= kNormMaxC; }
 bool types_ok(int t, int r) { return (t == DFCSA_DT_BF16 && (r == DFCSA_DT_BF16 || r == DFCSA_DT_F32)) ||
                                      (t == DFCSA_DT_F32 && r == DFCSA_DT_F32); }
 
@@ -356,7 +357,7 @@ struct RotaryArgs {
   unsigned char axis[DFCSA_ROTARY_MAX_PAIRS];
 };
 
-constexpr int kRotLds = 2048;   // angles (cos, sin) a workgroup holds
+constexpr int kRotLds = 256;   // angles (cos, sin) a workgroup holds
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
@@ -490,12 +491,11 @@ int dfcsa_dequant_q8(int dtype, int64_t rows, int C, int group, const void* y8, 
   const int64_t n8 = rows * (C / 8), blocks = (n8 + 255) / 256;
   if (blocks > 0x7fffffff) return DFCSA_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  const DivMod dm = make_divmod(C / 8);
   if (dtype == DFCSA_DT_F32)
-    hipLaunchKernelGGL((dequant_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, st, n8, C / 8, dm, gsh, C / group,
+    hipLaunchKernelGGL((dequant_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, st, n8, C / 8, gsh, C / group,
                        (const uint2*)y8, scales, (float*)out);
   else if (dtype == DFCSA_DT_BF16)
-    hipLaunchKernelGGL((dequant_kernel<bf16_t>), dim3((unsigned)blocks), dim3(256), 0, st, n8, C / 8, dm, gsh,
+    hipLaunchKernelGGL((dequant_kernel<bf16_t>), dim3((unsigned)blocks), dim3(256), 0, st, n8, C / 8, gsh,
                        C / group, (const uint2*)y8, scales, (bf16_t*)out);
   else
     return DFCSA_EINVAL;
@@ -539,7 +539,7 @@ int dfcsa_rotary(const dfcsa_rotary_desc* d, void* stream) {
   // one angle per thread of a workgroup, as far as that leaves a workgroup for each CU
   int tok = 256 / a.P;
   tok = tok < 1 ? 1 : tok;
-  while (tok > 1 && (tokens + tok - 1) / tok < 512) tok >>= 1;
+  while (tok > 1 && ((tokens + tok - 1) / tok < 512 || (int64_t)heads * a.D * tok > 1 << 28)) tok >>= 1;
   a.tok = tok;
   hipStream_t st = (hipStream_t)stream;
   if (d->dtype == DFCSA_DT_F32) launch_rotary<float>(a, vec, st);

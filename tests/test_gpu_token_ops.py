@@ -4,6 +4,7 @@ Tolerances are bounds on the rounding errors of the computed formulas: UT, half 
 (bf16 2^-8, fp32 2^-24); UP, the rounding of P and dS before the second products (bf16 inputs only); UF = 2^-24
 for each fp32 operation, a sum of n terms counting n of them; times 1.1 for the products of two errors."""
 import math
+import random
 
 import pytest
 import torch
@@ -317,7 +318,9 @@ CASES = [  # B, N, H, Hk, D, window, sinks, causal
     (1, 127, 2, 1, 40, 40, 0, False), (1, 128, 3, 1, 80, 7, 70, True), (2, 129, 6, 2, 96, 129, 0, True),
     (1, 200, 4, 4, 64, 57, 4, False), (1, 300, 5, 5, 32, 1, 300, True), (1, 257, 2, 2, 24, 64, 130, False),
     (1, 700, 8, 2, 128, 100, 3, True), (1, 650, 3, 1, 112, 33, 200, False), (1, 1100, 2, 1, 64, 2000, 0, True),
-    (3, 385, 1, 1, 128, 128, 1, True)]
+    (3, 385, 1, 1, 128, 128, 1, True),
+    # rows beyond the window of the sinks' keys: a pass of their own, with several blocks of sinks, two-sided
+    (1, 2500, 4, 2, 64, 100, 40, True), (1, 1700, 2, 2, 128, 60, 200, False), (2, 1300, 1, 1, 96, 1300, 0, True)]
 
 
 @pytest.mark.parametrize("ty", [BF, F32])
@@ -326,6 +329,20 @@ def test_attention(B, N, H, Hk, D, window, sinks, causal, ty):
     g = gen(N + D)
     q, k, v, do = rand(g, B, N, H, D, type=ty), rand(g, B, N, Hk, D, type=ty), rand(g, B, N, Hk, D, type=ty), rand(g, B, N, H, D, type=ty)
     check_train(q, k, v, do, window, sinks, causal)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_drawn(seed):
+    """Sizes, windows, sinks, lengths and types at random."""
+    r = random.Random(seed)
+    ty = r.choice([BF, F32])
+    Hk, G, D, B = r.choice([1, 2, 3]), r.choice([1, 1, 2, 3, 5, 8]), 8 * r.randint(1, 16), r.choice([1, 2, 3])
+    N = r.choice([r.randint(1, 70), r.randint(60, 500), r.randint(400, 900)])
+    window, sinks = r.choice([1, r.randint(1, 40), r.randint(1, N), 2 * N]), r.choice([0, 1, 5, r.randint(0, N), 70])
+    lengths = [r.randint(0, N + 3) for _ in range(B)] if r.random() < 0.5 else None
+    g = gen(seed)
+    q, k, v, do = (rand(g, B, N, h, D, type=ty) for h in (Hk * G, Hk, Hk, Hk * G))
+    check_train(q, k, v, do, window, sinks, r.random() < 0.6, lengths, scale=r.choice([None, 0.3, 0.05]))
 
 
 @pytest.mark.parametrize("ty", [BF, F32])
@@ -615,6 +632,22 @@ def test_side_stream():
         got = (*got, *torch.autograd.grad(got, leaves, douts))
     torch.cuda.current_stream().wait_stream(s)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_streams_at_once():
+    """The same calls on two streams side by side: no memory is shared between calls."""
+    run, _ = token_calls()
+    want = run()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(3):
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    for out in got:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
 def token_calls():
