@@ -931,9 +931,10 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
       f16_t s = zero16(), dp = zero16();
       __builtin_amdgcn_s_setprio(1);   // 146 -> 142 us
 #pragma unroll
-      for (int st = 0; st < I::NS; ++st) s = Mma<T>::mma(im.row_frag(cur, 32 * kb, st), q[st], s);
-#pragma unroll
-      for (int st = 0; st < I::NS; ++st) dp = Mma<T>::mma(im.row_frag(cur + I::BYTES, 32 * kb, st), dof[st], dp);
+      for (int st = 0; st < I::NS; ++st) {   // two chains of dependent products, side by side
+        s = Mma<T>::mma(im.row_frag(cur, 32 * kb, st), q[st], s);
+        dp = Mma<T>::mma(im.row_frag(cur + I::BYTES, 32 * kb, st), dof[st], dp);
+      }
       __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - dl);
@@ -1123,9 +1124,8 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
       if constexpr (KLDS) kk = im.row_frag(kimg + kb * 32 * I::PITCH, 0, st);
       else kk = kf[st];
       s = Mma<T>::mma(im.row_frag(cur, 32 * rb, st), kk, s);
+      dp = Mma<T>::mma(im.row_frag(cur + RB, 32 * rb, st), vf[st], dp);
     }
-#pragma unroll
-    for (int st = 0; st < I::NS; ++st) dp = Mma<T>::mma(im.row_frag(cur + RB, 32 * rb, st), vf[st], dp);
   };
   auto products = [&](const char* cur, int buf, int r0, int rb, bool masked) {
 #pragma unroll
