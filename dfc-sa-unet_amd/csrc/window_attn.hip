@@ -331,6 +331,18 @@ template <int KT> __device__ __forceinline__ TileList tiles_of(const Span& v) {
   return t;
 }
 
+// Order of a block's LDS reads and matrix instructions: AHEAD reads, then MM products and READS reads in
+// turn, so that a product's operands are under way while the ones before it run.  Left alone the
+// compiler reads each operand just before its product and waits for it.
+template <int AHEAD, int MM, int READS, int N> __device__ __forceinline__ void interleave() {
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, MM, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+}
+
 __device__ __forceinline__ f16_t zero16() {
   f16_t z;
 #pragma unroll
@@ -935,6 +947,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
         s = Mma<T>::mma(im.row_frag(cur, 32 * kb, st), q[st], s);
         dp = Mma<T>::mma(im.row_frag(cur + I::BYTES, 32 * kb, st), dof[st], dp);
       }
+      if constexpr (sizeof(T) == 2) interleave<4, 2, 2, I::NS>();
       __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - dl);
@@ -948,6 +961,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
 #pragma unroll
         for (int d = 0; d < I::ND; ++d) dq[d] = Mma<T>::mma(im.col_frag(cur, 32 * kb, st, d), ds, dq[d]);
       }
+      if constexpr (sizeof(T) == 2) interleave<8, 1, 2, 2 * I::ND>();
     }
   };
   if (tl.n > 0) {
@@ -1126,6 +1140,7 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
       s = Mma<T>::mma(im.row_frag(cur, 32 * rb, st), kk, s);
       dp = Mma<T>::mma(im.row_frag(cur + RB, 32 * rb, st), vf[st], dp);
     }
+    if constexpr (sizeof(T) == 2) interleave<(KLDS ? 6 : 4), 2, (KLDS ? 3 : 2), I::NS>();
   };
   auto products = [&](const char* cur, int buf, int r0, int rb, bool masked) {
 #pragma unroll
@@ -1159,6 +1174,7 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
         dk[d] = Mma<T>::mma(im.col_frag(cur, 32 * rb, st, d), df, dk[d]);
       }
     }
+    if constexpr (sizeof(T) == 2) interleave<8, 1, 2, 4 * I::ND>();
     __builtin_amdgcn_s_setprio(0);
   };
 
