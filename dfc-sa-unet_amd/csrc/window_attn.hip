@@ -376,6 +376,7 @@ template <typename T, int DP> struct Online {
 #pragma unroll
       for (int st = 0; st < I::NS; ++st) s[b] = Mma<T>::mma(im.row_frag(kimg, 32 * b, st), q[st], s[b]);
     }
+    if constexpr (sizeof(T) == 2) interleave<NSUB == 2 ? 4 : 3, NSUB, NSUB, I::NS>();
     if (masked) {
       asm volatile("");   // a branch around the selects, not selects every time
 #pragma unroll
