@@ -12,8 +12,10 @@ namespace {
 // The sum of squares, rstd and the products are fp32; r is rounded to the stream's type before the
 // statistics because the stream is what the backward (and the next block) reads.
 //
-// A row is held by WAVES waves of one workgroup (1: C <= 2048, four rows per workgroup; 4: wider
-// rows), NC chunks of 8 columns per lane.
+// A row is held by WAVES waves of one workgroup (1: C <= 2048, four rows per workgroup and no barrier; 4:
+// wider rows), NC chunks of 8 columns per lane, from its one read to its writes.  Measured: 16384 rows of
+// 4096 in bf16 87 us forward (537 MB, 6.2 TB/s) and 113 us backward (537 MB, 4.75 TB/s; a large copy moves
+// 5.0); 8191 rows of 2560 to 8 bits from an fp32 stream 43 us (231 MB, 5.4 TB/s).
 constexpr int kNormMaxC = 16384;
 constexpr int kNormMaxRows = 0x7fff0000;   // a row index plus a grid's rows stays an int
 constexpr float kE4m3Max = 448.0f;
@@ -141,8 +143,9 @@ __global__ void __launch_bounds__(256) rms_fwd_kernel(int rows, int C, const T* 
 }
 
 // Backward: u = dy * w, xh = r * rstd: d = rstd (u - xh mean(u xh)) + dr; dx = T(d), dres = R(d).
-// dw is summed per workgroup over its rows (fp32) into part[gridDim.x][C]; colsum_kernel adds those in
-// a fixed order, so the result does not depend on the order workgroups run in.
+// dw is summed per workgroup over its rows (fp32) into part[gridDim.x][C]; rms_dw_kernel adds those in
+// a fixed order, so the result does not depend on the order workgroups run in.  Fetching the next row
+// before this one's sum is known measured no faster (115 us): the waves of a CU cover for each other.
 template <typename T, typename R, int WAVES, int NC>
 __global__ void __launch_bounds__(256) rms_bwd_kernel(int rows, int C, const T* __restrict__ dy,
                                                       const R* __restrict__ dr, const R* __restrict__ r,
@@ -225,7 +228,7 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(int rows, int C, const T* 
 }
 
 // out[c] = sum over n rows of part[.][c]: 16 columns per workgroup, 64 row slices of 16 threads with four
-// loads in flight each, then the slices in a fixed order
+// loads in flight each, then the slices in a fixed order (784 rows of 768: 6 us; with 8 slices 29 us)
 __global__ void __launch_bounds__(1024) rms_dw_kernel(int n, int C, const float* __restrict__ part,
                                                       float* __restrict__ out) {
   __shared__ float sm[64][17];
@@ -342,7 +345,8 @@ bool types_ok(int t, int r) { return (t == DFCSA_DT_BF16 && (r == DFCSA_DT_BF16 
 // formed in fp64 and reduced to its fraction exactly; only the fraction goes on in fp32.
 //
 // A workgroup takes tok tokens: it computes their P angles once into LDS and applies them to all heads,
-// V channels of both halves per item.  Bound by the read and the write of q and k.
+// V channels of both halves per item.  Bound by the read and the write of q and k: 16384 tokens of 16 + 4
+// heads of 128 in bf16 (168 MB) take 29 us, 5.8 TB/s.
 struct RotaryArgs {
   const void* src[2];
   void* dst[2];

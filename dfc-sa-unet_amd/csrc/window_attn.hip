@@ -642,7 +642,12 @@ __device__ __forceinline__ void exact_key(const WArgs& a, const Seq& seq, int bh
 }
 
 // ============================================================================ forward
-// 128 rows per workgroup, 32 per wave; key tiles double-buffered in LDS.
+// 128 rows per workgroup, 32 per wave; key tiles double-buffered in LDS, one barrier a tile: a tile's DMA
+// runs while the one before it is worked on.  64 KB of LDS and up to 256 registers leave two workgroups
+// on a CU, two waves on a SIMD (three with 32-key tiles measured no faster: 118 against 113 us).
+// Measured at 8192 tokens, 16 / 4 heads of 128, window 1024: 104 us, 620 TFLOP/s of the 1145 that a large
+// library product reaches here; 25 us of it are the reads of q and the writes of o, its rest and lse, the
+// matrix unit is busy 29 % of the time, the vector unit (exponentials, maxima, sums) 37 %.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wattn_fwd_kernel(const WArgs a) {
   typedef Img<T, DP> I;
@@ -705,7 +710,10 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
 }
 
 // Few rows (at most 32 per tile): the four waves share the rows and split the keys, each with its own
-// LDS ring of 32-key tiles and no barrier in the loop; joined at the end.
+// LDS ring of 32-key tiles and no barrier in the loop; joined at the end.  Bound by the caches' bytes:
+// 32 sequences, one token each over 4096 + 16 keys of 8 heads of 128 in bf16 (539 MB) take 99 us, 5.4 TB/s
+// (a large copy: 5.0).  One sequence over 1024 + 4 keys of 4 heads, split over 36 workgroups: 7.3 us + 4.1
+// for the join, all of it latency.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
   typedef Img<T, DP> I;
@@ -880,6 +888,8 @@ __global__ void __launch_bounds__(256) wattn_join_kernel(const WArgs a) {
 
 // ============================================================================ backward: dQ
 // As the forward, with S and dP per key tile; also writes delta = dO . O for the key-major pass.
+// Measured as above: 135 us, 720 TFLOP/s over its three products; its rows' q, dO, O and O's rest are
+// 134 MB of the 250 that the whole call has to move.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wattn_dq_kernel(const WArgs a) {
   typedef Img<T, DP> I;
@@ -1002,7 +1012,10 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
 // 128 keys per workgroup, 32 per wave (lane column = key); row tiles of Q and dO double-buffered in
 // LDS.  bf16 wider than 64: eight waves, two for each 32 keys, which take the two 32-row halves of a
 // tile and add up at the end through LDS (one such workgroup fills a CU: measured 284 -> 225 us at 8192
-// tokens, 16 / 4 heads of 128, window 1024, against four waves with one tile per CU).
+// tokens, 16 / 4 heads of 128, window 1024, against four waves with one tile per CU; 162 us with the far
+// rows taken out and the operands read ahead: 800 TFLOP/s over four products).  LDS reads bound it next
+// (K is read again for every row block: 320 of about 1024 cycles of a CU's LDS a block, beside the
+// products' own).  Running the two waves of a SIMD half a tile apart measured slower (185 us).
 // A workgroup takes the rows whose window reaches its keys, or one of cwin chunks of them; the rows
 // further away that see sinks are wattn_far_kernel's.  fp32 parts are added in order by wattn_dkv_join.
 __device__ __forceinline__ void key_rows(const WArgs& a, const Seq& seq, int kt, int rt, int& i0, int& i1) {
@@ -1274,6 +1287,7 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
 // Rows beyond the window of the sinks' key tiles: they see `sinks` keys only.  A workgroup has one block
 // of 32 sink keys (a.far32 of them) and one of cfar chunks of the rows; each wave runs through its own
 // row blocks with its own LDS ring, without barriers; the waves' sums are added at the end into part.
+// Measured as above (28 000 rows, 4 sinks): 18 us; as chunks of the key-major kernel the rows cost 40.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
   typedef Img<T, DP> I;
