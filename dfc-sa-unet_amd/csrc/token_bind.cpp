@@ -374,11 +374,13 @@ std::tuple<Tensor, std::optional<Tensor>> rotary(const Tensor& q, const std::opt
 }
 
 // ------------------------------------------------------------------ attention
-// strides the kernels read in place, or a contiguous copy
+// a dimension of one has whatever stride its tensor came with; it is never multiplied by more than 0
+int64_t step(const Tensor& t, int i) { return t.size(i) == 1 ? 0 : t.stride(i); }
+// strides the kernels read in place, or a contiguous copy; group: heads that a tile spans (k and v: 0)
 Tensor strided(const Tensor& t, int64_t group) {
   const int64_t es = t.element_size();
-  if (t.stride(3) != 1 || (uintptr_t)t.data_ptr() % 16 || t.stride(0) * es % 16 || t.stride(1) * es % 16 ||
-      t.stride(2) * es % 16 || t.stride(1) * es >= 1 << 23 || t.stride(2) * es * group >= 1 << 29)
+  if (t.stride(3) != 1 || (uintptr_t)t.data_ptr() % 16 || step(t, 0) * es % 16 || step(t, 1) * es % 16 ||
+      step(t, 2) * es % 16 || step(t, 1) * es >= 1 << 23 || step(t, 2) * es * group >= 1 << 29)
     return packed(t);
   return t;
 }
@@ -418,7 +420,7 @@ struct Attn {
   float scale;
 };
 void set_strides(int64_t (&s)[3], const Tensor& t) {
-  for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
+  for (int i = 0; i < 3; ++i) s[i] = step(t, i);
 }
 dfcsa_wattn_desc attn_desc(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, const Attn& p,
                            const Tensor& o, const Tensor& lse, const Tensor& rest) {
@@ -471,7 +473,7 @@ struct WindowAttention : public Function<WindowAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const Tensor& v0,
                         const std::optional<Tensor>& lengths0, int64_t window, int64_t sinks, bool causal, double scale) {
     const Tensor lengths = lengths0.value_or(Tensor());
-    const Tensor q = strided(q0, q0.size(2) / k0.size(2)), k = strided(k0, 1), v = strided(v0, 1);
+    const Tensor q = strided(q0, q0.size(2) / k0.size(2)), k = strided(k0, 0), v = strided(v0, 0);
     const Tensor lse = floats(q, q.size(0) * q.size(1) * q.size(2));
     // bf16: the backward's dO . O needs more of O than its 8 bits, so what the rounding left is kept too
     const Tensor rest = q.scalar_type() == at::kBFloat16 ? at::empty(q.sizes(), q.options()) : Tensor();
@@ -487,7 +489,7 @@ struct WindowAttention : public Function<WindowAttention> {
     first_order();
     const auto s = ctx->get_saved_variables();
     const int64_t G = s[0].size(2) / s[1].size(2);
-    const Tensor q = strided(s[0], G), k = strided(s[1], 1), v = strided(s[2], 1), dout = strided(g[0], G);
+    const Tensor q = strided(s[0], G), k = strided(s[1], 0), v = strided(s[2], 0), dout = strided(g[0], G);
     const Attn p{(int)ctx->saved_data["window"].toInt(), (int)ctx->saved_data["sinks"].toInt(),
                  ctx->saved_data["causal"].toBool(), false, (float)ctx->saved_data["scale"].toDouble()};
     const On on(q);
@@ -533,7 +535,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
   if (lengths.defined()) lengths = lengths.contiguous();
   if (wants_grad({&q, &k, &v}))
     return WindowAttention::apply(q, k, v, lengths.defined() ? std::optional<Tensor>(lengths) : std::nullopt, (int64_t)clamp32(window), (int64_t)clamp32(sinks), causal, scale);
-  return attend(strided(q, q.size(2) / k.size(2)), strided(k, 1), strided(v, 1), lengths,
+  return attend(strided(q, q.size(2) / k.size(2)), strided(k, 0), strided(v, 0), lengths,
                 Attn{clamp32(window), clamp32(sinks), causal, false, (float)scale}, Tensor(), Tensor());
 }
 
@@ -543,7 +545,7 @@ Tensor window_attention_cached(const Tensor& q, const Tensor& k, const Tensor& v
     throw std::runtime_error("window_attention_cached has no gradient: call it under torch.no_grad(), or window_attention");
   attn_check(q, k, v, window, sinks, scale, lengths);
   if (q.numel() == 0 || k.size(1) == 0) return at::zeros(q.sizes(), q.options());
-  return attend(strided(q, q.size(2) / k.size(2)), strided(k, 1), strided(v, 1), lengths.contiguous(),
+  return attend(strided(q, q.size(2) / k.size(2)), strided(k, 0), strided(v, 0), lengths.contiguous(),
                 Attn{clamp32(window), clamp32(sinks), true, true, (float)scale}, Tensor(), Tensor());
 }
 

@@ -1491,8 +1491,9 @@ bool fill(const dfcsa_wattn_desc* d, WArgs& a, bool backward) {
     if (!ptr[i] || (uintptr_t)ptr[i] % 16) return false;
     for (int j = 0; j < 3; ++j)
       if (str[i][j] < 0 || (str[i][j] * es) % 16) return false;
-    // offsets within one tile are 32 bits wide
-    if (str[i][1] * es >= (1 << 23) || str[i][2] * es * a.G >= (1 << 29)) return false;
+    // offsets within one tile are 32 bits wide (a tile of q or dout spans heads, one of k or v does not)
+    const bool rows = i == 0 || i == 3;
+    if (str[i][1] * es >= (1 << 23) || (rows && str[i][2] * es * a.G >= (1 << 29))) return false;
   }
   a.q = d->q; a.k = d->k; a.v = d->v;
   a.qb = d->q_stride[0] * es; a.qt = d->q_stride[1] * es; a.qh = d->q_stride[2] * es;

@@ -162,3 +162,12 @@ def test_attention_workspace_is_checked():
     assert LIB.dfcsa_wattn_work_floats(ctypes.addressof(d), 1, ctypes.byref(n)) == 0 and n.value > 0
     d.work_floats = n.value - 1
     assert LIB.dfcsa_wattn_bwd(ctypes.addressof(d), None) == EINVAL
+
+
+def test_attention_takes_head_major_caches():
+    # a head of k or v is a base of its own: its stride has no limit, whatever the group
+    n = ctypes.c_int64()
+    for H in (2, 16):
+        far = (1 << 40, 64, 1 << 34)
+        d = attn_desc(B=1, T=1, M=4096, H=H, Hk=2, cached=1, lengths=P16, k_stride=far, v_stride=far)
+        assert LIB.dfcsa_wattn_work_floats(ctypes.addressof(d), 0, ctypes.byref(n)) == 0

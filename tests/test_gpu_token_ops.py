@@ -765,3 +765,31 @@ def test_refusals():
     e = torch.empty(1, 0, 2, 16, device=DEV, requires_grad=True)
     assert torch.autograd.grad(t.window_attention(e, e, e, 3).sum(), e)[0].shape == e.shape
     assert t.window_attention_cached(q, q[:, :0], q[:, :0], n, 3).abs().sum() == 0
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+def test_attention_dimensions_of_one_have_any_stride(ty):
+    """One token of one head cut from rows of 9 elements: its strides are 9 although it is contiguous."""
+    g = gen(81)
+    k, v = rand(g, 1, 40, 1, 8, type=ty), rand(g, 1, 40, 1, 8, type=ty)
+    n = torch.tensor([33], dtype=torch.int32, device=DEV)
+    wide = rand(g, 1, 1, 1, 9, type=ty)
+    for q in (wide[..., :8], wide[..., 1:]):   # the second is misaligned as well
+        assert torch.equal(tk().window_attention_cached(q, k, v, n, 20, 2),
+                           tk().window_attention_cached(q.reshape(8).clone().view(1, 1, 1, 8), k, v, n, 20, 2))
+        leaves = [t.detach().requires_grad_() for t in (q, q + 1, q - 1)]
+        do = rand(g, 1, 1, 1, 9, type=ty)[..., 1:]
+        check_train(*leaves, do, 1, 0, True)
+
+
+def test_attention_head_major_cache():
+    cap, Hk, D = 1 << 18, 2, 128   # 8 query heads of a key head times 2^26 bytes reach 2^29
+    g = gen(82)
+    k, v = (torch.zeros(1, Hk, cap, D, dtype=BF, device=DEV).transpose(1, 2) for _ in range(2))
+    for t in (k, v):
+        t[0, -500:] = rand(g, 500, Hk, D, type=BF)
+        t[0, :4] = rand(g, 4, Hk, D, type=BF)
+    q = rand(g, 1, 1, 16, D, type=BF)
+    n = torch.tensor([cap], dtype=torch.int32, device=DEV)
+    assert torch.equal(tk().window_attention_cached(q, k, v, n, 300, 4),
+                       tk().window_attention_cached(q, k.contiguous(), v.contiguous(), n, 300, 4))
