@@ -218,6 +218,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_residual_q8(const Tensor& x0, const 
 }
 
 Tensor dequant_q8(const Tensor& y8, const Tensor& scales, at::ScalarType out) {
+  if (wants_grad({&scales})) throw std::runtime_error("dequant_q8 has no gradient: call it under torch.no_grad()");
   need_gpu({&y8, &scales});
   if (y8.scalar_type() != at::kFloat8_e4m3fn || scales.scalar_type() != at::kFloat)
     bad_type("float8_e4m3fn values and float32 scales are needed, got " + name(y8.scalar_type()) + " and " +
@@ -386,7 +387,7 @@ Tensor strided(const Tensor& t, int64_t group) {
 }
 
 void attn_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale,
-                const Tensor& lengths) {
+                const Tensor& lengths, bool cached) {
   need_gpu({&q, &k, &v, &lengths});
   dtype_of(q, "q");
   if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
@@ -412,6 +413,12 @@ void attn_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t windo
   const int64_t G = H / Hk;
   if (T > INT_MAX || M > INT_MAX || T * G > 1 << 29 || M * G > 1 << 29 || B * Hk > 1 << 24)
     bad_value("at most 2^29 tokens times heads per key head, and 2^24 sequences times key heads");
+  // tiles of 128 rows or keys: what one launch of the kernels can hold (cached: the rows alone count)
+  const int64_t long_side = std::max(T * G, cached ? 0 : M);
+  if (B * Hk * std::max<int64_t>((long_side + 127) / 128, 1) >= (1 << 23) - 8)
+    bad_value("sequences times key heads times tiles of 128 tokens: fewer than 2^23 - 8 are needed");
+  if (H * D * q.element_size() >= 1 << 23) bad_value("a token of q: less than 2^23 bytes are needed");
+  if (!std::isfinite((float)scale * 1.5f)) bad_value("scale: too large for float32 scores");
 }
 
 struct Attn {
@@ -527,7 +534,7 @@ int clamp32(int64_t v) { return (int)std::min<int64_t>(v, INT_MAX); }
 Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, bool causal,
                         double scale, const std::optional<Tensor>& lengths0) {
   Tensor lengths = lengths0.value_or(Tensor());
-  attn_check(q, k, v, window, sinks, scale, lengths);
+  attn_check(q, k, v, window, sinks, scale, lengths, false);
   if (k.size(1) != q.size(1))
     bad_value(std::to_string(q.size(1)) + " queries and " + std::to_string(k.size(1)) +
               " keys: as many are needed (or window_attention_cached)");
@@ -543,7 +550,7 @@ Tensor window_attention_cached(const Tensor& q, const Tensor& k, const Tensor& v
                                int64_t sinks, double scale) {
   if (wants_grad({&q, &k, &v}))
     throw std::runtime_error("window_attention_cached has no gradient: call it under torch.no_grad(), or window_attention");
-  attn_check(q, k, v, window, sinks, scale, lengths);
+  attn_check(q, k, v, window, sinks, scale, lengths, true);
   if (q.numel() == 0 || k.size(1) == 0) return at::zeros(q.sizes(), q.options());
   return attend(strided(q, q.size(2) / k.size(2)), strided(k, 0), strided(v, 0), lengths.contiguous(),
                 Attn{clamp32(window), clamp32(sinks), true, true, (float)scale}, Tensor(), Tensor());

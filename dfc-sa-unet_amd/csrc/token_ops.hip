@@ -7,6 +7,14 @@
 
 namespace {
 
+// Workgroups of 256 threads in a grid of two dimensions where they are many: a launch counts the
+// threads of one dimension in 32 bits.
+dim3 grid2(int64_t groups) {
+  const int64_t y = (groups + (1 << 22) - 1) >> 22;
+  return dim3((unsigned)((groups + y - 1) / y), (unsigned)y);
+}
+__device__ __forceinline__ int64_t group2() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // ============================================================================ RMS norm
 // r = R(x + res); y = T(r * rstd * w), rstd = rsqrt(mean(r^2) + eps).
 // The sum of squares, rstd and the products are fp32; r is rounded to the stream's type before the
@@ -256,7 +264,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) dequant_kernel(int64_t n8, int C8, int gsh, int ng,
                                                       const uint2* __restrict__ y8, const float* __restrict__ scales,
                                                       T* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = group2() * 256 + threadIdx.x;
   if (i >= n8) return;
   const int64_t row = i / C8;
   const int c8 = (int)(i - row * C8);
@@ -366,7 +374,8 @@ constexpr int kRotLds = 256;   // angles (cos, sin) a workgroup holds
 template <typename T, int V>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   __shared__ __attribute__((aligned(16))) float cs[kRotLds], sn[kRotLds];
-  const int64_t tokens = (int64_t)a.B * a.N, t0 = (int64_t)blockIdx.x * a.tok;
+  const int64_t tokens = (int64_t)a.B * a.N, t0 = group2() * a.tok;
+  if (t0 >= tokens) return;
   const int nt = (int)min((int64_t)a.tok, tokens - t0);
   for (int e = threadIdx.x; e < nt * a.P; e += 256) {
     const int tl = e / a.P, j = e - tl * a.P;
@@ -441,7 +450,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
 template <typename T>
 void launch_rotary(const RotaryArgs& a, bool vec, hipStream_t st) {
   const int64_t tokens = (int64_t)a.B * a.N;
-  const dim3 grid((unsigned)((tokens + a.tok - 1) / a.tok));
+  const dim3 grid = grid2((tokens + a.tok - 1) / a.tok);
   if (vec) hipLaunchKernelGGL((rotary_kernel<T, 8>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((rotary_kernel<T, 1>), grid, dim3(256), 0, st, a);
 }
@@ -496,10 +505,10 @@ int dfcsa_dequant_q8(int dtype, int64_t rows, int C, int group, const void* y8, 
   if (blocks > 0x7fffffff) return DFCSA_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DFCSA_DT_F32)
-    hipLaunchKernelGGL((dequant_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, st, n8, C / 8, gsh, C / group,
+    hipLaunchKernelGGL((dequant_kernel<float>), grid2(blocks), dim3(256), 0, st, n8, C / 8, gsh, C / group,
                        (const uint2*)y8, scales, (float*)out);
   else if (dtype == DFCSA_DT_BF16)
-    hipLaunchKernelGGL((dequant_kernel<bf16_t>), dim3((unsigned)blocks), dim3(256), 0, st, n8, C / 8, gsh,
+    hipLaunchKernelGGL((dequant_kernel<bf16_t>), grid2(blocks), dim3(256), 0, st, n8, C / 8, gsh,
                        C / group, (const uint2*)y8, scales, (bf16_t*)out);
   else
     return DFCSA_EINVAL;

@@ -29,6 +29,7 @@
 // without bank conflicts from the same image.  Rows no query of the workgroup sees load as zeros (the
 // buffer descriptor's bounds check), so what lies in padding is never multiplied.
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 #include "dfcsa_internal.h"
@@ -1468,7 +1469,7 @@ __global__ void __launch_bounds__(256) wattn_dkv_join_kernel(const WArgs a) {
 bool fill(const dfcsa_wattn_desc* d, WArgs& a, bool backward) {
   if (!d || (d->dtype != DFCSA_DT_F32 && d->dtype != DFCSA_DT_BF16)) return false;
   if (d->B <= 0 || d->T <= 0 || d->M <= 0 || d->H <= 0 || d->Hk <= 0 || d->H > 65536 || d->H % d->Hk || d->D < 8 || d->D % 8 ||
-      d->D > 128 || d->window < 1 || d->sinks < 0 || !(d->scale > 0.f) || !d->q || !d->k || !d->v || !d->o)
+      d->D > 128 || d->window < 1 || d->sinks < 0 || !(d->scale > 0.f) || !std::isfinite(d->scale * kLog2e) || !d->q || !d->k || !d->v || !d->o)
     return false;
   if (!d->cached && d->T != d->M) return false;
   if (d->cached && (!d->lengths || backward || !d->causal)) return false;
@@ -1516,6 +1517,12 @@ bool fill(const dfcsa_wattn_desc* d, WArgs& a, bool backward) {
   return true;
 }
 
+// a launch counts its threads in 32 bits (groups are padded to a multiple of 8)
+bool fits(int64_t groups, int threads) { return (groups + 7) * threads < (int64_t)1 << 32; }
+int dkv_threads(const WArgs& a, bool f32) { return !f32 && a.D > 64 ? 512 : 256; }
+// threads of the join over ntile key tiles
+int64_t join_items(const WArgs& a, int64_t ntile) { return ntile * 128 * (2 * a.D / 4) * a.B * a.Hk; }
+
 // The forward's plan: few = the kernel whose waves split the keys of 32 rows; splits over the keys
 // where the row tiles alone do not fill the card.  The estimate is in rounds of the waves (few: 128
 // keys, else a tile of 64 or 32), 3 of which a workgroup takes to start and end, and the join about as
@@ -1561,6 +1568,7 @@ void plan_bwd(WArgs& a, bool f32) {
   double best = 0;
   a.cwin = 1;
   for (int c = 1; c <= 8 && c <= std::max<int64_t>(1, wt / 2); ++c) {
+    if (c > 1 && !(fits(a.tiles * bh * c, 512) && join_items(a, a.tiles) < (int64_t)1 << 30)) break;
     const double rounds = (double)((a.tiles * bh * c + slots - 1) / slots);
     double t = rounds * ((double)((wt + c - 1) / c) + 4) * tile;
     if (c > 1) t += 4 + (double)c * a.M * bh * a.D * 16 / 5e6;
@@ -1575,7 +1583,7 @@ void plan_bwd(WArgs& a, bool f32) {
   const int64_t far = std::max<int64_t>(high, 0) + std::max<int64_t>(low, 0);
   a.far32 = a.cfar = 0;
   // a pass of their own costs two launches, about 12 us; without it the sinks' tiles take the far rows too
-  if (a.sinks > 0 && (double)(far * a.G / rt) * tile > 12) {
+  if (a.sinks > 0 && (double)(far * a.G / rt) * tile > 12 && join_items(a, a.nsink) < (int64_t)1 << 30) {
     a.far32 = (a.sinks + 31) / 32;
     const int64_t blocks = (far * a.G + 31) / 32, base = bh * a.far32;
     a.cfar = (int)std::max<int64_t>(1, std::min<int64_t>({(256 + base - 1) / base, blocks / 8, 64}));
@@ -1614,7 +1622,7 @@ int run_bwd(WArgs a, hipStream_t st) {
   }
   DFCSA_CHECK_LAUNCH();
   const int bh = a.B * a.Hk;
-  BY_WIDTH(wattn_dkv_kernel, dim3((unsigned)xcd_pad(a.tiles * a.cwin * bh)), sizeof(T) == 2 && a.D > 64 ? 512 : 256, a);
+  BY_WIDTH(wattn_dkv_kernel, dim3((unsigned)xcd_pad(a.tiles * a.cwin * bh)), dkv_threads(a, sizeof(T) == 4), a);
   DFCSA_CHECK_LAUNCH();
   if (a.cfar) {
     BY_WIDTH(wattn_far_kernel, dim3((unsigned)xcd_pad(a.far32 * a.cfar * bh)), 256, a);
@@ -1622,7 +1630,7 @@ int run_bwd(WArgs a, hipStream_t st) {
   }
   const int ntile = a.cwin > 1 ? a.tiles : (a.cfar ? a.nsink : 0);
   if (ntile) {
-    const int64_t e = (int64_t)ntile * 128 * (2 * a.D / 4) * bh;
+    const int64_t e = join_items(a, ntile);
     hipLaunchKernelGGL((wattn_dkv_join_kernel<T>), dim3((unsigned)((e + 255) / 256)), dim3(256), 0, st, a);
     DFCSA_CHECK_LAUNCH();
   }
@@ -1652,7 +1660,8 @@ int dfcsa_wattn_fwd(const dfcsa_wattn_desc* d, void* stream) {
   if (!fill(d, a, false)) return DFCSA_EINVAL;
   bool few;
   plan_fwd(a, d->dtype == DFCSA_DT_F32, few);
-  if ((int64_t)a.tiles * a.B * a.Hk * a.splits > 0x7ffffff0) return DFCSA_EINVAL;
+  if (!fits((int64_t)a.tiles * a.B * a.Hk * a.splits, 256)) return DFCSA_EINVAL;
+  if (a.splits > 1 && !fits(((int64_t)a.B * a.Hk * a.R + 7) / 8, 256)) return DFCSA_EINVAL;
   if (fwd_work(a) > 0 && (!d->work || d->work_floats < fwd_work(a))) return DFCSA_EINVAL;
   return d->dtype == DFCSA_DT_F32 ? run_fwd<float>(a, few, (hipStream_t)stream) : run_fwd<bf16_t>(a, few, (hipStream_t)stream);
 }
@@ -1661,7 +1670,10 @@ int dfcsa_wattn_bwd(const dfcsa_wattn_desc* d, void* stream) {
   WArgs a;
   if (!fill(d, a, true)) return DFCSA_EINVAL;
   plan_bwd(a, d->dtype == DFCSA_DT_F32);
-  if (((int64_t)a.tiles * a.cwin + (int64_t)a.far32 * a.cfar + (a.R + 127) / 128) * a.B * a.Hk > 0x7ffffff0) return DFCSA_EINVAL;
+  const int64_t bh = (int64_t)a.B * a.Hk;
+  if (!fits((a.R + 127) / 128 * bh, 256) || !fits((int64_t)a.tiles * a.cwin * bh, dkv_threads(a, d->dtype == DFCSA_DT_F32)) ||
+      !fits((int64_t)a.far32 * a.cfar * bh, 256))
+    return DFCSA_EINVAL;
   if (bwd_work(a) > 0 && (!d->work || d->work_floats < bwd_work(a))) return DFCSA_EINVAL;
   return d->dtype == DFCSA_DT_F32 ? run_bwd<float>(a, (hipStream_t)stream) : run_bwd<bf16_t>(a, (hipStream_t)stream);
 }

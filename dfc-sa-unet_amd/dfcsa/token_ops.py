@@ -40,10 +40,13 @@ E4M3 = torch.float8_e4m3fn
 
 
 def _whole(v, what):
-    i = int(v)
+    try:
+        i = int(v)
+    except OverflowError:   # infinity
+        raise ValueError(f"{what} {v}: a whole number is needed") from None
     if i != v:
         raise ValueError(f"{what} {v}: a whole number is needed")
-    return i
+    return max(-1 << 62, min(i, 1 << 62))   # more than there are tokens is as good as any number of them
 
 
 # ------------------------------------------------------------------ RMS norm of the residual stream
@@ -92,7 +95,7 @@ def rotary(q, k, positions, axes, base=10000.0, shared=False, interleaved=False)
 
 # ------------------------------------------------------------------ attention
 def _scale(scale, q):
-    return 1.0 / math.sqrt(q.shape[-1] or 1) if scale is None else float(scale)
+    return 1.0 / math.sqrt(q.shape[-1] if q.dim() and q.shape[-1] else 1) if scale is None else float(scale)
 
 
 def window_attention(q, k, v, window, sinks=0, causal=True, scale=None, lengths=None):

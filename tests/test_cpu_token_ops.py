@@ -171,3 +171,25 @@ def test_attention_takes_head_major_caches():
         far = (1 << 40, 64, 1 << 34)
         d = attn_desc(B=1, T=1, M=4096, H=H, Hk=2, cached=1, lengths=P16, k_stride=far, v_stride=far)
         assert LIB.dfcsa_wattn_work_floats(ctypes.addressof(d), 0, ctypes.byref(n)) == 0
+
+
+@pytest.mark.parametrize("over", [dict(B=1 << 23, T=1, M=1, sinks=0), dict(B=1 << 14, T=1 << 17, M=1 << 17, H=2, Hk=1, D=8)])
+def test_attention_launches_past_32_bits_are_refused(over):
+    # 2^24 workgroups of 256 threads and more
+    d = attn_desc(**over)
+    assert LIB.dfcsa_wattn_fwd(ctypes.addressof(d), None) == EINVAL
+    assert LIB.dfcsa_wattn_bwd(ctypes.addressof(d), None) == EINVAL
+
+
+def test_argument_corners():
+    q, n = torch.randn(1, 4, 2, 8), torch.ones(1, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        tk.window_attention(q, q, q, float("inf"))
+    with pytest.raises(ValueError):
+        tk.window_attention_cached(q, q, q, n, 2, float("inf"))
+    for call in (lambda: tk.window_attention(q, q, q, 1 << 70), lambda: tk.window_attention(q[0, 0, 0, 0], q, q, 2)):
+        with pytest.raises(RuntimeError, match="GPU"):   # so the arguments before it are taken
+            call()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        tk.dequant_q8(torch.zeros(2, 8).to(tk.E4M3), torch.ones(2, 1, requires_grad=True))
+    assert LIB.dfcsa_wattn_fwd(ctypes.addressof(attn_desc(scale=3e38)), None) == EINVAL

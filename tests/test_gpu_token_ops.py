@@ -793,3 +793,40 @@ def test_attention_head_major_cache():
     n = torch.tensor([cap], dtype=torch.int32, device=DEV)
     assert torch.equal(tk().window_attention_cached(q, k, v, n, 300, 4),
                        tk().window_attention_cached(q, k.contiguous(), v.contiguous(), n, 300, 4))
+
+
+def test_many_workgroups():
+    """More than 2^22 workgroups of rotary and dequant_q8: a grid of two dimensions, against two halves."""
+    t, g = tk(), gen(83)
+    N, D = (1 << 22) + 5, 272   # one token a workgroup
+    q = rand(g, 1, N, 1, D, type=BF)
+    pos = torch.arange(N, dtype=torch.int32, device=DEV)[:, None]
+    whole, _ = t.rotary(q, None, pos, (136,))
+    for part in (slice(0, N // 2), slice(N // 2, N)):
+        assert torch.equal(whole[:, part], t.rotary(q[:, part], None, pos[part], (136,))[0])
+    del q, whole
+    rows, C = (1 << 19) + 1, 16384   # 2^33 elements and one row
+    y8 = torch.empty(rows, C, dtype=torch.uint8, device=DEV).random_(0, 127, generator=g).view(t.E4M3)   # no NaN
+    s = rand(g, rows, 1)
+    whole = t.dequant_q8(y8, s)
+    for part in (slice(0, rows // 2), slice(rows // 2, rows)):
+        assert torch.equal(whole[part], t.dequant_q8(y8[part], s[part]))
+    assert torch.equal(whole[-1].float(), (y8[-1].float() * s[-1]).to(BF).float())
+    del y8, whole
+    torch.cuda.empty_cache()
+
+
+def test_attention_limits_are_refused():
+    t = tk()
+    q = torch.zeros(1, 1, 1, 8, dtype=BF, device=DEV).expand(1 << 23, 1, 1, 8)
+    with pytest.raises(ValueError, match="2\\^23"):
+        t.window_attention(q, q, q, 1)
+    wide = torch.zeros(1, 1, 1, 128, dtype=F32, device=DEV).expand(1, 1, 1 << 14, 128)
+    with pytest.raises(ValueError, match="token of q"):
+        t.window_attention(wide, wide, wide, 1)
+    q = torch.zeros(1, 3, 1, 8, device=DEV)
+    with pytest.raises(ValueError, match="scale"):
+        t.window_attention(q, q, q, 1, scale=3e38)
+    # a window of more than all tokens, however large
+    q = rand(gen(84), 1, 40, 2, 8)
+    assert torch.equal(t.window_attention(q, q, q, 1 << 70), t.window_attention(q, q, q, 40))
