@@ -1418,7 +1418,7 @@ __global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
 #pragma unroll 1
     for (int i = wave; i < 32; i += 4) {
       float* p = out + i * 2 * a.D;
-      if (kw + i < min(a.sinks, seq.len))
+      if (kw + i < a.sinks)   // the join reads these, padding too (zeros)
         exact_key<T, float>(a, seq, bh, kw + i, b0 * 32, l1 * 32, h0 * 32, h1 * 32, p, p + a.D);
     }
   }

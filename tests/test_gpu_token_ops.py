@@ -830,3 +830,18 @@ def test_attention_limits_are_refused():
     # a window of more than all tokens, however large
     q = rand(gen(84), 1, 40, 2, 8)
     assert torch.equal(t.window_attention(q, q, q, 1 << 70), t.window_attention(q, q, q, 40))
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+def test_attention_infinite_far_row_and_padded_sinks(ty):
+    """More sinks than the sequence has tokens, and an infinite gradient in a row far from them: the keys
+    behind the sequence's end still get zeros."""
+    g = gen(85)
+    N, n, D = 2048, 390, 64
+    q, k, v, do = (rand(g, 1, N, 1, D, type=ty) for _ in range(4))
+    do[0, 10] = math.inf
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    o = tk().window_attention(*leaves, 8, 400, causal=False, lengths=lens)
+    for d in torch.autograd.grad(o, leaves, do):
+        assert torch.equal(d[0, n:], torch.zeros_like(d[0, n:]))
