@@ -520,7 +520,8 @@ __device__ __forceinline__ void finish_rows(const WArgs& a, int bh, int split, i
 // A product of matrix tiles multiplies every element of both: where a hidden key's P is 0 and its V (or K,
 // or a hidden row's Q or dO) is infinite or NaN, the 0 * inf reaches rows that do not see it.  Nothing is
 // tested for that in the loops; a wave whose results are not all finite forms them again here, from the
-// visible pairs alone, one row (or key) at a time with two columns per lane.
+// visible pairs alone, one row (or key) at a time with two columns per lane.  A sum that is NaN in all
+// columns stays it, so a row that sees a NaN ends there and inputs of nothing but NaN cost little.
 __device__ __forceinline__ bool finite_all(const f16_t& v) {
   bool ok = true;
 #pragma unroll
@@ -572,6 +573,11 @@ __device__ __forceinline__ void exact_row(const WArgs& a, const Seq& seq, int bh
       o0 = o0 * al + p * v.x;
       o1 = o1 * al + p * v.y;
       m = mn;
+      if (l != l) {   // the same in all lanes: every column is NaN from here on
+        o0 = o1 = l;
+        it = it1;
+        break;
+      }
     }
   const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
   const float lse = l == 0.f ? kNegInf : m + __builtin_amdgcn_logf(l);
@@ -610,6 +616,10 @@ __device__ __forceinline__ void exact_dq(const WArgs& a, const Seq& seq, int bh,
       const float ds = __builtin_amdgcn_exp2f(s * a.scale2 - lse) * (dp - dl);
       d0 += ds * k.x;
       d1 += ds * k.y;
+      if (ds != ds) {
+        it = tl.n;
+        break;
+      }
     }
   put_two<T>((T*)a.dq + (((int64_t)b * a.T + x.t) * a.H + hk * a.G + x.g) * a.D, d, a.D, d0 * a.scale, d1 * a.scale);
 }
@@ -636,6 +646,7 @@ __device__ __forceinline__ void exact_key(const WArgs& a, const Seq& seq, int bh
       k1 += ds * q.y;
       v0 += p * g.x;
       v1 += p * g.y;
+      if (p != p) break;
     }
   }
   put_two<O>(outk, d, a.D, k0 * a.scale, k1 * a.scale);

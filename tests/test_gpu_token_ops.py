@@ -845,3 +845,22 @@ def test_attention_infinite_far_row_and_padded_sinks(ty):
     o = tk().window_attention(*leaves, 8, 400, causal=False, lengths=lens)
     for d in torch.autograd.grad(o, leaves, do):
         assert torch.equal(d[0, n:], torch.zeros_like(d[0, n:]))
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+def test_attention_of_nothing_but_nan(which, ty):
+    """Every result that depends on a NaN is NaN, padding keeps its zeros."""
+    g = gen(86)
+    N, n = 700, 690
+    t = [rand(g, 1, N, h, 64, type=ty) for h in (4, 2, 2, 4)]
+    t[which].fill_(math.nan)
+    leaves = [x.requires_grad_() for x in t[:3]]
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    o = tk().window_attention(*leaves, 50, 4, lengths=lens)
+    got = (o, *torch.autograd.grad(o, leaves, t[3]))
+    # v reaches dS through dO . (V - O); dV is P^T dO, which knows of q, k and dO; O of all but dO
+    hit = {0: (1, 1, 1, 1), 1: (1, 1, 1, 1), 2: (1, 1, 1, 0), 3: (0, 1, 1, 1)}[which]
+    for x, nan in zip(got, hit):
+        assert torch.isnan(x[0, :n]).all() if nan else torch.isfinite(x[0, :n]).all()
+        assert torch.equal(x[0, n:], torch.zeros_like(x[0, n:]))
