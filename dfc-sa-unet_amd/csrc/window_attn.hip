@@ -22,7 +22,7 @@
 // operand is read from LDS in that order -- transposed by ds_read_b64_tr_b16 for bf16.  P and dS are
 // rounded to bf16 for that second product (bf16 inputs only): at most 2^-8 of each, which the sum over a
 // row's keys averages; the results' error is 1.4 times that of rounding the exact ones (measured 0.0024
-// against 0.0017 of their norm).  What bounds each kernel, and what was measured, stands at it.
+// against 0.0017 of their norm; with few visible keys up to 1.6 times).  What bounds each kernel, and what was measured, stands at it.
 //
 // LDS images hold one row per key (or query row) with 16-byte chunks XOR-swizzled by the row, on the
 // source side of an LDS-DMA load: rows are read by 16-byte reads and columns by transposing reads
@@ -48,7 +48,13 @@ typedef __attribute__((address_space(3))) s4_t lds_s4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
-constexpr float kGrow = 8.0f;   // the running maximum moves only when a row outgrows it by 2^8
+// The running maximum moves only when a row outgrows it by 2^kGrow (at 8192 tokens, window 1024: 105 us
+// against 111).  A row's largest P is then no longer 1 and rounds to bf16 like the others.  Over many keys
+// that averages out; with few it does not (2 sinks and a window of 3, width 8: dK's error 0.0031 instead of
+// 0.0025 of its norm), so row tiles that visit at most kFewTiles key tiles, and the kernel for few rows,
+// which waits for memory anyway, follow the maximum exactly.
+constexpr float kGrow = 8.0f;
+constexpr int kFewTiles = 8;
 
 struct WArgs {
   int B, T, M, H, Hk, G, D, R;
@@ -355,7 +361,7 @@ __device__ __forceinline__ f16_t zero16() {
 template <typename T, int DP> struct Online {
   typedef Img<T, DP> I;
   typedef typename I::frag frag;
-  float m, l;        // maximum (log2 units, lags by at most kGrow), this half's sum
+  float m, l;        // maximum (log2 units), this half's sum
   f16_t o[I::ND];    // O^T: column = row of the tile, rows = head columns
   __device__ __forceinline__ void init() {
     m = kNegInf;
@@ -365,10 +371,10 @@ template <typename T, int DP> struct Online {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   }
-  // NSUB blocks of 32 keys from key0
+  // NSUB blocks of 32 keys from key0; the maximum lags by at most grow
   template <int NSUB>
   __device__ __forceinline__ void step(const I& im, const char* kimg, const char* vimg, int key0, const frag (&q)[I::NS],
-                                       float scale2, bool masked, const RowMask& mask, int lane) {
+                                       float scale2, bool masked, const RowMask& mask, int lane, float grow) {
     f16_t s[NSUB];
     float mx = kNegInf;
 #pragma unroll
@@ -388,7 +394,7 @@ template <typename T, int DP> struct Online {
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scale2;
-    if (__any(mx > m + kGrow || (m == kNegInf && mx > kNegInf))) {
+    if (__any(mx > m + grow || (m == kNegInf && mx > kNegInf))) {
       asm volatile("");   // keeps this a branch: as selects, the 16 ND products would run every time
       const float mn = fmaxf(m, mx);
       const float al = mn == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -706,7 +712,8 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
     }
     const int key0 = tl[it] * KT;
     if (sees_any(my, key0, key0 + KT))
-      st.template step<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane);
+      st.template step<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane,
+                                tl.n <= kFewTiles ? 0.f : kGrow);
   }
   const float lsum = st.l + __shfl_xor(st.l, 32, 64);
   lds_barrier();   // the tiles are read
@@ -780,7 +787,7 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
       wait_vm<0>();
     }
     const int key0 = tl[it] * KT;
-    st.template step<1>(im, c, c + IB, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane);
+    st.template step<1>(im, c, c + IB, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane, 0.f);
     if (STG == 1 && it + 4 < it1) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       dma.issue(kbase, a.kt, tl[it + 4] * KT, my.lo, my.hi, my.sl, n, 0);
