@@ -1574,7 +1574,8 @@ int64_t fwd_work(const WArgs& a) { return a.splits == 1 ? 0 : (int64_t)a.splits 
 // workgroups than run at once cost a second round of them all, too few leave CUs idle, and more than
 // one chunk costs the fp32 parts' way to memory and back.  Estimated in microseconds: a row tile is 2
 // (bf16, width 128; 64 x 128 pairs) or 6 (fp32, 32 x 128), a workgroup starts and ends in 4 of them, the
-// parts move at 5 TB/s behind a 4 us launch.  The far rows are cut to a workgroup for each CU.
+// parts move at 5 TB/s behind a 4 us launch.  The far rows are cut to a workgroup for each CU, a block of 32
+// rows for each of its waves (two blocks: 21 instead of 14 us in fp32, 3 x 1531 tokens, 6 / 2 heads of 80).
 void plan_bwd(WArgs& a, bool f32) {
   a.tiles = (a.M + 127) / 128;
   a.nsink = (a.sinks + 127) / 128;
@@ -1604,7 +1605,7 @@ void plan_bwd(WArgs& a, bool f32) {
   if (a.sinks > 0 && (double)(far * a.G / rt) * tile > 12 && join_items(a, a.nsink) < (int64_t)1 << 30) {
     a.far32 = (a.sinks + 31) / 32;
     const int64_t blocks = (far * a.G + 31) / 32, base = bh * a.far32;
-    a.cfar = (int)std::max<int64_t>(1, std::min<int64_t>({(256 + base - 1) / base, blocks / 8, 64}));
+    a.cfar = (int)std::max<int64_t>(1, std::min<int64_t>({(256 + base - 1) / base, blocks / 4, 64}));
   }
 }
 int64_t bwd_work(const WArgs& a) { return far_at(a) + (int64_t)a.B * a.Hk * a.far32 * a.cfar * 32 * 2 * a.D; }
