@@ -415,8 +415,8 @@ void attn_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t windo
     bad_value("at most 2^29 tokens times heads per key head, and 2^24 sequences times key heads");
   // tiles of 128 rows or keys: what one launch of the kernels can hold (cached: the rows alone count)
   const int64_t long_side = std::max(T * G, cached ? 0 : M);
-  if (B * Hk * std::max<int64_t>((long_side + 127) / 128, 1) >= (1 << 23) - 8)
-    bad_value("sequences times key heads times tiles of 128 tokens: fewer than 2^23 - 8 are needed");
+  if (B * Hk * std::max<int64_t>((long_side + 127) / 128, 1) >= (1 << 23) - 24)
+    bad_value("sequences times key heads times tiles of 128 tokens: fewer than 2^23 - 24 are needed");
   if (H * D * q.element_size() >= 1 << 23) bad_value("a token of q: less than 2^23 bytes are needed");
   if (!std::isfinite((float)scale * 1.5f)) bad_value("scale: too large for float32 scores");
 }

@@ -864,3 +864,57 @@ def test_attention_of_nothing_but_nan(which, ty):
     for x, nan in zip(got, hit):
         assert torch.isnan(x[0, :n]).all() if nan else torch.isfinite(x[0, :n]).all()
         assert torch.equal(x[0, n:], torch.zeros_like(x[0, n:]))
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("B,N,H,Hk,D,window,sinks,causal,lengths", [
+    (3, 700, 6, 2, 80, 90, 7, True, [700, 320, 0]), (3, 700, 2, 2, 128, 200, 0, False, [1, 700, 128]),
+    (5, 400, 4, 1, 64, 50, 4, True, [129, 127, 128, 400, 3]), (2, 1500, 2, 1, 128, 400, 40, True, [200, 1400]),
+    (4, 130, 3, 1, 32, 130, 0, False, [0, 0, 130, 0]), (2, 300, 2, 2, 40, 60, 0, True, [0, 0])])
+def test_attention_padded_tiles(B, N, H, Hk, D, window, sinks, causal, lengths, ty):
+    """Padding of all sizes: live tiles are dealt out first, and the backward cuts them by how many there are."""
+    g = gen(B * N + D)
+    q, k, v, do = (rand(g, B, N, h, D, type=ty) for h in (H, Hk, Hk, H))
+    first = check_train(q, k, v, do, window, sinks, causal, lengths)
+    for a, b in zip(first, check_train(q, k, v, do, window, sinks, causal, lengths)):
+        assert torch.equal(a, b)
+    for b, n in enumerate(lengths):
+        for x in first:
+            assert torch.equal(x[b, n:], torch.zeros_like(x[b, n:]))
+
+
+@pytest.mark.parametrize("B", [63, 64, 65])
+def test_attention_many_padded_sequences(B):
+    """Up to 64 sequences' lengths are looked through by a workgroup; more take the plain order."""
+    g = gen(B)
+    N = 150
+    q, k, v, do = (rand(g, B, N, 2, 32, type=BF) for _ in range(4))
+    check_train(q, k, v, do, 40, 2, True, [(37 * b) % (N + 1) for b in range(B)])
+
+
+def test_attention_padded_graph_with_other_lengths():
+    """A captured call finds its tiles by the lengths of the replay, not of the capture."""
+    t, g = tk(), gen(87)
+    q, k, v, do = (rand(g, 3, 600, h, 64, type=F32) for h in (6, 2, 2, 6))
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    n = torch.tensor([600, 600, 600], dtype=torch.int32, device=DEV)
+
+    def run():
+        o = t.window_attention(*leaves, 90, 3, lengths=n)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for lens in ([600, 10, 300], [0, 0, 0], [5, 600, 129], [600, 600, 600]):
+        n.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in out]
+        for a, b in zip(got, run()):
+            assert torch.equal(a, b)
