@@ -22,7 +22,10 @@
 // operand is read from LDS in that order -- transposed by ds_read_b64_tr_b16 for bf16.  P and dS are
 // rounded to bf16 for that second product (bf16 inputs only): at most 2^-8 of each, which the sum over a
 // row's keys averages; the results' error is 1.4 times that of rounding the exact ones (measured 0.0024
-// against 0.0017 of their norm; with few visible keys up to 1.6 times).  What bounds each kernel, and what was measured, stands at it.
+// against 0.0017 of their norm; with few visible keys up to 1.6 times).  The kernel for few rows waits for
+// memory, so it multiplies P as two bf16, the second one what the first rounded off: its error is the
+// results' own rounding (cached, 1000 keys: 0.0020 -> 0.0016 of their norm; 101 us before and after at 32
+// sequences).  What bounds each kernel, and what was measured, stands at it.
 //
 // LDS images hold one row per key (or query row) with 16-byte chunks XOR-swizzled by the row, on the
 // source side of an LDS-DMA load: rows are read by 16-byte reads and columns by transposing reads
@@ -172,6 +175,16 @@ template <> struct Mma<bf16_t> {
     union { uint32_t u[4]; frag f; } r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) r.u[i] = cvt2(p[8 * st + 2 * i], p[8 * st + 2 * i + 1]);
+    return r.f;
+  }
+  // what pack() rounded off, as a fragment of its own
+  __device__ __forceinline__ static frag pack_rest(const f16_t& p, int st, const frag& hi) {
+    union { uint32_t u[4]; frag f; } h, r;
+    h.f = hi;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r.u[i] = cvt2(p[8 * st + 2 * i] - __uint_as_float(h.u[i] << 16),
+                    p[8 * st + 2 * i + 1] - __uint_as_float(h.u[i] & 0xffff0000u));
     return r.f;
   }
 };
@@ -432,8 +445,8 @@ template <typename T, int DP> struct Online {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
   }
-  // NSUB blocks of 32 keys from key0; the maximum lags by at most grow
-  template <int NSUB>
+  // NSUB blocks of 32 keys from key0; the maximum lags by at most grow.  FINE: P as two bf16
+  template <int NSUB, bool FINE = false>
   __device__ __forceinline__ void step(const I& im, const char* kimg, const char* vimg, int key0, const frag (&q)[I::NS],
                                        float scale2, bool masked, const RowMask& mask, int lane, float grow) {
     f16_t s[NSUB];
@@ -478,6 +491,12 @@ template <typename T, int DP> struct Online {
         l = Mma<T>::add(p, l);   // of P as it is multiplied
 #pragma unroll
         for (int d = 0; d < I::ND; ++d) o[d] = Mma<T>::mma(im.col_frag(vimg, 32 * b, st, d), p, o[d]);
+        if constexpr (FINE && sizeof(T) == 2) {
+          const frag low = Mma<T>::pack_rest(s[b], st, p);
+          l = Mma<T>::add(low, l);
+#pragma unroll
+          for (int d = 0; d < I::ND; ++d) o[d] = Mma<T>::mma(im.col_frag(vimg, 32 * b, st, d), low, o[d]);
+        }
       }
     }
     __builtin_amdgcn_s_setprio(0);
@@ -849,7 +868,7 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
       wait_vm<0>();
     }
     const int key0 = tl[it] * KT;
-    st.template step<1>(im, c, c + IB, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane, 0.f);
+    st.template step<1, true>(im, c, c + IB, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane, 0.f);
     if (STG == 1 && it + 4 < it1) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       dma.issue(kbase, a.kt, tl[it + 4] * KT, my.lo, my.hi, my.sl, n, 0);

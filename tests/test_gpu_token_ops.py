@@ -918,3 +918,21 @@ def test_attention_padded_graph_with_other_lengths():
         got = [x.clone() for x in out]
         for a, b in zip(got, run()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B,T,cap,H,Hk,D,window,sinks,lengths", [c for c in CACHED if c[1] * c[3] // c[4] <= 64 and max(c[8]) > 1] + [
+    (1, 1, 4096, 16, 4, 128, 1024, 4, [4096])])
+def test_attention_few_rows_keep_p(B, T, cap, H, Hk, D, window, sinks, lengths):
+    """Up to 64 rows a key head: the results' error is that of rounding the exact ones to bf16.  P in two bf16 is off by
+    2^-16, fp32 sums and scores by less: independent errors add in squares, 2^-14 of the norm beside the rounding's
+    2^-10.5 or more is 1.004 times it.  (P in one bf16: 1.08 to 1.35 times.)"""
+    g = gen(cap + D)
+    q, k, v = rand(g, B, T, H, D, type=BF), rand(g, B, cap, Hk, D, type=BF), rand(g, B, cap, Hk, D, type=BF)
+    o = tk().window_attention_cached(q, k, v, torch.tensor(lengths, dtype=torch.int32, device=DEV), window, sinks)
+    err = rounding = 0.0
+    for b in range(B):
+        L = min(max(lengths[b], 0), cap)
+        want = attn_ref(q[b], k[b], v[b], None, visible(T, cap, L, L - T, window, sinks, True), 1 / math.sqrt(D), BF)[0][0]
+        err += float((o[b].double() - want).square().sum())
+        rounding += float((want.to(BF).double() - want).square().sum())
+    assert math.sqrt(err) <= 1.03 * math.sqrt(rounding), math.sqrt(err / rounding)
