@@ -954,9 +954,10 @@ __global__ void __launch_bounds__(256) wattn_join_kernel(const WArgs a) {
   float mm = fmaxf(l0, l1);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 32));
-  // a NaN sum has to reach the result: the maximum drops it, its weight does not
-  const float f0 = l0 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(l0 - mm);
-  const float f1 = l1 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(l1 - mm);
+  // A NaN sum has to reach the result: the maximum drops it, its weight does not.  Below 0: a split that saw
+  // nothing.  One whose weight rounds to 0 saw something, and 0 times its infinity or NaN is NaN as in one piece.
+  const float f0 = l0 == kNegInf ? -1.f : __builtin_amdgcn_exp2f(l0 - mm);
+  const float f1 = l1 == kNegInf ? -1.f : __builtin_amdgcn_exp2f(l1 - mm);
   float s[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
   const float* p = a.part + row * a.D + (c < a.D ? c : 0);
   for (int z0 = 0; z0 < a.splits; z0 += 4) {
@@ -966,8 +967,8 @@ __global__ void __launch_bounds__(256) wattn_join_kernel(const WArgs a) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int z = z0 + k;
-      const float f = z < a.splits ? __shfl(z < 32 ? f0 : f1, z & 31, 32) : 0.f;
-      if (f == 0.f) continue;   // a split that saw nothing
+      const float f = z < a.splits ? __shfl(z < 32 ? f0 : f1, z & 31, 32) : -1.f;
+      if (f < 0.f) continue;
       ls += f;
       s[0] += f * x[k].x;
       s[1] += f * x[k].y;

@@ -936,3 +936,21 @@ def test_attention_few_rows_keep_p(B, T, cap, H, Hk, D, window, sinks, lengths):
         err += float((o[b].double() - want).square().sum())
         rounding += float((want.to(BF).double() - want).square().sum())
     assert math.sqrt(err) <= 1.03 * math.sqrt(rounding), math.sqrt(err / rounding)
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("T,cap,H,Hk", [(1, 4096, 2, 2), (70, 5000, 8, 8), (4, 90, 2, 1)])
+def test_attention_visible_nan_of_no_weight(T, cap, H, Hk, ty):
+    """A NaN or infinity in a visible value reaches the row however small its weight is, also where the keys are split
+    (the first two) and the weight of its whole split rounds to 0: 0 times it is NaN."""
+    g, D = gen(cap), 64
+    q, k, v = torch.ones(1, T, H, D, dtype=ty, device=DEV), rand(g, 1, cap, Hk, D, type=ty), rand(g, 1, cap, Hk, D, type=ty)
+    k[0, cap - T] = 40.0   # seen by all rows: a score of 320, e^250 times all others
+    n = torch.tensor([cap], dtype=torch.int32, device=DEV)
+    o = tk().window_attention_cached(q, k, v, n, cap)
+    within(o, v[:, cap - T, None].repeat_interleave(H // Hk, 2).expand_as(o).double(), 4 * UT[ty] * v.double().abs().amax().expand_as(o), "o")
+    for bad in (math.nan, math.inf):
+        for at in (5, cap // 2):
+            w = v.clone()
+            w[0, at] = bad
+            assert not torch.isfinite(tk().window_attention_cached(q, k, w, n, cap)).any(), (bad, at)
