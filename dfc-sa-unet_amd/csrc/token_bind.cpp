@@ -8,7 +8,9 @@
 // library), so there is one copy of it in the process, whichever file it came from.
 #include <torch/extension.h>
 
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -61,6 +63,29 @@ std::string shape(const Tensor& t) {
 }
 std::string name(at::ScalarType t) { return std::string(c10::toString(t)); }
 
+// The kernels read and write memory that torch's own operators allocated: a tracer would record the allocation and
+// return uninitialised memory, a forward-mode tangent would be lost, and wrapped tensors have no memory to read.
+bool traced() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Mode = c10::impl::TorchDispatchModeKey;
+  if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch)) return true;
+  if (!Modes::any_modes_set()) return false;
+  return Modes::get_mode(Mode::PROXY) || Modes::get_mode(Mode::FAKE) || Modes::get_mode(Mode::FUNCTIONAL);
+}
+void need_plain(at::ArrayRef<Tensor> ts) {
+  if (traced())
+    throw std::runtime_error("dfcsa.token_ops cannot be traced (torch.jit.trace, make_fx, torch.export, fake tensors)");
+  constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
+                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize,
+                                         c10::DispatchKey::ZeroTensor});
+  for (const Tensor& t : ts) {
+    if (!t.defined()) continue;
+    if (t._fw_grad(0).defined())
+      throw std::runtime_error("dfcsa.token_ops has no forward-mode derivatives: detach() inputs that carry a tangent");
+    if (t.key_set().has_any(wrapped) || t.layout() != at::kStrided)
+      throw std::runtime_error("dfcsa.token_ops needs dense tensors, not tensors wrapped by torch.func or a subclass with a dispatch of its own");
+  }
+}
 void need_gpu(std::initializer_list<const Tensor*> ts) {
   const Tensor* first = nullptr;
   for (const Tensor* t : ts) {
@@ -81,9 +106,10 @@ void done(int rc, const char* what) {
   throw std::runtime_error(std::string(what) + " failed: " +
                            (rc == DFCSA_EINVAL ? "invalid argument/shape" : "HIP error " + std::to_string(-rc)));
 }
-void first_order() {
+void first_order(const variable_list& g) {
   TORCH_CHECK(!at::GradMode::is_enabled(),
               "dfcsa.token_ops: gradients are first order only (create_graph=True is refused)");
+  need_plain(g);
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -156,7 +182,7 @@ struct RmsNorm : public Function<RmsNorm> {
     return {y, r};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    first_order();
+    first_order(g);
     const auto saved = ctx->get_saved_variables();
     const Tensor &r = saved[0], &rstd = saved[1], w = packed(saved[2]);
     const auto xt = (at::ScalarType)ctx->saved_data["x"].toInt();
@@ -182,6 +208,7 @@ struct RmsNorm : public Function<RmsNorm> {
 };
 
 std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor& x, const Tensor& res, const Tensor& w, double eps) {
+  need_plain({x, res, w});
   if (wants_grad({&x, &res, &w})) {
     norm_args(x, res, w, eps);
     const variable_list o = RmsNorm::apply(x, res, w, eps);
@@ -200,6 +227,7 @@ int64_t group_of(int64_t group, int64_t C) {
 
 std::tuple<Tensor, Tensor, Tensor> rms_norm_residual_q8(const Tensor& x0, const Tensor& res0, const Tensor& w0,
                                                         double eps, int64_t group) {
+  need_plain({x0, res0, w0});
   if (wants_grad({&x0, &res0, &w0}))
     throw std::runtime_error("rms_norm_residual_q8 has no gradient: call it under torch.no_grad(), or rms_norm_residual");
   const Norm n = norm_args(x0, res0, w0, eps);
@@ -218,6 +246,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_residual_q8(const Tensor& x0, const 
 }
 
 Tensor dequant_q8(const Tensor& y8, const Tensor& scales, at::ScalarType out) {
+  need_plain({y8, scales});
   if (wants_grad({&scales})) throw std::runtime_error("dequant_q8 has no gradient: call it under torch.no_grad()");
   need_gpu({&y8, &scales});
   if (y8.scalar_type() != at::kFloat8_e4m3fn || scales.scalar_type() != at::kFloat)
@@ -348,7 +377,7 @@ struct Rotary : public Function<Rotary> {
     return {a, b};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    first_order();
+    first_order(g);
     const Tensor gq = ctx->needs_input_grad(0) ? g[0] : Tensor();
     const Tensor gk = g.size() > 1 && ctx->needs_input_grad(1) ? g[1] : Tensor();
     if (!gq.defined() && !gk.defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
@@ -361,6 +390,7 @@ struct Rotary : public Function<Rotary> {
 std::tuple<Tensor, std::optional<Tensor>> rotary(const Tensor& q, const std::optional<Tensor>& k0, const Tensor& pos,
                                                  const TablePtr& table, bool interleaved) {
   const Tensor k = k0.value_or(Tensor());
+  need_plain({q, k, pos});
   rotary_check(q, k, pos, *table);
   Tensor a, b;
   if (wants_grad({&q, &k})) {
@@ -493,7 +523,7 @@ struct WindowAttention : public Function<WindowAttention> {
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    first_order();
+    first_order(g);
     const auto s = ctx->get_saved_variables();
     const int64_t G = s[0].size(2) / s[1].size(2);
     const Tensor q = strided(s[0], G), k = strided(s[1], 0), v = strided(s[2], 0), dout = strided(g[0], G);
@@ -521,8 +551,8 @@ struct Nothing : public Function<Nothing> {
     ctx->save_for_backward({q, k, v});
     return at::zeros(q.sizes(), q.options());
   }
-  static variable_list backward(AutogradContext* ctx, variable_list) {
-    first_order();
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_order(g);
     variable_list z;
     for (const Tensor& t : ctx->get_saved_variables()) z.push_back(at::zeros_like(t));
     return z;
@@ -534,6 +564,7 @@ int clamp32(int64_t v) { return (int)std::min<int64_t>(v, INT_MAX); }
 Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, bool causal,
                         double scale, const std::optional<Tensor>& lengths0) {
   Tensor lengths = lengths0.value_or(Tensor());
+  need_plain({q, k, v, lengths});
   attn_check(q, k, v, window, sinks, scale, lengths, false);
   if (k.size(1) != q.size(1))
     bad_value(std::to_string(q.size(1)) + " queries and " + std::to_string(k.size(1)) +
@@ -548,6 +579,7 @@ Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64
 
 Tensor window_attention_cached(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, int64_t window,
                                int64_t sinks, double scale) {
+  need_plain({q, k, v, lengths});
   if (wants_grad({&q, &k, &v}))
     throw std::runtime_error("window_attention_cached has no gradient: call it under torch.no_grad(), or window_attention");
   attn_check(q, k, v, window, sinks, scale, lengths, true);

@@ -16,7 +16,9 @@ Types: bf16 or fp32 (the framework's two precisions), statistics and sums in fp3
 enqueues on the current stream of its tensors' device, allocates from torch's caching allocator only
 (so it can be captured into a graph) and never synchronises.  Arguments are checked on the host:
 ValueError for shapes and values, TypeError for types, RuntimeError for tensors that are not on the
-GPU.  Results do not depend on the order in which workgroups run.  Gradients are first order only.
+GPU.  Results do not depend on the order in which workgroups run.  Gradients are first order only; what torch
+would need an operator of its own for (forward-mode tangents, torch.func's transforms, torch.jit.trace,
+make_fx and torch.export, tensor subclasses with a dispatch of their own) is refused with a RuntimeError.
 """
 import ctypes
 import functools

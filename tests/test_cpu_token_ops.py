@@ -193,3 +193,60 @@ def test_argument_corners():
     with pytest.raises(RuntimeError, match="no gradient"):
         tk.dequant_q8(torch.zeros(2, 8).to(tk.E4M3), torch.ones(2, 1, requires_grad=True))
     assert LIB.dfcsa_wattn_fwd(ctypes.addressof(attn_desc(scale=3e38)), None) == EINVAL
+
+
+def calls(x, q):
+    """Each entry point with one of x [2, 8] and q [1, 4, 2, 8] among its arguments."""
+    n, pos = torch.ones(1, dtype=torch.int32), torch.zeros(4, 1, dtype=torch.int32)
+    y, w, r = torch.ones(2, 8), torch.ones(8), torch.ones(1, 4, 2, 8)
+    return (lambda: tk.rms_norm_residual(x, y, w)[0], lambda: tk.rms_norm_residual(y, x, w)[0],
+            lambda: tk.rms_norm_residual_q8(y, x, w)[1], lambda: tk.dequant_q8(y.to(tk.E4M3), x[:, :1]),
+            lambda: tk.rotary(q, r, pos, (2,))[0], lambda: tk.rotary(r, q, pos, (2,))[0],
+            lambda: tk.window_attention(r, q, r, 2), lambda: tk.window_attention(q, r, r, 2),
+            lambda: tk.window_attention_cached(r, r, q, n, 2))
+
+
+@pytest.mark.parametrize("i", range(9))
+def test_forward_mode_is_refused(i):
+    with torch.autograd.forward_ad.dual_level():
+        x, q = (torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) for t in (torch.randn(2, 8), torch.randn(1, 4, 2, 8)))
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                calls(x, q)[i]()
+
+
+@pytest.mark.parametrize("i", range(9))
+def test_tracing_is_refused(i):
+    x, q = torch.randn(2, 8), torch.randn(1, 4, 2, 8)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(lambda x, q: calls(x, q)[i](), (x, q))
+    for mode in ("real", "fake", "symbolic"):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.fx.experimental.proxy_tensor.make_fx(lambda x, q: calls(x, q)[i](), tracing_mode=mode)(x, q)
+    with torch._subclasses.FakeTensorMode(), pytest.raises(RuntimeError, match="cannot be traced"):
+        calls(torch.empty(2, 8, device="cuda"), torch.empty(1, 4, 2, 8, device="cuda"))[i]()
+
+
+class Wrapped(torch.Tensor):
+    """A tensor without memory of its own."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError
+
+
+@pytest.mark.parametrize("i", [0, 1, 2, 4, 5, 6, 7, 8])
+def test_wrapped_tensors_are_refused(i):
+    x, q = torch.randn(2, 8), torch.randn(1, 4, 2, 8)
+    with pytest.raises(RuntimeError, match="dense tensors"):
+        torch.func.vmap(lambda x, q: calls(x, q)[i]())(x[None], q[None])
+    with pytest.raises(RuntimeError, match="dense tensors|forward-mode"):
+        torch.func.jvp(lambda x, q: calls(x, q)[i](), (x, q), (x, q))
+    with pytest.raises(RuntimeError, match="dense tensors"):
+        torch.func.grad(lambda x, q: calls(x, q)[i]().sum(), (0, 1))(x, q)
+    with pytest.raises(RuntimeError, match="dense tensors"):
+        calls(Wrapped(x), Wrapped(q))[i]()

@@ -954,3 +954,15 @@ def test_attention_visible_nan_of_no_weight(T, cap, H, Hk, ty):
             w = v.clone()
             w[0, at] = bad
             assert not torch.isfinite(tk().window_attention_cached(q, k, w, n, cap)).any(), (bad, at)
+
+
+def test_tangents_of_gradients_are_refused():
+    """Forward mode over the backward pass: the gradients' tangents would be lost."""
+    t, g = tk(), gen(101)
+    q, x = rand(g, 1, 9, 2, 16).requires_grad_(), rand(g, 3, 16).requires_grad_()
+    w, pos = torch.ones(16, device=DEV), torch.zeros(9, 1, dtype=torch.int32, device=DEV)
+    for leaf, out in ((x, t.rms_norm_residual(x, x, w)[0]), (q, t.rotary(q, None, pos, (4,))[0]), (q, t.window_attention(q, q, q, 3))):
+        with torch.autograd.forward_ad.dual_level():
+            d = torch.autograd.forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, leaf, d)
