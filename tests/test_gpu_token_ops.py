@@ -966,3 +966,16 @@ def test_tangents_of_gradients_are_refused():
             d = torch.autograd.forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, leaf, d)
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("N,D,window,sinks", [(2048, 64, 30, 40), (300, 96, 30, 100), (5000, 128, 100, 4)])
+def test_attention_infinite_far_gradient(N, D, window, sinks, ty):
+    """An infinite gradient in one column of a row far from the sinks: their dV is infinite there (P is above 0), not NaN."""
+    g = gen(N)
+    q, k, v, do = (rand(g, 1, N, 1, D, type=ty) for _ in range(4))
+    do[0, N - 2, 0, 5] = math.inf
+    v.requires_grad_()
+    (dv,) = torch.autograd.grad(tk().window_attention(q, k, v, window, sinks, causal=False), v, do)
+    assert torch.isposinf(dv[0, :sinks, 0, 5]).all()
+    assert torch.isfinite(dv[0, :sinks, 0, :5]).all() and torch.isfinite(dv[0, :sinks, 0, 6:]).all()
