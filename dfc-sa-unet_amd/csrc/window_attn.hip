@@ -83,6 +83,43 @@ struct WArgs {
   int far32, cfar;       // blocks of 32 sinks, and chunks of the rows beyond the window that see them (0: none)
 };
 
+// A kernel's second, rare pass gets the kernel's arguments (by address: for kernels whose one argument is a WArgs), the
+// thread's index, its place and LDS as values that the compiler takes for others.  What it needs is then formed
+// there again, and not held in registers through the first pass (that spilled scalar registers in the first's loop:
+// forward 104 -> 111 us at 8192 tokens, key-major pass 162 -> 175; as a function that is called it needs a stack,
+// which costs the launch after it 0.45 us).
+// The waves on a SIMD that a kernel's first pass reaches, which the second must not lower; it may spill for them.
+// P: 0 forward, 1 dQ, 2 dK / dV, 3 few rows, 4 far rows; widths 32, 64, 96, 128 in bf16, then in fp32.
+template <typename T, int DP> constexpr int simd_waves(int P) {
+  constexpr int w[5][8] = {{4, 4, 2, 2, 4, 3, 2, 1}, {4, 3, 2, 2, 4, 2, 2, 1}, {4, 2, 2, 2, 3, 2, 1, 1},
+                           {2, 2, 1, 1, 1, 1, 1, 1}, {2, 2, 1, 1, 1, 1, 1, 1}};
+  return w[P][(sizeof(T) == 2 ? 0 : 4) + DP / 32 - 1];
+}
+// As the largest number too: the scheduler gives up the order that interleave() asks for where that takes a kernel
+// from more waves to fewer (key-major pass, width 64: 28.8 -> 32.7 us).
+#define SIMD_WAVES(P) __attribute__((amdgpu_waves_per_eu(simd_waves<T, DP>(P), simd_waves<T, DP>(P))))
+struct Again {
+  uint64_t args;
+  unsigned smem, bad;
+  int tid;
+};
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ unsigned lds_addr(const void* p) {
+  return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p;
+}
+__device__ __forceinline__ char* lds_at(unsigned offset) {
+  return (char*)(__attribute__((address_space(3))) char*)(size_t)(unsigned)uniform((int)offset);
+}
+__device__ __forceinline__ Again again(const char* smem, const void* bad, int tid) {
+  Again g{(uint64_t)__builtin_amdgcn_kernarg_segment_ptr(), lds_addr(smem), lds_addr(bad), tid};
+  asm volatile("" : "+s"(g.args), "+v"(g.tid));
+  return g;
+}
+__device__ __forceinline__ const WArgs& args_of(const Again& g) {
+  const uint64_t p = (uint64_t)(unsigned)uniform((int)(g.args >> 32)) << 32 | (unsigned)uniform((int)g.args);
+  return *(const WArgs*)(const __attribute__((address_space(4))) WArgs*)p;
+}
+
 // two values to bf16 in one instruction
 __device__ __forceinline__ uint32_t cvt2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){a, b}, bh2_t));
@@ -274,9 +311,6 @@ __device__ __forceinline__ i4_t make_rsrc(const void* base) {
   asm volatile("s_nop 4" : "+s"(r));
   return r;
 }
-__device__ __forceinline__ unsigned lds_addr(const char* p) {
-  return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p;
-}
 // lds: wave-uniform
 __device__ __forceinline__ void dma16(const i4_t& rsrc, unsigned voff, unsigned lds) {
   unsigned keep;
@@ -328,6 +362,7 @@ struct RowMask {   // of this lane's row: visible(key) = key in [lo, lo + span] 
   int lo;
   unsigned span;
   int sl;
+  __device__ __forceinline__ bool sees(int key) const { return (unsigned)(key - lo) <= span || key < sl; }
   // accumulator rows (keys key0 + 8 (e / 4) + e % 4) that the row does not see become `by`
   __device__ __forceinline__ void hide(f16_t& s, int key0, float by) const {
     const unsigned k = (unsigned)(key0 - lo);
@@ -431,6 +466,117 @@ __device__ __forceinline__ f16_t zero16() {
   return z;
 }
 
+// ------------------------------------------------------------------ values that are not finite
+// A product of matrix tiles multiplies every element of both: where a hidden key's P is 0 and its V (or K,
+// or a hidden row's Q or dO) is infinite or NaN, the 0 * inf reaches rows that do not see it.  Nothing is
+// tested for that in the loops; a workgroup that ends with a sum that is not finite runs its tiles once
+// more with strict_product, and the waves concerned write again.
+//
+// There the product takes the finite elements of A; what the others add follows from three cases.  With t
+// the number of visible pairs whose A is not finite, and s the sum of sign(A) sign(B) over them (0 for a
+// NaN A and for a B of 0, whose product is NaN): t > s where something adds -inf or NaN, t > -s where
+// something adds +inf or NaN.  Both are small whole numbers, exact as matrix products of -1, 0 and 1.  So
+// inputs of nothing but NaN or infinities cost up to 6 times what others do (8192 tokens, 16 / 4 heads of 128,
+// window 1024, forward and backward: 0.42 ms; a row of NaN among the sinks' values 1.2, nothing but NaN in
+// q, v or dO 1.7, 1.6 and 1.4; one row and key after the other, without matrix products, they took up to 160).
+__device__ __forceinline__ bool finite_all(const f16_t& v) {
+  bool ok = true;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) ok = ok && (__float_as_uint(v[e]) & 0x7f800000u) != 0x7f800000u;
+  return ok;
+}
+// a fragment's finite elements, the others 0; all: were they all finite
+__device__ __forceinline__ s8_t finite_part(s8_t a, bool& all) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool bad = (a[e] & 0x7f80) == 0x7f80;
+    all = all && !bad;
+    a[e] = bad ? (short)0 : a[e];
+  }
+  return a;
+}
+__device__ __forceinline__ f4_t finite_part(f4_t a, bool& all) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool bad = (__float_as_uint(a[e]) & 0x7f800000u) == 0x7f800000u;
+    all = all && !bad;
+    a[e] = bad ? 0.f : a[e];
+  }
+  return a;
+}
+// 1 where an element is not finite (kind), its sign where it is infinite (sign)
+__device__ __forceinline__ void classes(const s8_t& a, s8_t& kind, s8_t& sign) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    kind[e] = (a[e] & 0x7f80) == 0x7f80 ? (short)0x3f80 : (short)0;
+    sign[e] = (a[e] & 0x7fff) == 0x7f80 ? (short)(0x3f80 | (a[e] & 0x8000)) : (short)0;
+  }
+}
+__device__ __forceinline__ void classes(const f4_t& a, f4_t& kind, f4_t& sign) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t b = __float_as_uint(a[e]);
+    kind[e] = (b & 0x7f800000u) == 0x7f800000u ? 1.f : 0.f;
+    sign[e] = (b & 0x7fffffffu) == 0x7f800000u ? (b >> 31 ? -1.f : 1.f) : 0.f;
+  }
+}
+// o += A^T b over the 32 rows of img from r0; b is 0 at hidden pairs, see(e): is accumulator element e's visible
+template <typename T, int DP, bool FINE, typename See>
+__device__ __forceinline__ void strict_product(const Img<T, DP>& im, const char* img, int r0, const f16_t& b,
+                                               f16_t (&o)[Img<T, DP>::ND], See see) {
+  typedef Img<T, DP> I;
+  typedef typename I::frag frag;
+  constexpr int NST = 32 / Mma<T>::KS;
+  bool all = true;
+#pragma unroll
+  for (int st = 0; st < NST; ++st) {
+    const frag p = Mma<T>::pack(b, st);
+    frag low = p;
+    if constexpr (FINE && sizeof(T) == 2) low = Mma<T>::pack_rest(b, st, p);
+#pragma unroll
+    for (int d = 0; d < I::ND; ++d) {
+      __builtin_amdgcn_sched_barrier(0);   // one fragment's registers at a time: this is the rare path
+      const frag a = finite_part(im.col_frag(img, r0, st, d), all);
+      o[d] = Mma<T>::mma(a, p, o[d]);
+      if constexpr (FINE && sizeof(T) == 2) o[d] = Mma<T>::mma(a, low, o[d]);
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  if (!__any(!all)) return;
+#pragma unroll 1
+  for (int neg = 0; neg < 2; ++neg) {   // t > -s, then t > s
+    const float by = neg ? -1.f : 1.f;
+    frag sg[NST], vis[NST];
+#pragma unroll
+    for (int st = 0; st < NST; ++st) {
+      f16_t x, y;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        x[e] = b[e] > 0.f ? by : (b[e] < 0.f ? -by : 0.f);
+        y[e] = see(e) ? 1.f : 0.f;
+      }
+      sg[st] = Mma<T>::pack(x, st);
+      vis[st] = Mma<T>::pack(y, st);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int d = 0; d < I::ND; ++d) {
+      f16_t t = zero16();
+#pragma unroll
+      for (int st = 0; st < NST; ++st) {
+        __builtin_amdgcn_sched_barrier(0);
+        frag kind, sign;
+        classes(im.col_frag(img, r0, st, d), kind, sign);
+        t = Mma<T>::mma(sign, sg[st], Mma<T>::mma(kind, vis[st], t));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] -= t[e] > 0.f ? by * kNegInf : 0.f;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // ------------------------------------------------------------------ softmax state of 32 rows (one per lane column)
 template <typename T, int DP> struct Online {
   typedef Img<T, DP> I;
@@ -501,19 +647,44 @@ template <typename T, int DP> struct Online {
     }
     __builtin_amdgcn_s_setprio(0);
   }
+  // the same with lse, the row's log-sum over all its keys (log2; +inf: it sees none), and strict products
+  template <int NSUB, bool FINE = false>
+  __device__ __forceinline__ void again(const I& im, const char* kimg, const char* vimg, int key0, const frag (&q)[I::NS],
+                                        float scale2, const RowMask& mask, int lane, float lse) {
+#pragma unroll 1
+    for (int b = 0; b < NSUB; ++b) {
+      f16_t s = zero16();
+#pragma unroll
+      for (int st = 0; st < I::NS; ++st) s = Mma<T>::mma(im.row_frag(kimg, 32 * b, st), q[st], s);
+      const int k0 = key0 + 32 * b + 4 * (lane >> 5);
+      mask.hide(s, k0, kNegInf);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale2, -lse));
+      strict_product<T, DP, FINE>(im, vimg, 32 * b, s, o, [&](int e) { return mask.sees(k0 + 8 * (e >> 2) + (e & 3)); });
+    }
+  }
 };
 
-// this lane's row of a [token][head] tensor as fragments (rows past the end: zeros)
-template <typename T, int DP>
+// this lane's row of a [token][head] tensor as fragments (rows that are not ok: zeros).  ALL: the row is there
+// whether ok or not, and is loaded without branches (the dQ pass in fp32 spills beside them, 53 -> 57 us at width
+// 64; in bf16 they are the faster form, 137 against 141 us at 8192 tokens)
+template <typename T, int DP, bool ALL = false>
 __device__ __forceinline__ void load_frags(const char* row, bool ok, int D, int lane,
                                            typename Mma<T>::frag (&f)[Img<T, DP>::NS]) {
   constexpr int KS = Mma<T>::KS;
 #pragma unroll
   for (int st = 0; st < Img<T, DP>::NS; ++st) {
     const int d = KS * st + KS / 2 * (lane >> 5);
+    constexpr int NE = sizeof(f[0]) / sizeof(f[0][0]);
+    if constexpr (ALL) {
+      const auto x = *(const typename Mma<T>::frag*)(row + (d < D ? d : 0) * (int)sizeof(T));
 #pragma unroll
-    for (int e = 0; e < (int)(sizeof(f[0]) / sizeof(f[0][0])); ++e) f[st][e] = 0;
-    if (ok && d < D) f[st] = *(const typename Mma<T>::frag*)(row + d * (int)sizeof(T));
+      for (int e = 0; e < NE; ++e) f[st][e] = ok && d < D ? x[e] : 0;
+    } else {
+#pragma unroll
+      for (int e = 0; e < NE; ++e) f[st][e] = 0;
+      if (ok && d < D) f[st] = *(const typename Mma<T>::frag*)(row + d * (int)sizeof(T));
+    }
   }
 }
 template <typename T> __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
@@ -602,143 +773,6 @@ __device__ __forceinline__ void finish_rows(const WArgs& a, int bh, int split, i
   }
 }
 
-// ------------------------------------------------------------------ rows and keys one at a time
-// A product of matrix tiles multiplies every element of both: where a hidden key's P is 0 and its V (or K,
-// or a hidden row's Q or dO) is infinite or NaN, the 0 * inf reaches rows that do not see it.  Nothing is
-// tested for that in the loops; a wave whose results are not all finite forms them again here, from the
-// visible pairs alone, one row (or key) at a time with two columns per lane.  A sum that is NaN in all
-// columns stays it, so a row that sees a NaN ends there and inputs of nothing but NaN cost little.
-__device__ __forceinline__ bool finite_all(const f16_t& v) {
-  bool ok = true;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) ok = ok && (__float_as_uint(v[e]) & 0x7f800000u) != 0x7f800000u;
-  return ok;
-}
-template <typename T> __device__ __forceinline__ float2 two(const void* row, int d, int D) {
-  if (d >= D) return make_float2(0.f, 0.f);
-  const T* p = (const T*)row + d;
-  return make_float2(ElemTraits<T>::to_f(p[0]), ElemTraits<T>::to_f(p[1]));
-}
-template <typename T> __device__ __forceinline__ void put_two(void* row, int d, int D, float x, float y) {
-  if (d >= D) return;
-  ((T*)row)[d] = ElemTraits<T>::from_f(x);
-  ((T*)row)[d + 1] = ElemTraits<T>::from_f(y);
-}
-struct At {   // a packed row's place
-  int t, g;
-};
-__device__ __forceinline__ At at_row(const WArgs& a, int r) {
-  At x;
-  x.t = dm_div(a.dmG, r);
-  x.g = r - x.t * a.G;
-  return x;
-}
-__device__ __forceinline__ bool sees(const RowMask& m, int key) { return (unsigned)(key - m.lo) <= m.span || key < m.sl; }
-
-// row r over the keys of tiles [it0, it1) of KT keys, to where finish_rows puts it
-template <typename T>
-__device__ __forceinline__ void exact_row(const WArgs& a, const Seq& seq, int bh, int split, int r, const TileList& tl, int it0,
-                                       int it1, int KT) {
-  const int lane = threadIdx.x & 63, d = 2 * lane, b = bh / a.Hk, hk = bh - b * a.Hk;
-  const At x = at_row(a, r);
-  const RowMask mask = row_mask(a, seq, r);
-  const bool live = mask.lo != 0x7fffffff;
-  const char* kb = (const char*)a.k + b * a.kb + hk * a.kh;
-  const char* vb = (const char*)a.v + b * a.vb + hk * a.vh;
-  float2 q = make_float2(0.f, 0.f);
-  if (live) q = two<T>((const char*)a.q + b * a.qb + x.t * a.qt + (hk * a.G + x.g) * a.qh, d, a.D);
-  float m = kNegInf, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int it = it0; it < it1; ++it)
-    for (int key = tl[it] * KT; key < (tl[it] + 1) * KT; ++key) {
-      if (!sees(mask, key)) continue;
-      const float2 k = two<T>(kb + (int64_t)key * a.kt, d, a.D), v = two<T>(vb + (int64_t)key * a.vt, d, a.D);
-      const float s = wave_sum(q.x * k.x + q.y * k.y) * a.scale2;
-      const float mn = fmaxf(m, s), ms = mn == kNegInf ? 0.f : mn;
-      const float al = __builtin_amdgcn_exp2f(m - ms), p = __builtin_amdgcn_exp2f(s - ms);
-      l = l * al + p;
-      o0 = o0 * al + p * v.x;
-      o1 = o1 * al + p * v.y;
-      m = mn;
-      if (l != l) {   // the same in all lanes: every column is NaN from here on
-        o0 = o1 = l;
-        it = it1;
-        break;
-      }
-    }
-  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-  const float lse = l == 0.f ? kNegInf : m + __builtin_amdgcn_logf(l);
-  const int64_t row = (int64_t)bh * a.R + r, rows = (int64_t)a.B * a.Hk * a.R;
-  if (a.splits == 1) {
-    const int64_t at = (((int64_t)b * a.T + x.t) * a.H + hk * a.G + x.g) * a.D;
-    put_two<T>((T*)a.o + at, d, a.D, o0 * inv, o1 * inv);
-    if (sizeof(T) == 2 && a.rest)
-      put_two<bf16_t>(a.rest + at, d, a.D, o0 * inv - bf2f(f2bf(o0 * inv)), o1 * inv - bf2f(f2bf(o1 * inv)));
-    if (a.lse && lane == 0) a.lse[row] = lse;
-  } else {
-    put_two<float>(a.part + (split * rows + row) * a.D, d, a.D, o0 * inv, o1 * inv);
-    if (lane == 0) a.part[a.splits * rows * a.D + split * rows + row] = lse;
-  }
-}
-// dQ of row r
-template <typename T>
-__device__ __forceinline__ void exact_dq(const WArgs& a, const Seq& seq, int bh, int r, const TileList& tl, int KT, float lse,
-                                      float dl) {
-  const int lane = threadIdx.x & 63, d = 2 * lane, b = bh / a.Hk, hk = bh - b * a.Hk;
-  const At x = at_row(a, r);
-  const RowMask mask = row_mask(a, seq, r);
-  const char* kb = (const char*)a.k + b * a.kb + hk * a.kh;
-  const char* vb = (const char*)a.v + b * a.vb + hk * a.vh;
-  float2 q = make_float2(0.f, 0.f), g = q;
-  if (mask.lo != 0x7fffffff) {
-    q = two<T>((const char*)a.q + b * a.qb + x.t * a.qt + (hk * a.G + x.g) * a.qh, d, a.D);
-    g = two<T>((const char*)a.dO + b * a.ob + x.t * a.ot + (hk * a.G + x.g) * a.oh, d, a.D);
-  }
-  float d0 = 0.f, d1 = 0.f;
-  for (int it = 0; it < tl.n; ++it)
-    for (int key = tl[it] * KT; key < (tl[it] + 1) * KT; ++key) {
-      if (!sees(mask, key)) continue;
-      const float2 k = two<T>(kb + (int64_t)key * a.kt, d, a.D), v = two<T>(vb + (int64_t)key * a.vt, d, a.D);
-      const float s = wave_sum(q.x * k.x + q.y * k.y), dp = wave_sum(g.x * v.x + g.y * v.y);
-      const float ds = __builtin_amdgcn_exp2f(s * a.scale2 - lse) * (dp - dl);
-      d0 += ds * k.x;
-      d1 += ds * k.y;
-      if (ds != ds) {
-        it = tl.n;
-        break;
-      }
-    }
-  put_two<T>((T*)a.dq + (((int64_t)b * a.T + x.t) * a.H + hk * a.G + x.g) * a.D, d, a.D, d0 * a.scale, d1 * a.scale);
-}
-// dK and dV of a key over rows [r0, r1) and [r2, r3), to outk and outv (type O)
-template <typename T, typename O>
-__device__ __forceinline__ void exact_key(const WArgs& a, const Seq& seq, int bh, int key, int r0, int r1, int r2, int r3,
-                                       O* outk, O* outv) {
-  const int lane = threadIdx.x & 63, d = 2 * lane, b = bh / a.Hk, hk = bh - b * a.Hk;
-  float2 k = make_float2(0.f, 0.f), v = k;
-  float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-  if (key < seq.len) {
-    k = two<T>((const char*)a.k + b * a.kb + (int64_t)key * a.kt + hk * a.kh, d, a.D);
-    v = two<T>((const char*)a.v + b * a.vb + (int64_t)key * a.vt + hk * a.vh, d, a.D);
-    for (int r = r0; r < max(r1, r3); r = r + 1 == r1 && r2 < r3 && r2 > r ? r2 : r + 1) {
-      if (r >= a.R || (r >= r1 && (r < r2 || r >= r3))) continue;
-      if (!sees(row_mask(a, seq, r), key)) continue;
-      const At x = at_row(a, r);
-      const float2 q = two<T>((const char*)a.q + b * a.qb + x.t * a.qt + (hk * a.G + x.g) * a.qh, d, a.D);
-      const float2 g = two<T>((const char*)a.dO + b * a.ob + x.t * a.ot + (hk * a.G + x.g) * a.oh, d, a.D);
-      const float s = wave_sum(q.x * k.x + q.y * k.y), dp = wave_sum(g.x * v.x + g.y * v.y);
-      const float p = __builtin_amdgcn_exp2f(s * a.scale2 - a.lse[(int64_t)bh * a.R + r]);
-      const float ds = p * (dp - a.delta[(int64_t)bh * a.R + r]);
-      k0 += ds * q.x;
-      k1 += ds * q.y;
-      v0 += p * g.x;
-      v1 += p * g.y;
-      if (p != p) break;
-    }
-  }
-  put_two<O>(outk, d, a.D, k0 * a.scale, k1 * a.scale);
-  put_two<O>(outv, d, a.D, v0, v1);
-}
-
 // ============================================================================ forward
 // 128 rows per workgroup, 32 per wave; key tiles double-buffered in LDS, one barrier a tile: a tile's DMA
 // runs while the one before it is worked on.  64 KB of LDS and up to 256 registers leave two workgroups
@@ -746,15 +780,12 @@ __device__ __forceinline__ void exact_key(const WArgs& a, const Seq& seq, int bh
 // Measured at 8192 tokens, 16 / 4 heads of 128, window 1024: 104 us, 620 TFLOP/s of the 1145 that a large
 // library product reaches here; 25 us of it are the reads of q and the writes of o, its rest and lse, the
 // matrix unit is busy 30 % of the time, the vector unit (exponentials, maxima, sums) 38 % (counters, 2.4 GHz).
-template <typename T, int DP>
-__global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wattn_fwd_kernel(const WArgs a) {
+// all tiles, their results written; true: some are not finite.  lse, lsum: of the lane's row, formed by the first pass
+template <typename T, int DP, bool strict>
+__device__ __forceinline__ bool fwd_pass(const WArgs& a, const Spot& at, int tid, char* smem, int* s_bad, float& lse, float& lsum) {
   typedef Img<T, DP> I;
   constexpr int KT = I::ROWS;
-  __shared__ __attribute__((aligned(16))) char smem[4 * I::BYTES];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int per = a.splits;
-  const Spot at = spot(a, a.tiles, a.G, per);
-  if (at.bh < 0) return;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int split = at.sub, tile = at.tile, bh = at.bh;
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const Seq seq = seq_of(a, b);
@@ -776,6 +807,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
   }
   I im;
   im.init(lane);
+  bool bad = strict && __builtin_amdgcn_readfirstlane(s_bad[wave]);
   Online<T, DP> st;
   st.init();
   if (it0 < it1) {
@@ -792,21 +824,61 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
       dma.issue(vbase, a.vt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt + I::BYTES, wave);
     }
     const int key0 = tl[it] * KT;
-    if (sees_any(my, key0, key0 + KT))
+    if (!sees_any(my, key0, key0 + KT)) continue;
+    if constexpr (!strict)
       st.template step<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane,
                                 tl.n <= kFewTiles ? 0.f : kGrow);
+    else if (bad)
+      st.template again<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, mask, lane, lse);
   }
-  const float lsum = st.l + __shfl_xor(st.l, 32, 64);
-  lds_barrier();   // the tiles are read
-  finish_rows<T, DP>(a, bh, split, rw, st.o, st.m, lsum, smem + wave * 32 * out_pitch<DP>(), lane);
-  bool ok = true;
+  if constexpr (!strict) {
+    lsum = st.l + __shfl_xor(st.l, 32, 64);
+    lse = st.m;
+    bool ok = true;
 #pragma unroll
-  for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(st.o[d]);
-  if (__any(!ok && r < a.R)) {
-    wait_vm<0>();   // the stores that these replace
-#pragma unroll 1
-    for (int i = rw; i < min(rw + 32, a.R); ++i) exact_row<T>(a, seq, bh, split, i, tl, it0, it1, KT);
+    for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(st.o[d]);
+    bad = __any(!ok && r < a.R);
+    if (lane == 0) s_bad[wave] = bad;
   }
+  lds_barrier();   // the tiles are read, the waves' results known
+  if (!strict || bad) finish_rows<T, DP>(a, bh, split, rw, st.o, lse, lsum, smem + wave * 32 * out_pitch<DP>(), lane);
+  if (strict || !(s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3])) return false;
+  wait_vm<0>();   // the stores that the next ones replace
+  lds_barrier();
+  lse = lsum == 0.f ? -kNegInf : lse + __builtin_amdgcn_logf(lsum);
+  lsum = lsum == 0.f ? 0.f : 1.f;
+  return true;
+}
+template <typename T, int DP>
+__device__ __forceinline__ void fwd_again(Again g, Spot at, float lse, float lsum) {
+  at = Spot{uniform(at.bh), uniform(at.tile), uniform(at.sub)};
+  fwd_pass<T, DP, true>(args_of(g), at, g.tid, lds_at(g.smem), (int*)lds_at(g.bad), lse, lsum);
+}
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) SIMD_WAVES(0) wattn_fwd_kernel(const WArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[4 * Img<T, DP>::BYTES];
+  __shared__ int s_bad[4];
+  int per = a.splits;
+  const Spot at = spot(a, a.tiles, a.G, per);
+  if (at.bh < 0) return;
+  float lse = 0.f, lsum = 0.f;
+  if (fwd_pass<T, DP, false>(a, at, threadIdx.x, smem, s_bad, lse, lsum))
+    fwd_again<T, DP>(again(smem, s_bad, threadIdx.x), at, lse, lsum);
+}
+
+// weights and sum of one row's results of four waves
+__device__ __forceinline__ void join_waves(const float (&m)[4][32], const float (&l)[4][32], int row, float (&f)[4], float& inv,
+                                           float& lse) {
+  float mm = kNegInf, ls = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, m[w][row]);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = mm == kNegInf ? (l[w][row] == 0.f ? 0.f : l[w][row]) : __builtin_amdgcn_exp2f(m[w][row] - mm);
+    ls += f[w] * l[w][row];
+  }
+  inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);
+  lse = ls == 0.f ? kNegInf : mm + __builtin_amdgcn_logf(ls);
 }
 
 // Few rows (at most 32 per tile): the four waves share the rows and split the keys, each with its own
@@ -814,19 +886,22 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
 // 32 sequences, one token each over 4096 + 16 keys of 8 heads of 128 in bf16 (539 MB) take 99 us, 5.4 TB/s
 // (a large copy: 5.0).  One sequence over 1024 + 4 keys of 4 heads, split over 36 workgroups: 7.3 us + 4.1
 // for the join, all of it latency.
-template <typename T, int DP>
-__global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
+template <typename T, int DP> struct Few {
   typedef Img<T, DP> I;
-  constexpr int KT = 32, IB = KT * I::PITCH;
-  constexpr int STG = IB <= 8192 ? 2 : 1;   // stages of K and V per wave (wide fp32: one fits)
-  constexpr int RING = STG * 2 * IB;
-  constexpr int OUT = 32 * (DP + 4) * 4;
-  constexpr int PER = RING > OUT ? RING : OUT;
-  __shared__ __attribute__((aligned(16))) char smem[4 * PER];
-  __shared__ float sm_m[4][32], sm_l[4][32];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int L = xcd_remap(blockIdx.x, a.tiles * a.B * a.Hk * a.splits);
-  if (L < 0) return;
+  static constexpr int KT = 32, IB = KT * I::PITCH;
+  static constexpr int STG = IB <= 8192 ? 2 : 1;   // stages of K and V per wave (wide fp32: one fits)
+  static constexpr int RING = STG * 2 * IB;
+  static constexpr int OUT = 32 * (DP + 4) * 4;
+  static constexpr int PER = RING > OUT ? RING : OUT;
+};
+// all tiles, their results written; true: some are not finite.  lse: of row lane & 31 over these keys, for the second time
+template <typename T, int DP, bool strict>
+__device__ __forceinline__ bool few_pass(const WArgs& a, int L, int tid, char* smem, float (&sm_m)[4][32], float (&sm_l)[4][32],
+                                         float& lse) {
+  typedef Few<T, DP> F;
+  typedef Img<T, DP> I;
+  constexpr int KT = F::KT, IB = F::IB, STG = F::STG, PER = F::PER;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int split = L % a.splits, tile = (L / a.splits) % a.tiles, bh = L / (a.splits * a.tiles);
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const Seq seq = seq_of(a, b);
@@ -849,6 +924,7 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
   }
   I im;
   im.init(lane);
+  const int row = tid >> 3, c0 = (tid & 7) * (DP / 8), rr = r0 + row;   // of the join: 8 threads a row
   Online<T, DP> st;
   st.init();
   if (it0 < it1) {
@@ -868,7 +944,10 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
       wait_vm<0>();
     }
     const int key0 = tl[it] * KT;
-    st.template step<1, true>(im, c, c + IB, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane, 0.f);
+    if constexpr (!strict)
+      st.template step<1, true>(im, c, c + IB, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane, 0.f);
+    else
+      st.template again<1, true>(im, c, c + IB, key0, q, a.scale2, mask, lane, lse);
     if (STG == 1 && it + 4 < it1) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       dma.issue(kbase, a.kt, tl[it + 4] * KT, my.lo, my.hi, my.sl, n, 0);
@@ -885,25 +964,15 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
     for (int g = 0; g < 4; ++g)
       *(float4*)(mine + 32 * d + 8 * g + 4 * (lane >> 5)) =
           make_float4(st.o[d][4 * g], st.o[d][4 * g + 1], st.o[d][4 * g + 2], st.o[d][4 * g + 3]);
-  if (lane < 32) {
+  if (!strict && lane < 32) {
     sm_m[wave][lane] = st.m;
     sm_l[wave][lane] = lsum;
   }
   __syncthreads();
-  // 8 threads a row, DP / 8 columns each
-  const int row = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (DP / 8), rr = r0 + row;
+  float f[4], inv, out_lse;
+  if constexpr (strict) f[0] = f[1] = f[2] = f[3] = inv = 1.f;   // P came with the row's sum taken off
+  else join_waves(sm_m, sm_l, row, f, inv, out_lse);
   bool ok = true;
-  float mm = kNegInf;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm_m[w][row]);
-  float f[4], ls = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = mm == kNegInf ? (sm_l[w][row] == 0.f ? 0.f : sm_l[w][row]) : __builtin_amdgcn_exp2f(sm_m[w][row] - mm);
-    ls += f[w] * sm_l[w][row];
-  }
-  const float inv = ls > 0.f ? 1.0f / ls : (ls == 0.f ? 0.f : ls);
-  const float lse = ls == 0.f ? kNegInf : mm + __builtin_amdgcn_logf(ls);
   const int64_t orow = (int64_t)bh * a.R + rr, rows = (int64_t)a.B * a.Hk * a.R;
   const int t = dm_div(a.dmG, min(rr, a.R - 1)), g = rr - t * a.G;
   const int64_t at = (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
@@ -931,15 +1000,29 @@ __global__ void __launch_bounds__(256) wattn_few_kernel(const WArgs a) {
       }
     }
   }
-  if ((threadIdx.x & 7) == 0 && rr < a.R) {
-    if (pp) a.part[a.splits * rows * a.D + split * rows + orow] = lse;
-    else if (a.lse) a.lse[orow] = lse;
+  if (!strict && (tid & 7) == 0 && rr < a.R) {
+    if (pp) a.part[a.splits * rows * a.D + split * rows + orow] = out_lse;
+    else if (a.lse) a.lse[orow] = out_lse;
   }
-  if (__syncthreads_or(!ok)) {   // (also the barrier between these stores and the ones that replace them)
-    const int f = (int)((int64_t)tl.n * split / a.splits);
-#pragma unroll 1
-    for (int i = r0 + wave; i < min(r0 + 32, a.R); i += 4) exact_row<T>(a, seq, bh, split, i, tl, f, it1, KT);
-  }
+  if (strict || !__syncthreads_or(!ok)) return false;
+  join_waves(sm_m, sm_l, lane & 31, f, inv, lse);
+  if (lse == kNegInf) lse = -kNegInf;   // sees nothing
+  return true;
+}
+template <typename T, int DP> __device__ __forceinline__ void few_again(Again g, int L, float lse) {
+  typedef float Stat[4][32];
+  Stat& unused = *(Stat*)lds_at(g.bad);
+  few_pass<T, DP, true>(args_of(g), uniform(L), g.tid, lds_at(g.smem), unused, unused, lse);
+}
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) SIMD_WAVES(3) wattn_few_kernel(const WArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[4 * Few<T, DP>::PER];
+  __shared__ float sm_m[4][32], sm_l[4][32];
+  const int L = xcd_remap(blockIdx.x, a.tiles * a.B * a.Hk * a.splits);
+  if (L < 0) return;
+  float lse = 0.f;
+  if (few_pass<T, DP, false>(a, L, threadIdx.x, smem, sm_m, sm_l, lse))
+    few_again<T, DP>(again(smem, sm_m, threadIdx.x), L, lse);
 }
 
 // One row per 32 threads: the splits' results weighted by their sums, in split order.  At most 64
@@ -991,16 +1074,14 @@ __global__ void __launch_bounds__(256) wattn_join_kernel(const WArgs a) {
 // As the forward, with S and dP per key tile; also writes delta = dO . O for the key-major pass.
 // Measured as above: 135 us, 720 TFLOP/s over its three products; its rows' q, dO, O and O's rest are
 // 134 MB of the 250 that the whole call has to move.
-template <typename T, int DP>
-__global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wattn_dq_kernel(const WArgs a) {
+// all tiles, their results written; true: some are not finite
+template <typename T, int DP, bool strict>
+__device__ __forceinline__ bool dq_pass(const WArgs& a, const Spot& at, int tid, char* smem, int* s_bad) {
   typedef Img<T, DP> I;
   typedef typename I::frag frag;
   constexpr int KT = I::ROWS;
-  __shared__ __attribute__((aligned(16))) char smem[4 * I::BYTES];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int per = 1;
-  const Spot at = spot(a, a.tiles, a.G, per);
-  if (at.bh < 0) return;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool bad = !strict || __builtin_amdgcn_readfirstlane(s_bad[wave]);   // are these the wave's results
   const int tile = at.tile, bh = at.bh;
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const Seq seq = seq_of(a, b);
@@ -1018,16 +1099,17 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
   const int t = dm_div(a.dmG, min(r, a.R - 1)), g = min(r, a.R - 1) - t * a.G;
   const int64_t orow = (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D;
   frag q[I::NS], dof[I::NS];
-  load_frags<T, DP>((const char*)a.q + b * a.qb + t * a.qt + (hk * a.G + g) * a.qh, live, a.D, lane, q);
-  load_frags<T, DP>((const char*)a.dO + b * a.ob + t * a.ot + (hk * a.G + g) * a.oh, live, a.D, lane, dof);
+  constexpr bool ALL = sizeof(T) == 4 && DP <= 96;
+  load_frags<T, DP, ALL>((const char*)a.q + b * a.qb + t * a.qt + (hk * a.G + g) * a.qh, live, a.D, lane, q);
+  load_frags<T, DP, ALL>((const char*)a.dO + b * a.ob + t * a.ot + (hk * a.G + g) * a.oh, live, a.D, lane, dof);
   float dl = 0.f, lse = 0.f;
   {
     frag of[I::NS];
-    load_frags<T, DP>((const char*)((const T*)a.o + orow), live, a.D, lane, of);
+    load_frags<T, DP, ALL>((const char*)((const T*)a.o + orow), live, a.D, lane, of);
     constexpr int NE = sizeof(frag) / sizeof(T);
     if (sizeof(T) == 2 && a.rest) {
       frag rf[I::NS];
-      load_frags<T, DP>((const char*)(a.rest + orow), live, a.D, lane, rf);
+      load_frags<T, DP, ALL>((const char*)(a.rest + orow), live, a.D, lane, rf);
 #pragma unroll
       for (int st = 0; st < I::NS; ++st)
 #pragma unroll
@@ -1043,14 +1125,12 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
     dl += __shfl_xor(dl, 32, 64);
     const int64_t row = (int64_t)bh * a.R + r;
     if (live) lse = a.lse[row];
-    if (r < a.R && lane < 32) a.delta[row] = dl;
+    if (!strict && r < a.R && lane < 32) a.delta[row] = dl;
   }
   f16_t dq[I::ND];
-#pragma unroll
-  for (int d = 0; d < I::ND; ++d) dq[d] = zero16();
   I im;
   im.init(lane);
-  auto body = [&](const char* cur, int key0, bool masked) {
+  auto body = [&](const char* cur, int key0, bool masked) __attribute__((always_inline)) {
 #pragma unroll 1   // one 32 x 32 block's registers at a time; the other wave of the SIMD fills the gaps
     for (int kb = 0; kb < KT / 32; ++kb) {
       f16_t s = zero16(), dp = zero16();
@@ -1068,15 +1148,23 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
         asm volatile("");
         mask.hide(s, key0 + 32 * kb + 4 * (lane >> 5), 0.f);
       }
+      if constexpr (strict) {
+        strict_product<T, DP, false>(im, cur, 32 * kb, s, dq,
+                                     [&](int e) { return mask.sees(key0 + 32 * kb + 4 * (lane >> 5) + 8 * (e >> 2) + (e & 3)); });
+      } else {
 #pragma unroll
-      for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
-        const frag ds = Mma<T>::pack(s, st);
+        for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+          const frag ds = Mma<T>::pack(s, st);
 #pragma unroll
-        for (int d = 0; d < I::ND; ++d) dq[d] = Mma<T>::mma(im.col_frag(cur, 32 * kb, st, d), ds, dq[d]);
+          for (int d = 0; d < I::ND; ++d) dq[d] = Mma<T>::mma(im.col_frag(cur, 32 * kb, st, d), ds, dq[d]);
+        }
+        if constexpr (sizeof(T) == 2) interleave<8, 1, 2, 2 * I::ND>();
       }
-      if constexpr (sizeof(T) == 2) interleave<8, 1, 2, 2 * I::ND>();
     }
   };
+  const int64_t obase = ((int64_t)b * a.T * a.H + hk * a.G) * a.D;
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d) dq[d] = zero16();
   if (tl.n > 0) {
     dma.issue(kbase, a.kt, tl[0] * KT, wg.lo, wg.hi, wg.sl, lds_addr(smem), wave);
     dma.issue(vbase, a.vt, tl[0] * KT, wg.lo, wg.hi, wg.sl, lds_addr(smem) + I::BYTES, wave);
@@ -1091,23 +1179,38 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 || DP <= 64) ? 2 : 1) wat
       dma.issue(vbase, a.vt, tl[it + 1] * KT, wg.lo, wg.hi, wg.sl, nxt + I::BYTES, wave);
     }
     const int key0 = tl[it] * KT;
-    if (sees_any(my, key0, key0 + KT)) body(cur, key0, !sees_all(a, seq, my, key0, key0 + KT));
+    if (bad && sees_any(my, key0, key0 + KT)) body(cur, key0, strict || !sees_all(a, seq, my, key0, key0 + KT));
+  }
+  if constexpr (!strict) {
+    bool ok = true;
+#pragma unroll
+    for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(dq[d]);
+    const int any = __any(!ok && r < a.R);
+    if (lane == 0) s_bad[wave] = any;
   }
   lds_barrier();
-  const int64_t obase = ((int64_t)b * a.T * a.H + hk * a.G) * a.D;
-  store_rows<T, DP, false>(smem + wave * 32 * out_pitch<DP>(), dq, a.scale, a.D, lane, [&](int i) -> T* {
-    const int ti = dm_div(a.dmG, min(rw + i, a.R - 1)), gi = rw + i - ti * a.G;
-    return rw + i < a.R ? (T*)a.dq + obase + ((int64_t)ti * a.H + gi) * a.D : nullptr;
-  });
-  bool ok = true;
-#pragma unroll
-  for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(dq[d]);
-  if (__any(!ok && r < a.R)) {
-    wait_vm<0>();   // the stores that these replace
-#pragma unroll 1
-    for (int i = 0; i < 32 && rw + i < a.R; ++i)
-      exact_dq<T>(a, seq, bh, rw + i, tl, KT, __shfl(lse, i, 64), __shfl(dl, i, 64));
-  }
+  if (bad)
+    store_rows<T, DP, false>(smem + wave * 32 * out_pitch<DP>(), dq, a.scale, a.D, lane, [&](int i) -> T* {
+      const int ti = dm_div(a.dmG, min(rw + i, a.R - 1)), gi = rw + i - ti * a.G;
+      return rw + i < a.R ? (T*)a.dq + obase + ((int64_t)ti * a.H + gi) * a.D : nullptr;
+    });
+  if (strict || !(s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3])) return false;
+  wait_vm<0>();   // the stores that the next ones replace
+  lds_barrier();
+  return true;
+}
+template <typename T, int DP> __device__ __forceinline__ void dq_again(Again g, Spot at) {
+  at = Spot{uniform(at.bh), uniform(at.tile), uniform(at.sub)};
+  dq_pass<T, DP, true>(args_of(g), at, g.tid, lds_at(g.smem), (int*)lds_at(g.bad));
+}
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) SIMD_WAVES(1) wattn_dq_kernel(const WArgs a) {
+  __shared__ __attribute__((aligned(16))) char smem[4 * Img<T, DP>::BYTES];
+  __shared__ int s_bad[4];
+  int per = 1;
+  const Spot at = spot(a, a.tiles, a.G, per);
+  if (at.bh < 0) return;
+  if (dq_pass<T, DP, false>(a, at, threadIdx.x, smem, s_bad)) dq_again<T, DP>(again(smem, s_bad, threadIdx.x), at);
 }
 
 // ============================================================================ backward: dK, dV
@@ -1133,26 +1236,35 @@ __device__ __forceinline__ void key_rows(const WArgs& a, const Seq& seq, int kt,
     i1 = ((p1 + 1) * a.G + rt - 1) / rt;
   }
 }
+constexpr int kBoth = 0, kDv = 1, kDk = 2;
 template <typename T, int DP> constexpr int dkv_waves() { return sizeof(T) == 2 && DP > 64 ? 8 : 4; }
-template <typename T, int DP>
-__global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && DP > 64 ? 1 : 2) wattn_dkv_kernel(const WArgs a) {
+template <typename T, int DP> struct Dkv {
   typedef Img<T, DP> I;
-  typedef typename I::frag frag;
   // bf16 heads wider than 64: K (32 registers) stays in LDS, so that two waves fit on a SIMD beside the
   // 128 accumulators
-  constexpr bool KLDS = sizeof(T) == 2 && DP > 64;
-  constexpr int NW = dkv_waves<T, DP>();
-  constexpr int RT = I::ROWS, RB = RT * I::PITCH;
+  static constexpr bool KLDS = sizeof(T) == 2 && DP > 64;
+  static constexpr int NW = dkv_waves<T, DP>();
+  static constexpr int RT = I::ROWS, RB = RT * I::PITCH;
+  static constexpr int OUT = NW == 8 ? 4 * 64 * (DP / 2) * 4 : 0;   // one wave's dK or dV, four times
+  static constexpr int NB = 2;   // row tiles in LDS
+  static constexpr int MAIN = 2 * NB * RB + (KLDS ? 128 * I::PITCH : 0);
+  static constexpr int LDS = MAIN > OUT ? MAIN : OUT;
+  struct Stats {
+    float l[NB][RT], d[NB][RT];
+  };
+};
+// the row tiles for both sums, or strictly for one (its registers, and no more); true: some are not finite
+template <typename T, int DP, int which>
+__device__ __forceinline__ bool dkv_pass(const WArgs& a, const Spot& place, int nch, int tid, char* smem,
+                                         typename Dkv<T, DP>::Stats& stats, int* s_bad) {
+  typedef Img<T, DP> I;
+  typedef Dkv<T, DP> P;
+  typedef typename I::frag frag;
+  constexpr bool KLDS = P::KLDS, strict = which != kBoth, k_sum = which != kDv, v_sum = which != kDk;
+  constexpr int NW = P::NW, RT = P::RT, RB = P::RB, NB = P::NB;
   constexpr int NI = RT * I::CPR / 64 / NW;
-  constexpr int OUT = NW == 8 ? 4 * 64 * (DP / 2) * 4 : 0;   // one wave's dK or dV, four times
-  constexpr int NB = 2;   // row tiles in LDS
-  constexpr int MAIN = 2 * NB * RB + (KLDS ? 128 * I::PITCH : 0);
-  __shared__ __attribute__((aligned(256))) char smem[MAIN > OUT ? MAIN : OUT];
-  __shared__ __attribute__((aligned(16))) float s_l[NB][RT], s_d[NB][RT];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int nch = 0;
-  const Spot place = spot(a, a.tiles, 1, nch);
-  if (place.bh < 0) return;
+  auto &s_l = stats.l, &s_d = stats.d;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = place.bh, kt = place.tile, ch = place.sub, item = kt * a.cwin + ch;
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const Seq seq = seq_of(a, b);
@@ -1163,6 +1275,7 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
   const int c0 = i0 + (int)((int64_t)n * ch / nch), c1 = i0 + (int)((int64_t)n * (ch + 1) / nch);
 
   const int kb = wave & 3, half = wave >> 2;
+  const bool bad = !strict || __builtin_amdgcn_readfirstlane(s_bad[kb]);   // are these the wave's results
   const int kw = k0 + kb * 32, key = kw + (lane & 31);
   const bool kok = key < seq.len;
   frag kf[KLDS ? 1 : I::NS], vf[I::NS];
@@ -1215,7 +1328,7 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
   const char* qbase = (const char*)a.q + b * a.qb + hk * a.G * a.qh;
   const char* obase = (const char*)a.dO + b * a.ob + hk * a.G * a.oh;
   const int rlim = min(seq.len * a.G, a.R);   // live rows
-  auto issue = [&](int tile, unsigned img) {
+  auto issue = [&](int tile, unsigned img) __attribute__((always_inline)) {
     const int r0 = tile * RT, t0 = dm_div(a.dmG, r0);
     const i4_t rq = make_rsrc(qbase + t0 * a.qt), ro = make_rsrc(obase + t0 * a.ot);
 #pragma unroll
@@ -1228,25 +1341,23 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
   };
   const float* lbase = a.lse + (int64_t)bh * a.R;
   const float* dbase = a.delta + (int64_t)bh * a.R;
-  auto stat = [&](int tile) {   // threads [0, RT): lse, [64, 64 + RT): delta
-    const int i = threadIdx.x & 63, r = tile * RT + i;
+  auto stat = [&](int tile) __attribute__((always_inline)) {   // threads [0, RT): lse, [64, 64 + RT): delta
+    const int i = tid & 63, r = tile * RT + i;
     if (i >= RT || wave > 1) return 0.f;
     if (wave == 0) return r < rlim ? lbase[r] : __builtin_inff();   // exp2(. - inf) = 0
     return r < rlim ? dbase[r] : 0.f;
   };
-  auto put = [&](float v, int buf) {
-    const int i = threadIdx.x & 63;
+  auto put = [&](float v, int buf) __attribute__((always_inline)) {
+    const int i = tid & 63;
     if (i < RT && wave == 0) s_l[buf][i] = v;
     if (i < RT && wave == 1) s_d[buf][i] = v;
   };
   f16_t dk[I::ND], dv[I::ND];
-#pragma unroll
-  for (int d = 0; d < I::ND; ++d) dk[d] = dv[d] = zero16();
   I im;
   im.init(lane);
   // one 32 x 32 block in two phases: S and dP; then P, dS and the products with them
   f16_t s, dp;
-  auto scores = [&](const char* cur, int rb) {
+  auto scores = [&](const char* cur, int rb) __attribute__((always_inline)) {
     s = zero16();
     dp = zero16();
 #pragma unroll
@@ -1259,7 +1370,7 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
     }
     if constexpr (sizeof(T) == 2) interleave<(KLDS ? 6 : 4), 2, (KLDS ? 3 : 2), I::NS>();
   };
-  auto products = [&](const char* cur, int buf, int r0, int rb, bool masked) {
+  auto products = [&](const char* cur, int buf, int r0, int rb, bool masked) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int rr = 32 * rb + 8 * g + 4 * (lane >> 5);
@@ -1272,7 +1383,7 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
     }
     if (masked) {
       asm volatile("");
-      const int rr = r0 + 4 * (lane >> 5), ge = vlo - rr, lt = vhi - rr;
+      const int rr = r0 + 4 * (lane >> 5), ge = vlo - rr, lt = (strict ? min(vhi, rlim) : vhi) - rr;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int c = 8 * (e >> 2) + (e & 3);
@@ -1281,20 +1392,34 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
         dp[e] = see ? dp[e] : 0.f;
       }
     }
-    __builtin_amdgcn_s_setprio(1);   // 220 -> 215 us
+    if constexpr (strict) {
+      auto see = [&](int e) {
+        const int row = r0 + 4 * (lane >> 5) + 8 * (e >> 2) + (e & 3);
+        return row >= vlo && row < min(vhi, rlim);
+      };
+      if constexpr (which == kDv) strict_product<T, DP, false>(im, cur + RB, 32 * rb, s, dv, see);
+      else strict_product<T, DP, false>(im, cur, 32 * rb, dp, dk, see);
+    } else {
+      __builtin_amdgcn_s_setprio(1);   // 220 -> 215 us
 #pragma unroll
-    for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
-      const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
+      for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+        const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
 #pragma unroll
-      for (int d = 0; d < I::ND; ++d) {
-        dv[d] = Mma<T>::mma(im.col_frag(cur + RB, 32 * rb, st, d), pf, dv[d]);
-        dk[d] = Mma<T>::mma(im.col_frag(cur, 32 * rb, st, d), df, dk[d]);
+        for (int d = 0; d < I::ND; ++d) {
+          dv[d] = Mma<T>::mma(im.col_frag(cur + RB, 32 * rb, st, d), pf, dv[d]);
+          dk[d] = Mma<T>::mma(im.col_frag(cur, 32 * rb, st, d), df, dk[d]);
+        }
       }
+      if constexpr (sizeof(T) == 2) interleave<8, 1, 2, 4 * I::ND>();
+      __builtin_amdgcn_s_setprio(0);
     }
-    if constexpr (sizeof(T) == 2) interleave<8, 1, 2, 4 * I::ND>();
-    __builtin_amdgcn_s_setprio(0);
   };
 
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d) {
+    if constexpr (k_sum) dk[d] = zero16();
+    if constexpr (v_sum) dv[d] = zero16();
+  }
   if (c0 < c1) {
     put(stat(c0), 0);
     issue(c0, lds_addr(smem));
@@ -1313,21 +1438,32 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
 #pragma unroll 1   // one block's registers at a time; the other waves of the SIMD fill the gaps
     for (int rb = NW == 8 ? half : 0; rb < RT / 32; rb += NW == 8 ? 2 : 1) {
       const int r0 = it * RT + 32 * rb;
-      if (r0 < nhi && r0 + 32 > nlo) {
+      if (bad && r0 < nhi && r0 + 32 > nlo) {
         scores(cur, rb);
-        products(cur, buf, r0, rb, r0 < alo || r0 + 32 > ahi);
+        products(cur, buf, r0, rb, strict || r0 < alo || r0 + 32 > ahi);
       }
     }
     if (more) put(nx, buf ^ 1);
   }
   wait_vm<0>();   // K's DMA, where no row tile waited for it
+  auto check = [&]() __attribute__((always_inline)) {
+    if constexpr (!strict) {
+      bool ok = true;
+#pragma unroll
+      for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(dk[d]) && finite_all(dv[d]);
+      const int any = __any(!ok);
+      if (lane == 0 && half == 0) s_bad[kb] = any;
+    }
+  };
+  if constexpr (NW != 8) check();
   __syncthreads();
   if constexpr (NW == 8) {
     // the second half's sums: [register group of 4][lane] in LDS, dK then dV
     float* x = (float*)smem + kb * 64 * (DP / 2) + lane * 4;
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-      f16_t(&acc)[I::ND] = pass ? dv : dk;
+    for (int i = 0; i < 2; ++i) {
+      if (i ? !v_sum : !k_sum) continue;
+      f16_t(&acc)[I::ND] = i ? dv : dk;
       if (half == 1)
 #pragma unroll
         for (int d = 0; d < I::ND; ++d)
@@ -1346,44 +1482,47 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
             acc[d][4 * g + 2] += v.z;
             acc[d][4 * g + 3] += v.w;
           }
+      if (i == 1) check();
       __syncthreads();
     }
-    if (half == 1) return;
   }
-  bool ok = true;
-#pragma unroll
-  for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(dk[d]) && finite_all(dv[d]);
-  if (a.cwin == 1 && !(kt < a.nsink && a.cfar)) {
-    char* lds = smem + kb * 32 * out_pitch<DP>();
-    auto at = [&](void* p) {
-      return [&, p](int i) { return kw + i < a.M ? (T*)p + (((int64_t)b * a.M + kw + i) * a.Hk + hk) * a.D : nullptr; };
-    };
-    store_rows<T, DP, false>(lds, dk, a.scale, a.D, lane, at(a.dk));
-    store_rows<T, DP, false>(lds, dv, 1.f, a.D, lane, at(a.dv));
-    if (__any(!ok)) {
-      wait_vm<0>();   // the stores that these replace
-#pragma unroll 1
-      for (int i = 0; i < 32 && kw + i < a.M; ++i) {
-        const int64_t to = (((int64_t)b * a.M + kw + i) * a.Hk + hk) * a.D;
-        exact_key<T, T>(a, seq, bh, kw + i, c0 * RT, c1 * RT, 0, 0, (T*)a.dk + to, (T*)a.dv + to);
-      }
+  if (half == 0 && bad) {   // these are the wave's results
+    if (a.cwin == 1 && !(kt < a.nsink && a.cfar)) {
+      char* lds = smem + kb * 32 * out_pitch<DP>();
+      auto at = [&](void* p) {
+        return [&, p](int i) { return kw + i < a.M ? (T*)p + (((int64_t)b * a.M + kw + i) * a.Hk + hk) * a.D : nullptr; };
+      };
+      if constexpr (k_sum) store_rows<T, DP, false>(lds, dk, a.scale, a.D, lane, at(a.dk));
+      if constexpr (v_sum) store_rows<T, DP, false>(lds, dv, 1.f, a.D, lane, at(a.dv));
+    } else if (key < a.M) {
+      const int items = a.cwin > 1 ? a.tiles * a.cwin : a.nsink;   // as in the join
+      float* p = a.part + (((int64_t)bh * items + item) * 128 + kb * 32 + (lane & 31)) * 2 * a.D;
+      if constexpr (k_sum) store_col<float, I::ND>(p, dk, a.scale, a.D, lane);
+      if constexpr (v_sum) store_col<float, I::ND>(p + a.D, dv, 1.f, a.D, lane);
     }
-    return;
   }
-  if (key < a.M) {
-    const int items = a.cwin > 1 ? a.tiles * a.cwin : a.nsink;   // as in the join
-    float* p = a.part + (((int64_t)bh * items + item) * 128 + kb * 32 + (lane & 31)) * 2 * a.D;
-    store_col<float, I::ND>(p, dk, a.scale, a.D, lane);
-    store_col<float, I::ND>(p + a.D, dv, 1.f, a.D, lane);
-  }
-  if (__any(!ok)) {
-    wait_vm<0>();
-    const int items = a.cwin > 1 ? a.tiles * a.cwin : a.nsink;
-#pragma unroll 1
-    for (int i = 0; i < 32 && kw + i < a.M; ++i) {
-      float* p = a.part + (((int64_t)bh * items + item) * 128 + kb * 32 + i) * 2 * a.D;
-      exact_key<T, float>(a, seq, bh, kw + i, c0 * RT, c1 * RT, 0, 0, p, p + a.D);
-    }
+  if (!(s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3])) return false;
+  wait_vm<0>();   // the stores that the next ones replace
+  lds_barrier();
+  return true;
+}
+template <typename T, int DP, int which>
+__device__ __forceinline__ void dkv_again(Again g, Spot place, int nch, unsigned stats) {
+  place = Spot{uniform(place.bh), uniform(place.tile), uniform(place.sub)};
+  dkv_pass<T, DP, which>(args_of(g), place, uniform(nch), g.tid, lds_at(g.smem),
+                         *(typename Dkv<T, DP>::Stats*)lds_at(stats), (int*)lds_at(g.bad));
+}
+template <typename T, int DP>
+__global__ void __launch_bounds__((64 * dkv_waves<T, DP>())) SIMD_WAVES(2) wattn_dkv_kernel(const WArgs a) {
+  __shared__ __attribute__((aligned(256))) char smem[Dkv<T, DP>::LDS];
+  __shared__ __attribute__((aligned(16))) typename Dkv<T, DP>::Stats stats;
+  __shared__ int s_bad[4];
+  int nch = 0;
+  const Spot place = spot(a, a.tiles, 1, nch);
+  if (place.bh < 0) return;
+  if (dkv_pass<T, DP, kBoth>(a, place, nch, threadIdx.x, smem, stats, s_bad)) {
+    dkv_again<T, DP, kDv>(again(smem, s_bad, threadIdx.x), place, nch, lds_addr(&stats));
+    dkv_again<T, DP, kDk>(again(smem, s_bad, threadIdx.x), place, nch, lds_addr(&stats));
   }
 }
 
@@ -1391,19 +1530,16 @@ __global__ void __launch_bounds__((64 * dkv_waves<T, DP>()), sizeof(T) == 4 && D
 // of 32 sink keys (a.far32 of them) and one of cfar chunks of the rows; each wave runs through its own
 // row blocks with its own LDS ring, without barriers; the waves' sums are added at the end into part.
 // Measured as above (28 000 rows, 4 sinks): 18 us; as chunks of the key-major kernel the rows cost 40.
-template <typename T, int DP>
-__global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
+// all row blocks, their sums written; true: some are not finite
+template <typename T, int DP, bool strict>
+__device__ __forceinline__ bool far_pass(const WArgs& a, int L, int tid, char* smem, float (&s_st)[4][64]) {
   typedef Img<T, DP> I;
   typedef typename I::frag frag;
   constexpr int RB = 32 * I::PITCH, STG = RB <= 8192 ? 2 : 1, RING = STG * 2 * RB;
   constexpr int NI = RB / 1024;
   static_assert(RING >= 64 * DP * 4, "the sums fit a wave's ring");
   constexpr int RT = I::ROWS;   // as wattn_dkv_kernel
-  __shared__ __attribute__((aligned(256))) char smem[4 * RING];
-  __shared__ __attribute__((aligned(16))) float s_st[4][64];   // lse, delta of the block
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int L = xcd_remap(blockIdx.x, a.far32 * a.cfar * a.B * a.Hk);
-  if (L < 0) return;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ch = L % a.cfar, sb = L / a.cfar % a.far32, bh = L / (a.cfar * a.far32);
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
   const Seq seq = seq_of(a, b);
@@ -1427,9 +1563,9 @@ __global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
   const char* qbase = (const char*)a.q + b * a.qb + hk * a.G * a.qh;
   const char* obase = (const char*)a.dO + b * a.ob + hk * a.G * a.oh;
   char* ring = smem + wave * RING;
-  auto row_of = [&](int i) { return (i < nlo ? i : hi0 + i - nlo) * 32; };
+  auto row_of = [&](int i) __attribute__((always_inline)) { return (i < nlo ? i : hi0 + i - nlo) * 32; };
   float st_v = 0.f;   // lanes [0, 32): lse of the block in flight, [32, 64): delta
-  auto issue = [&](int i, unsigned img) {
+  auto issue = [&](int i, unsigned img) __attribute__((always_inline)) {
     const int r0 = row_of(i), t0 = dm_div(a.dmG, r0);
     const int rs = r0 + (lane & 31);
     st_v = lane < 32 ? __builtin_inff() : 0.f;   // exp2(. - inf) = 0
@@ -1445,10 +1581,11 @@ __global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
     }
   };
   f16_t dk[I::ND], dv[I::ND];
-#pragma unroll
-  for (int d = 0; d < I::ND; ++d) dk[d] = dv[d] = zero16();
   I im;
   im.init(lane);
+  float* out = a.part + far_at(a) + ((int64_t)bh * a.far32 * a.cfar + sb * a.cfar + ch) * 32 * 2 * a.D;
+#pragma unroll
+  for (int d = 0; d < I::ND; ++d) dk[d] = dv[d] = zero16();
   if (c0 < c1) issue(c0, lds_addr(ring));
   int cur = 0;
   for (int i = c0; i < c1; i += 4, cur = (cur + 1) % STG) {
@@ -1473,13 +1610,25 @@ __global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
         s[4 * g + e] = kok ? p : 0.f;
       }
     }
+    if constexpr (strict) {
+      const int left = rlim - row_of(i) - 4 * (lane >> 5);
+      auto see = [&](int e) { return kok && 8 * (e >> 2) + (e & 3) < left; };
 #pragma unroll
-    for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
-      const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
+      for (int e = 0; e < 16; ++e) {
+        s[e] = see(e) ? s[e] : 0.f;
+        dp[e] = see(e) ? dp[e] : 0.f;
+      }
+      strict_product<T, DP, false>(im, q + RB, 0, s, dv, see);
+      strict_product<T, DP, false>(im, q, 0, dp, dk, see);
+    } else {
 #pragma unroll
-      for (int d = 0; d < I::ND; ++d) {
-        dv[d] = Mma<T>::mma(im.col_frag(q + RB, 0, st, d), pf, dv[d]);
-        dk[d] = Mma<T>::mma(im.col_frag(q, 0, st, d), df, dk[d]);
+      for (int st = 0; st < 32 / Mma<T>::KS; ++st) {
+        const frag pf = Mma<T>::pack(s, st), df = Mma<T>::pack(dp, st);
+#pragma unroll
+        for (int d = 0; d < I::ND; ++d) {
+          dv[d] = Mma<T>::mma(im.col_frag(q + RB, 0, st, d), pf, dv[d]);
+          dk[d] = Mma<T>::mma(im.col_frag(q, 0, st, d), df, dk[d]);
+        }
       }
     }
     if (STG == 1 && i + 4 < c1) {
@@ -1498,8 +1647,7 @@ __global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
     }
   __syncthreads();
   bool ok = true;
-  float* out = a.part + far_at(a) + ((int64_t)bh * a.far32 * a.cfar + sb * a.cfar + ch) * 32 * 2 * a.D;
-  for (int e = threadIdx.x; e < 2 * I::ND * 4 * 64; e += 256) {
+  for (int e = tid; e < 2 * I::ND * 4 * 64; e += 256) {
     const int ln = e & 63, grp = e >> 6, which = grp / (I::ND * 4), c = grp % (I::ND * 4) * 8 + 4 * (ln >> 5);
     float4 v = *(const float4*)((const float*)smem + e * 4);
 #pragma unroll
@@ -1512,18 +1660,23 @@ __global__ void __launch_bounds__(256, 1) wattn_far_kernel(const WArgs a) {
     }
     const float f = which ? 1.f : a.scale;
     const float t = v.x * 0.f + v.y * 0.f + v.z * 0.f + v.w * 0.f;   // NaN where one is not finite
-    ok = ok && t == 0.f;
+    ok = ok && (t == 0.f || kw + (ln & 31) >= a.sinks);              // (the join reads the sinks' alone)
     if (c < a.D) *(float4*)(out + (ln & 31) * 2 * a.D + which * a.D + c) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
   }
-  if (__syncthreads_or(!ok)) {
-    const int b0 = (int)((int64_t)nb * ch / a.cfar), l1 = min(c1, nlo), h0 = hi0 + max(b0 - nlo, 0), h1 = hi0 + c1 - nlo;
-#pragma unroll 1
-    for (int i = wave; i < 32; i += 4) {
-      float* p = out + i * 2 * a.D;
-      if (kw + i < a.sinks)   // the join reads these, padding too (zeros)
-        exact_key<T, float>(a, seq, bh, kw + i, b0 * 32, l1 * 32, h0 * 32, h1 * 32, p, p + a.D);
-    }
-  }
+  return !strict && __syncthreads_or(!ok);
+}
+template <typename T, int DP> __device__ __forceinline__ void far_again(Again g, int L) {
+  typedef float Stat[4][64];
+  far_pass<T, DP, true>(args_of(g), uniform(L), g.tid, lds_at(g.smem), *(Stat*)lds_at(g.bad));
+}
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) SIMD_WAVES(4) wattn_far_kernel(const WArgs a) {
+  constexpr int RB = 32 * Img<T, DP>::PITCH, RING = (RB <= 8192 ? 2 : 1) * 2 * RB;
+  __shared__ __attribute__((aligned(256))) char smem[4 * RING];
+  __shared__ __attribute__((aligned(16))) float s_st[4][64];   // lse, delta of the block
+  const int L = xcd_remap(blockIdx.x, a.far32 * a.cfar * a.B * a.Hk);
+  if (L < 0) return;
+  if (far_pass<T, DP, false>(a, L, threadIdx.x, smem, s_st)) far_again<T, DP>(again(smem, s_st, threadIdx.x), L);
 }
 
 // dK and dV of the key tiles in parts: the window's chunks, then the far rows' (sinks only), in order.

@@ -979,3 +979,98 @@ def test_attention_infinite_far_gradient(N, D, window, sinks, ty):
     (dv,) = torch.autograd.grad(tk().window_attention(q, k, v, window, sinks, causal=False), v, do)
     assert torch.isposinf(dv[0, :sinks, 0, 5]).all()
     assert torch.isfinite(dv[0, :sinks, 0, :5]).all() and torch.isfinite(dv[0, :sinks, 0, 6:]).all()
+
+
+def kinds(x):
+    return torch.isnan(x).int() + 2 * torch.isposinf(x).int() + 4 * torch.isneginf(x).int()
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("N,H,Hk,D,window,sinks,causal", [(130, 2, 1, 32, 40, 3, True), (40, 2, 2, 64, 9, 0, False),
+                                                          (300, 1, 1, 96, 30, 100, False), (900, 2, 1, 40, 60, 2, True)])
+def test_attention_infinite_values(N, H, Hk, D, window, sinks, causal, ty):
+    """Infinities of both signs and NaN in single places of v and dO: o and dV are infinite, NaN and finite where the
+    sums over the visible pairs are."""
+    g = gen(N + D)
+    q, k, v, do = (rand(g, 1, N, h, D, type=ty) for h in (H, Hk, Hk, H))
+    mask, scale = visible(N, N, N, 0, window, sinks, causal), 1 / math.sqrt(D)
+    want, bound = attn_ref(q[0], k[0], v[0], do[0], mask, scale, ty)
+    bad = torch.tensor([math.inf, -math.inf, math.nan], device=DEV)
+
+    def spoil(x):
+        x = x.clone()
+        for i in range(12):
+            x[0, (i * 37 + 1) % N, i % x.shape[2], (i * 5) % D] = bad[i % 3]
+        return x
+
+    vs, dos = spoil(v), spoil(do)
+    leaves = [t.requires_grad_() for t in (q, k, vs)]
+    o = tk().window_attention(*leaves, window, sinks, causal=causal)
+    dv = torch.autograd.grad(tk().window_attention(q, k, v.requires_grad_(), window, sinks, causal=causal), v, dos)[0]
+    # sign of each visible pair's term (every P is above 0), 3 for NaN: what a sum of them is
+    for got, src, see, fine, eps, heads in ((o, vs, mask.int(), want[0], bound[0], True), (dv, dos, mask.int().T, want[3], bound[3], False)):
+        x = src[0].detach()
+        if heads:
+            x = x.repeat_interleave(H // Hk, 1)
+        n = [torch.einsum("ab,bhd->ahd", see.double(), c.double()) for c in (torch.isnan(x), torch.isposinf(x), torch.isneginf(x))]
+        if not heads:
+            n = [c.view(N, Hk, H // Hk, D).sum(2) for c in n]
+        nan = (n[0] > 0) | ((n[1] > 0) & (n[2] > 0))
+        kind = nan.int() + 2 * ((n[1] > 0) & ~nan).int() + 4 * ((n[2] > 0) & ~nan).int()
+        assert torch.equal(kinds(got[0].detach()), kind)
+        free = kind == 0
+        assert free.any() and not free.all()
+        within(got[0][free], fine[free], eps[free], "finite ones")
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("T,cap", [(1, 4096), (4, 300), (100, 2000)])
+def test_attention_cached_infinite_values(T, cap, ty):
+    """The same over a cache, the keys split or not: which columns are infinite is the sum over visible pairs."""
+    g, H, Hk, D, window = gen(T + cap), 4, 2, 64, cap - 100
+    q, k, v = rand(g, 1, T, H, D, type=ty), rand(g, 1, cap, Hk, D, type=ty), rand(g, 1, cap, Hk, D, type=ty)
+    n = torch.tensor([cap - 5], dtype=torch.int32, device=DEV)
+    mask = visible(T, cap, cap - 5, cap - 5 - T, window, 3, True)
+    want, bound = attn_ref(q[0], k[0], v[0], None, mask, 1 / math.sqrt(D), ty)
+    w = v.clone()
+    w[0, 1, 0, 3], w[0, cap // 2, 0, 3], w[0, cap - 7, 0, 5], w[0, cap - 6 - T // 2, 1, 7], w[0, cap - 3] = math.inf, -math.inf, -math.inf, math.nan, math.nan
+    o = tk().window_attention_cached(q, k, w, n, window, 3)
+    see = mask.double()
+    x = w[0].repeat_interleave(H // Hk, 1)
+    c = [torch.einsum("ab,bhd->ahd", see, torch.where(mask.any(0)[:, None, None], y, False).double()) > 0
+         for y in (torch.isnan(x), torch.isposinf(x), torch.isneginf(x))]
+    nan = c[0] | (c[1] & c[2])
+    kind = nan.int() + 2 * (c[1] & ~nan).int() + 4 * (c[2] & ~nan).int()
+    assert torch.equal(kinds(o[0]), kind)
+    within(o[0][kind == 0], want[0][kind == 0], bound[0][kind == 0], "finite ones")
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+def test_attention_of_values_that_are_not_finite_takes_no_longer_way(ty):
+    """Sums that are not finite are formed again with matrix products: a second pass of four products for one and their
+    operands' classes, 10 times the first's at most, and 25 here for short times.  (One pair after the other: over 100.)"""
+    g, N, H, Hk, D = gen(103), 4096, 8, 2, 128
+    t = [rand(g, 1, N, h, D, type=ty) for h in (H, Hk, Hk, H)]
+
+    def times(which=None, where=slice(None), value=0.0):
+        x = [y.clone() for y in t]
+        if which is not None:
+            x[which][where] = value
+        leaves, best = [y.requires_grad_() for y in x[:3]], [math.inf, math.inf]
+        for _ in range(4):
+            e = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+            e[0].record()
+            o = tk().window_attention(*leaves, 512, 4)
+            e[1].record()
+            torch.autograd.grad(o, leaves, x[3])
+            e[2].record()
+            torch.cuda.synchronize()
+            best = [min(best[0], e[0].elapsed_time(e[1])), min(best[1], e[1].elapsed_time(e[2]))]
+        return best
+
+    clean = times()
+    for case in ((0, slice(None), math.nan), (1, slice(None), math.inf), (2, slice(None), math.nan), (2, slice(None), math.inf),
+                 (3, slice(None), math.nan), (3, slice(None), -math.inf), (2, (0, 0), math.nan), (2, (0, 0, 0, 5), math.inf),
+                 (3, (0, 2000), math.inf), (1, (0, 1), math.inf), (0, (0, 2000), math.nan)):
+        spoilt = times(*case)
+        assert spoilt[0] < 25 * clean[0] and spoilt[1] < 25 * clean[1], (case, spoilt, clean)
