@@ -51,6 +51,7 @@ typedef __attribute__((address_space(3))) s4_t lds_s4;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
+constexpr float kNaN = __builtin_nanf("");
 // The running maximum moves only when a row outgrows it by 2^kGrow (at 8192 tokens, window 1024: 105 us
 // against 111).  A row's largest P is then no longer 1 and rounds to bf16 like the others.  Over many keys
 // that averages out; with few it does not (2 sinks and a window of 3, width 8: dK's error 0.0031 instead of
@@ -834,6 +835,8 @@ __device__ __forceinline__ bool fwd_pass(const WArgs& a, const Spot& at, int tid
   if constexpr (!strict) {
     lsum = st.l + __shfl_xor(st.l, 32, 64);
     lse = st.m;
+    // a live row sees its own position's key at least: a sum of 0 has only scores of -inf in it
+    if (a.splits == 1 && lsum == 0.f && mask.lo != 0x7fffffff) lsum = kNaN;
     bool ok = true;
 #pragma unroll
     for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(st.o[d]);
@@ -972,6 +975,8 @@ __device__ __forceinline__ bool few_pass(const WArgs& a, int L, int tid, char* s
   float f[4], inv, out_lse;
   if constexpr (strict) f[0] = f[1] = f[2] = f[3] = inv = 1.f;   // P came with the row's sum taken off
   else join_waves(sm_m, sm_l, row, f, inv, out_lse);
+  int p;
+  if (!strict && a.splits == 1 && out_lse == kNegInf && alive(a, seq, rr, p)) inv = out_lse = kNaN;   // scores of -inf alone
   bool ok = true;
   const int64_t orow = (int64_t)bh * a.R + rr, rows = (int64_t)a.B * a.Hk * a.R;
   const int t = dm_div(a.dmG, min(rr, a.R - 1)), g = rr - t * a.G;
@@ -1006,7 +1011,7 @@ __device__ __forceinline__ bool few_pass(const WArgs& a, int L, int tid, char* s
   }
   if (strict || !__syncthreads_or(!ok)) return false;
   join_waves(sm_m, sm_l, lane & 31, f, inv, lse);
-  if (lse == kNegInf) lse = -kNegInf;   // sees nothing
+  if (lse == kNegInf) lse = a.splits == 1 && mask.lo != 0x7fffffff ? kNaN : -kNegInf;   // or: sees nothing
   return true;
 }
 template <typename T, int DP> __device__ __forceinline__ void few_again(Again g, int L, float lse) {
@@ -1059,9 +1064,11 @@ __global__ void __launch_bounds__(256) wattn_join_kernel(const WArgs a) {
       s[3] += f * x[k].w;
     }
   }
-  const float inv = ls == 0.f ? 0.f : 1.0f / ls;
   const int bh = (int)(row / a.R), r = (int)(row - (int64_t)bh * a.R);
   const int b = bh / a.Hk, hk = bh - b * a.Hk, t = dm_div(a.dmG, r), g = r - t * a.G;
+  int pos;
+  if (ls == 0.f && alive(a, seq_of(a, b), r, pos)) ls = kNaN;   // sees keys, with scores of -inf alone
+  const float inv = ls == 0.f ? 0.f : 1.0f / ls;
   if (c < a.D) {
     const int64_t at = (((int64_t)b * a.T + t) * a.H + hk * a.G + g) * a.D + c;
     store4<T>((T*)a.o + at, s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv);

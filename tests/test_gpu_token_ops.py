@@ -1074,3 +1074,36 @@ def test_attention_of_values_that_are_not_finite_takes_no_longer_way(ty):
                  (3, (0, 2000), math.inf), (1, (0, 1), math.inf), (0, (0, 2000), math.nan)):
         spoilt = times(*case)
         assert spoilt[0] < 25 * clean[0] and spoilt[1] < 25 * clean[1], (case, spoilt, clean)
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+def test_attention_scores_of_minus_infinity(ty):
+    """A softmax over nothing but -inf is NaN; over -inf and others it is the others'.  Padding keeps its zeros."""
+    g, D = gen(107), 32
+    # training: row 6 sees keys 5 and 6 alone, whose scores are -inf, row 5 sees 4 as well, row 7 itself
+    for N in (40, 300):
+        q, k, v, do = (rand(g, 2, N, 1, D, type=ty) for _ in range(4))
+        q[..., 0] = 1.0
+        k[:, 5:7, :, 0] = -math.inf
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        n = torch.tensor([N, 6], dtype=torch.int32, device=DEV)
+        o = tk().window_attention(*leaves, 2, lengths=n)
+        dq, dk, dv = torch.autograd.grad(o, leaves, do)
+        hit = torch.zeros(2, N, dtype=torch.bool, device=DEV)
+        hit[0, 6] = True
+        assert torch.isnan(o[hit]).all() and torch.isfinite(o[~hit]).all()
+        assert torch.isnan(dq[hit]).all()
+        within(o[0, 5], v[0, 4].double(), 4 * UT[ty] * v[0, 4].double().abs(), "row 5")
+        within(o[0, 7], v[0, 7].double(), 4 * UT[ty] * v[0, 7].double().abs(), "row 7")
+        assert torch.equal(o[1, 6:], torch.zeros_like(o[1, 6:]))
+    # a cache, whole and split, one of two sequences with nothing but -inf; the first token lies before its start
+    for T, cap in ((1, 30), (1, 4096), (100, 4096)):
+        q, k, v = rand(g, 2, T, 2, D, type=ty), rand(g, 2, cap, 2, D, type=ty), rand(g, 2, cap, 2, D, type=ty)
+        q[..., 0] = 1.0
+        k[0, ..., 0] = -math.inf
+        n = torch.tensor([cap, cap - 3], dtype=torch.int32, device=DEV)
+        o = tk().window_attention_cached(q, k, v, n, cap)
+        assert torch.isnan(o[0]).all() and torch.isfinite(o[1]).all()
+        n = torch.tensor([0, T - 1], dtype=torch.int32, device=DEV)
+        o = tk().window_attention_cached(q, k, v, n, cap)
+        assert torch.equal(o[0], torch.zeros_like(o[0])) and torch.equal(o[1, 0], torch.zeros_like(o[1, 0]))
