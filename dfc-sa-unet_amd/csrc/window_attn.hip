@@ -661,6 +661,9 @@ template <typename T, int DP> struct Online {
       mask.hide(s, k0, kNegInf);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale2, -lse));
+      if constexpr (!FINE)   // lse is of the P that were multiplied then: the sum of these is nearly 1
+#pragma unroll
+        for (int st = 0; st < 32 / Mma<T>::KS; ++st) l = Mma<T>::add(Mma<T>::pack(s, st), l);
       strict_product<T, DP, FINE>(im, vimg, 32 * b, s, o, [&](int e) { return mask.sees(k0 + 8 * (e >> 2) + (e & 3)); });
     }
   }
@@ -744,10 +747,9 @@ __device__ __forceinline__ void store_rows(char* lds, const f16_t (&o)[DP / 32],
 // The results of a wave's 32 rows from rw over (part of) their keys: straight to o and lse, or to the
 // split's partial.  lds: 32 * out_pitch bytes of the wave's own.
 template <typename T, int DP>
-__device__ __forceinline__ void finish_rows(const WArgs& a, int bh, int split, int rw, const f16_t (&o)[DP / 32], float m,
-                                            float lsum, char* lds, int lane) {
+__device__ __forceinline__ void finish_rows(const WArgs& a, int bh, int split, int rw, const f16_t (&o)[DP / 32], float lsum,
+                                            float lse, char* lds, int lane) {
   const float inv = lsum > 0.f ? 1.0f / lsum : (lsum == 0.f ? 0.f : lsum);   // NaN sums stay NaN
-  const float lse = lsum == 0.f ? kNegInf : m + __builtin_amdgcn_logf(lsum);
   const int64_t row0 = (int64_t)bh * a.R, rows = (int64_t)a.B * a.Hk * a.R;
   const int r = rw + (lane & 31);
   if (a.splits == 1) {
@@ -781,9 +783,9 @@ __device__ __forceinline__ void finish_rows(const WArgs& a, int bh, int split, i
 // Measured at 8192 tokens, 16 / 4 heads of 128, window 1024: 104 us, 620 TFLOP/s of the 1145 that a large
 // library product reaches here; 25 us of it are the reads of q and the writes of o, its rest and lse, the
 // matrix unit is busy 30 % of the time, the vector unit (exponentials, maxima, sums) 38 % (counters, 2.4 GHz).
-// all tiles, their results written; true: some are not finite.  lse, lsum: of the lane's row, formed by the first pass
+// all tiles, their results written; true: some are not finite.  lse: of the lane's row, formed by the first pass
 template <typename T, int DP, bool strict>
-__device__ __forceinline__ bool fwd_pass(const WArgs& a, const Spot& at, int tid, char* smem, int* s_bad, float& lse, float& lsum) {
+__device__ __forceinline__ bool fwd_pass(const WArgs& a, const Spot& at, int tid, char* smem, int* s_bad, float& lse) {
   typedef Img<T, DP> I;
   constexpr int KT = I::ROWS;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -830,13 +832,14 @@ __device__ __forceinline__ bool fwd_pass(const WArgs& a, const Spot& at, int tid
       st.template step<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane,
                                 tl.n <= kFewTiles ? 0.f : kGrow);
     else if (bad)
-      st.template again<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, mask, lane, lse);
+      st.template again<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, mask, lane,
+                                   lse == kNegInf ? -kNegInf : lse);
   }
+  float lsum = st.l + __shfl_xor(st.l, 32, 64);
   if constexpr (!strict) {
-    lsum = st.l + __shfl_xor(st.l, 32, 64);
-    lse = st.m;
     // a live row sees its own position's key at least: a sum of 0 has only scores of -inf in it
     if (a.splits == 1 && lsum == 0.f && mask.lo != 0x7fffffff) lsum = kNaN;
+    lse = lsum == 0.f ? kNegInf : st.m + __builtin_amdgcn_logf(lsum);
     bool ok = true;
 #pragma unroll
     for (int d = 0; d < I::ND; ++d) ok = ok && finite_all(st.o[d]);
@@ -844,18 +847,16 @@ __device__ __forceinline__ bool fwd_pass(const WArgs& a, const Spot& at, int tid
     if (lane == 0) s_bad[wave] = bad;
   }
   lds_barrier();   // the tiles are read, the waves' results known
-  if (!strict || bad) finish_rows<T, DP>(a, bh, split, rw, st.o, lse, lsum, smem + wave * 32 * out_pitch<DP>(), lane);
+  if (!strict || bad) finish_rows<T, DP>(a, bh, split, rw, st.o, lsum, lse, smem + wave * 32 * out_pitch<DP>(), lane);
   if (strict || !(s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3])) return false;
   wait_vm<0>();   // the stores that the next ones replace
   lds_barrier();
-  lse = lsum == 0.f ? -kNegInf : lse + __builtin_amdgcn_logf(lsum);
-  lsum = lsum == 0.f ? 0.f : 1.f;
   return true;
 }
 template <typename T, int DP>
-__device__ __forceinline__ void fwd_again(Again g, Spot at, float lse, float lsum) {
+__device__ __forceinline__ void fwd_again(Again g, Spot at, float lse) {
   at = Spot{uniform(at.bh), uniform(at.tile), uniform(at.sub)};
-  fwd_pass<T, DP, true>(args_of(g), at, g.tid, lds_at(g.smem), (int*)lds_at(g.bad), lse, lsum);
+  fwd_pass<T, DP, true>(args_of(g), at, g.tid, lds_at(g.smem), (int*)lds_at(g.bad), lse);
 }
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) SIMD_WAVES(0) wattn_fwd_kernel(const WArgs a) {
@@ -864,9 +865,8 @@ __global__ void __launch_bounds__(256) SIMD_WAVES(0) wattn_fwd_kernel(const WArg
   int per = a.splits;
   const Spot at = spot(a, a.tiles, a.G, per);
   if (at.bh < 0) return;
-  float lse = 0.f, lsum = 0.f;
-  if (fwd_pass<T, DP, false>(a, at, threadIdx.x, smem, s_bad, lse, lsum))
-    fwd_again<T, DP>(again(smem, s_bad, threadIdx.x), at, lse, lsum);
+  float lse = 0.f;
+  if (fwd_pass<T, DP, false>(a, at, threadIdx.x, smem, s_bad, lse)) fwd_again<T, DP>(again(smem, s_bad, threadIdx.x), at, lse);
 }
 
 // weights and sum of one row's results of four waves

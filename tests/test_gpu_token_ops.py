@@ -1107,3 +1107,82 @@ def test_attention_scores_of_minus_infinity(ty):
         n = torch.tensor([0, T - 1], dtype=torch.int32, device=DEV)
         o = tk().window_attention_cached(q, k, v, n, cap)
         assert torch.equal(o[0], torch.zeros_like(o[0])) and torch.equal(o[1, 0], torch.zeros_like(o[1, 0]))
+
+
+# Where bf16 is rounded: P and dS before the second products, and the results.  Independent roundings add in squares, so
+# beside the results' own rounding (1) the first add up to 1 (less over few keys, where the largest P is 1 and the sum is
+# of the rounded ones): sqrt(2) of it for dV and O, and for dQ and dK with delta's part of P's rounding 1.46 to 1.53 with
+# windows of 2 to 64 keys when the formulas are put in 64 bits with those roundings alone; 1.73 and more if O's rounding
+# reaches delta, 2.0 and more with its rest subtracted (windows of 2 and 3: 1.93 to 2.27 and 2.8 to 3.7).
+def rel(got, want):
+    """The 2-norm of the error, in that of rounding the exact result to bf16."""
+    return float((got.double() - want).norm() / (want.to(BF).double() - want).norm())
+
+
+@pytest.mark.parametrize("N,H,Hk,D,window,causal", [
+    (60, 2, 2, 64, 2, True), (15, 16, 4, 128, 2, True), (62, 3, 3, 40, 3, False),   # up to 64 rows a key head
+    (300, 8, 8, 64, 2, True), (300, 8, 2, 128, 3, True), (1100, 4, 4, 96, 2, True), (500, 6, 6, 32, 2, False), (2500, 4, 2, 128, 3, True)])
+def test_attention_error_norms(N, H, Hk, D, window, causal):
+    """Over few keys dS is a small difference: its error shows whether delta is formed from more than O's 8 bits."""
+    g = gen(N + D)
+    q, k, v, do = (rand(g, 1, N, h, D, type=BF) for h in (H, Hk, Hk, H))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = tk().window_attention(*leaves, window, causal=causal)
+    got = (o.detach(), *torch.autograd.grad(o, leaves, do))
+    want, _ = attn_ref(q[0].detach(), k[0].detach(), v[0].detach(), do[0], visible(N, N, N, 0, window, 0, causal), 1 / math.sqrt(D), BF)
+    for name, a, b, limit in zip(("o", "dq", "dk", "dv"), got, want, (1.45, 1.65, 1.65, 1.5)):
+        assert rel(a[0], b) <= limit, (name, rel(a[0], b))
+
+
+@pytest.mark.parametrize("spoilt", [False, True])
+@pytest.mark.parametrize("N,H,Hk,D,window,limit", [(60, 2, 2, 64, 2, 0.85), (15, 16, 4, 128, 3, 0.85), (300, 8, 8, 64, 2, 0.85),
+                                                   (1100, 4, 2, 96, 3, 0.85), (2000, 1, 1, 64, 2000, 1.2)])
+def test_attention_rest_of_o(N, H, Hk, D, window, limit, spoilt):
+    """o and what its rounding left: together as far off as P's rounding makes them (0.33 to 0.7 of o's own over few keys,
+    up to 1 over many), not more (alone 1.05 and more, 1.4 over many).  The kernels for few rows, for tiles of rows, the
+    keys split and joined (the last); spoilt: rows formed again beside a NaN that they do not see.  lse as well."""
+    import ctypes
+    from dfcsa._lib import LIB, WattnDesc
+    g = gen(N + D)
+    q, k, v = rand(g, 1, N, H, D, type=BF), rand(g, 1, N, Hk, D, type=BF), rand(g, 1, N, Hk, D, type=BF)
+    live, first = (N - 1, N - 12) if spoilt else (N, 0)   # the last rows are formed again beside the last key's NaN
+    want, _ = attn_ref(q[0], k[0], v[0], None, visible(N, N, N, 0, window, 0, True), 1 / math.sqrt(D), BF)
+    if spoilt:
+        v[0, -1] = math.nan
+    o, rest, lse = torch.empty_like(q), torch.empty_like(q), torch.empty(Hk * N * (H // Hk), device=DEV)
+    d = WattnDesc(dtype=1, B=1, T=N, M=N, H=H, Hk=Hk, D=D, window=window, sinks=0, causal=1, cached=0, scale=1 / math.sqrt(D),
+                  q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), o=o.data_ptr(), o_rest=rest.data_ptr(), lse=lse.data_ptr())
+    d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    n = ctypes.c_int64()
+    assert LIB.dfcsa_wattn_work_floats(ctypes.addressof(d), 0, ctypes.byref(n)) == 0
+    assert (n.value > 0) == (N == 2000)
+    work = torch.empty(max(n.value, 1), device=DEV)
+    d.work, d.work_floats = work.data_ptr(), n.value
+    assert LIB.dfcsa_wattn_fwd(ctypes.addressof(d), torch.cuda.current_stream().cuda_stream) == 0
+    both, exact = (o.double() + rest.double())[0, first:live], want[0][first:live]
+    assert rel(both, exact) <= limit, rel(both, exact)
+    assert rel(o[0, first:live], exact) <= 1.45
+    s = (torch.einsum("nhd,mhd->hnm", q[0].double(), k[0].double().repeat_interleave(H // Hk, 1)) / math.sqrt(D)).masked_fill(
+        ~visible(N, N, N, 0, window, 0, True), -math.inf)
+    got = lse.view(Hk, N, H // Hk).permute(0, 2, 1).reshape(H, N).double() * math.log(2)
+    # of the rounded P: 2^-8 at most; scores and sums in fp32, and the lse's own rounding, stay below 2^-14 here
+    assert float((got - torch.logsumexp(s, -1)).abs().max()) <= 2.0 ** -8 + 2.0 ** -14
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+@pytest.mark.parametrize("N,H,Hk,D,window,sinks,causal", [(260, 2, 2, 64, 260, 0, True), (60, 2, 1, 64, 60, 3, True), (2500, 2, 1, 64, 100, 40, True),
+                                                          (700, 1, 1, 128, 700, 0, False), (1500, 2, 2, 96, 60, 4, False)])
+def test_attention_large_scores_backward(N, H, Hk, D, window, sinks, causal, ty):
+    """Scores of +-1000: P is formed again from the log-sum of rows whose maximum moved far, in all passes of the backward."""
+    g = gen(N + 41)
+    q, k, v, do = (rand(g, 1, N, h, D, type=ty) for h in (H, Hk, Hk, H))
+    k = (k * torch.linspace(0.1, 30, N, device=DEV)[:, None, None]).to(ty)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = tk().window_attention(*leaves, window, sinks, causal=causal, scale=0.125)
+    got = (o.detach(), *torch.autograd.grad(o, leaves, do))
+    want, bound = attn_ref(*(t[0].detach() for t in leaves), do[0], visible(N, N, N, 0, window, sinks, causal), 0.125, ty)
+    # a P below fp32's smallest normal number, 2^-126, is 0: each of a sum's at most N * H terms is off by that times at
+    # most |dP - delta| < 2^8 and |q| or |k| < 2^8 (0.125 of it)
+    floor = N * H * 2.0 ** -113
+    for name, a, b, e in zip(("o", "dq", "dk", "dv"), got, want, bound):
+        within(a[0], b, e + floor, name)
