@@ -530,8 +530,9 @@ struct WindowAttention : public Function<WindowAttention> {
     const Attn p{(int)ctx->saved_data["window"].toInt(), (int)ctx->saved_data["sinks"].toInt(),
                  ctx->saved_data["causal"].toBool(), false, (float)ctx->saved_data["scale"].toDouble()};
     const On on(q);
-    const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
-                 dv = at::empty(v.sizes(), v.options()), delta = at::empty(s[4].sizes(), s[4].options());
+    const bool keys = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);   // else the key-major passes are left out
+    const Tensor dq = at::empty(q.sizes(), q.options()), dk = keys ? at::empty(k.sizes(), k.options()) : Tensor(),
+                 dv = keys ? at::empty(v.sizes(), v.options()) : Tensor(), delta = at::empty(s[4].sizes(), s[4].options());
     dfcsa_wattn_desc d = attn_desc(q, k, v, s[5], p, s[3], s[4], s[6]);
     d.dout = ptr(dout);
     set_strides(d.dout_stride, dout);

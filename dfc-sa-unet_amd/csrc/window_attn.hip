@@ -1786,7 +1786,7 @@ bool fill(const dfcsa_wattn_desc* d, WArgs& a, bool backward) {
   a.pack = a.lengths && !a.cached && a.B <= kPackSeqs;
   if (backward) {
     a.ob = d->dout_stride[0] * es; a.ot = d->dout_stride[1] * es; a.oh = d->dout_stride[2] * es;
-    if (!d->lse || !d->delta || !d->dq || !d->dk || !d->dv) return false;
+    if (!d->lse || !d->delta || !d->dq || !d->dk != !d->dv) return false;   // dk and dv: both or neither
   }
   return true;
 }
@@ -1868,7 +1868,7 @@ void plan_bwd(WArgs& a, bool f32) {
     a.cfar = (int)std::max<int64_t>(1, std::min<int64_t>({(256 + base - 1) / base, blocks / 4, 64}));
   }
 }
-int64_t bwd_work(const WArgs& a) { return far_at(a) + (int64_t)a.B * a.Hk * a.far32 * a.cfar * 32 * 2 * a.D; }
+int64_t bwd_work(const WArgs& a) { return !a.dk ? 0 : far_at(a) + (int64_t)a.B * a.Hk * a.far32 * a.cfar * 32 * 2 * a.D; }
 
 #define BY_WIDTH(KERNEL, GRID, THREADS, ARGS)                                                        \
   do {                                                                                               \
@@ -1901,6 +1901,7 @@ int run_bwd(WArgs a, hipStream_t st) {
     BY_WIDTH(wattn_dq_kernel, dim3((unsigned)grid_of(a, (int64_t)a.tiles * a.B * a.Hk)), 256, a);
   }
   DFCSA_CHECK_LAUNCH();
+  if (!a.dk) return 0;
   const int bh = a.B * a.Hk;
   BY_WIDTH(wattn_dkv_kernel, dim3((unsigned)grid_of(a, (int64_t)a.tiles * a.cwin * bh)), dkv_threads(a, sizeof(T) == 4), a);
   DFCSA_CHECK_LAUNCH();

@@ -980,7 +980,8 @@ int dfcsa_rotary(const dfcsa_rotary_desc* d, void* stream);
  * only): token t is at position length - T + t.
  * lse [B][Hk][T * H / Hk]: log2 of the rows' sums, written by fwd (may be NULL there), read by bwd;
  * delta: scratch of the same size.  o_rest (bf16, may be NULL): [B][T][H][D] bf16, what the rounding of
- * o left, written by fwd, read by bwd for delta = dO . O.  work: dfcsa_wattn_work_floats floats (0: may be NULL). */
+ * o left, written by fwd, read by bwd for delta = dO . O.  dk and dv may both be NULL (bwd then forms dq alone).
+ * work: dfcsa_wattn_work_floats floats (0: may be NULL). */
 typedef struct {
   int dtype, B, T, M, H, Hk, D, window, sinks, causal, cached;
   float scale;

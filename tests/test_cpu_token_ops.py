@@ -250,3 +250,11 @@ def test_wrapped_tensors_are_refused(i):
         torch.func.grad(lambda x, q: calls(x, q)[i]().sum(), (0, 1))(x, q)
     with pytest.raises(RuntimeError, match="dense tensors"):
         calls(Wrapped(x), Wrapped(q))[i]()
+
+
+def test_attention_backward_without_key_gradients():
+    # neither dk nor dv: no workspace, which the same call with both has
+    n = ctypes.c_int64()
+    for over, some in ((dict(), True), (dict(dk=None, dv=None), False)):
+        d = attn_desc(B=1, T=4096, M=4096, **over)
+        assert LIB.dfcsa_wattn_work_floats(ctypes.addressof(d), 1, ctypes.byref(n)) == 0 and (n.value > 0) == some

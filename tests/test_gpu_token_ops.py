@@ -1186,3 +1186,26 @@ def test_attention_large_scores_backward(N, H, Hk, D, window, sinks, causal, ty)
     floor = N * H * 2.0 ** -113
     for name, a, b, e in zip(("o", "dq", "dk", "dv"), got, want, bound):
         within(a[0], b, e + floor, name)
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+def test_attention_one_input_at_a_time(ty):
+    """Gradients of some inputs alone are those of all; without k's and v's nothing is allocated or computed for them."""
+    g, N, H, D = gen(109), 3000, 4, 64
+    t = [rand(g, 1, N, H, D, type=ty) for _ in range(4)]
+    leaves = [x.detach().clone().requires_grad_() for x in t[:3]]
+    whole = torch.autograd.grad(tk().window_attention(*leaves, 100, 3), leaves, t[3])
+    for want in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        x = [y.detach().clone().requires_grad_(i in want) for i, y in enumerate(t[:3])]
+        o = tk().window_attention(*x, 100, 3)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(o, [x[i] for i in want], t[3])
+        peak = torch.cuda.max_memory_allocated() - before
+        for i, d in zip(want, got):
+            assert torch.equal(d, whole[i]), (want, i)
+        # dQ and delta (a float for each row).  The allocator counts a cached block whole where it is less than 1 MiB too
+        # long, for each of the two; dK and dV alone would be 3 MB or more.
+        if want == (0,):
+            assert peak <= t[0].numel() * t[0].element_size() + N * H * 4 + (2 << 20)
