@@ -199,7 +199,6 @@ template <> struct Mma<bf16_t> {
   __device__ __forceinline__ static f16_t mma(const frag& a, const frag& b, const f16_t& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bh8_t, a), __builtin_bit_cast(bh8_t, b), c, 0, 0, 0);
   }
-  // accumulator registers of contraction step st (16 rows of the 32) as a fragment
   // a sum plus a fragment's elements
   __device__ __forceinline__ static float add(const frag& f, float l) {
     union { frag f; uint32_t u[4]; } x;
@@ -209,6 +208,7 @@ template <> struct Mma<bf16_t> {
       l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bh2_t, x.u[i]), (bh2_t){(__bf16)1.0f, (__bf16)1.0f}, l, false);
     return l;
   }
+  // accumulator registers of contraction step st (16 rows of the 32) as a fragment
   __device__ __forceinline__ static frag pack(const f16_t& p, int st) {
     union { uint32_t u[4]; frag f; } r;
 #pragma unroll

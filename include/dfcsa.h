@@ -973,8 +973,8 @@ int dfcsa_rotary(const dfcsa_rotary_desc* d, void* stream);
  * position p when j < length, j <= p (causal), and |p - j| < window or j < sinks; o = softmax over the
  * visible keys of scale q.k, times v; zeros where nothing is visible.
  * q, o [B][T][H][D], k, v [B][M][Hk][D] (H % Hk == 0, D % 8 == 0, D <= 128); strides in elements
- * (batch, token, head) of q, k, v, dout: non-negative multiples of 16 bytes, token stride below 8 MiB,
- * head stride times H / Hk below 512 MiB;
+ * (batch, token, head) of q, k, v, dout: non-negative multiples of 16 bytes, token stride below 8 MiB;
+ * of q and dout, whose tiles span heads, head stride times H / Hk below 512 MiB (a head of k or v may lie anywhere);
  * o, dq, dk, dv contiguous.  lengths [B] int32 on the device (NULL: M; clamped to [0, M]).
  * cached == 0: T == M, token t is at position t.  cached != 0 (causal, lengths required, forward
  * only): token t is at position length - T + t.
