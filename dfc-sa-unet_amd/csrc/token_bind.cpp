@@ -151,7 +151,7 @@ Norm norm_args(const Tensor& x, const Tensor& res, const Tensor& w, double eps) 
   if (w.scalar_type() != at::kFloat) bad_type("weight: float32 is needed, got " + name(w.scalar_type()));
   if (w.dim() != 1 || w.size(0) != C) bad_value("weight " + shape(w) + ": (" + std::to_string(C) + ",) is needed");
   if (n.ty == DFCSA_DT_F32 && n.rt != DFCSA_DT_F32) bad_type("a float32 x needs a float32 residual");
-  if (!(eps >= 0.0) || !std::isfinite(eps)) bad_value("eps: a finite value of at least 0 is needed");
+  if (!(eps >= 0.0) || !std::isfinite((float)eps)) bad_value("eps: a finite fp32 value of at least 0 is needed");
   if (x.numel() / C > 0x7fff0000) bad_value("at most 2^31 - 2^16 rows");
   n.rows = (int)(x.numel() / C);
   n.C = (int)C;

@@ -2,6 +2,8 @@
 // (training, backward, 8-bit output) and rotary positions with several axes.  All of them move each
 // byte once and compute ~10 operations per element, so HBM bandwidth bounds them; every thread loads
 // and stores 16-byte words and a row (or a token's angles) stays on chip between its two uses.
+#include <cmath>
+
 #include "common.h"
 #include "dfcsa_internal.h"
 
@@ -342,6 +344,7 @@ int launch_bwd(int rows, int C, const void* dy, const void* dr, const void* r, c
 }
 
 bool norm_shape_ok(int rows, int C) { return rows > 0 && rows <= kNormMaxRows && C >= 8 && C % 8 == 0 && C <= kNormMaxC; }
+bool eps_ok(float eps) { return eps >= 0.f && std::isfinite(eps); }
 bool types_ok(int t, int r) { return (t == DFCSA_DT_BF16 && (r == DFCSA_DT_BF16 || r == DFCSA_DT_F32)) ||
                                      (t == DFCSA_DT_F32 && r == DFCSA_DT_F32); }
 
@@ -461,7 +464,7 @@ extern "C" {
 
 int dfcsa_rms_fwd(int dtype, int rdtype, int rows, int C, const void* x, const void* res, const float* w, float eps,
                   void* y, void* r, float* rstd, void* stream) {
-  if (!norm_shape_ok(rows, C) || !types_ok(dtype, rdtype) || !x || !res || !w || !y || !r) return DFCSA_EINVAL;
+  if (!norm_shape_ok(rows, C) || !types_ok(dtype, rdtype) || !x || !res || !w || !y || !r || !eps_ok(eps)) return DFCSA_EINVAL;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DFCSA_DT_F32) return launch_fwd<float, float, false>(rows, C, x, res, w, eps, y, r, rstd, nullptr, nullptr, C, st);
   if (rdtype == DFCSA_DT_F32) return launch_fwd<bf16_t, float, false>(rows, C, x, res, w, eps, y, r, rstd, nullptr, nullptr, C, st);
@@ -470,7 +473,7 @@ int dfcsa_rms_fwd(int dtype, int rdtype, int rows, int C, const void* x, const v
 
 int dfcsa_rms_fwd_q8(int dtype, int rdtype, int rows, int C, int group, const void* x, const void* res, const float* w,
                      float eps, void* y8, float* scales, void* r, void* stream) {
-  if (!norm_shape_ok(rows, C) || !types_ok(dtype, rdtype) || !x || !res || !w || !y8 || !scales || !r) return DFCSA_EINVAL;
+  if (!norm_shape_ok(rows, C) || !types_ok(dtype, rdtype) || !x || !res || !w || !y8 || !scales || !r || !eps_ok(eps)) return DFCSA_EINVAL;
   if (group == 0) group = C;
   if (group != C && ((group != 32 && group != 64 && group != 128) || C % group)) return DFCSA_EINVAL;
   hipStream_t st = (hipStream_t)stream;

@@ -258,3 +258,9 @@ def test_attention_backward_without_key_gradients():
     for over, some in ((dict(), True), (dict(dk=None, dv=None), False)):
         d = attn_desc(B=1, T=4096, M=4096, **over)
         assert LIB.dfcsa_wattn_work_floats(ctypes.addressof(d), 1, ctypes.byref(n)) == 0 and (n.value > 0) == some
+
+
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf")])
+def test_norm_eps_refusals(eps):
+    assert LIB.dfcsa_rms_fwd(1, 0, 4, 64, P16, P16, P16, eps, P16, P16, P16, None) == EINVAL
+    assert LIB.dfcsa_rms_fwd_q8(1, 0, 4, 64, 0, P16, P16, P16, eps, P16, P16, P16, None) == EINVAL

@@ -1209,3 +1209,11 @@ def test_attention_one_input_at_a_time(ty):
         # long, for each of the two; dK and dV alone would be 3 MB or more.
         if want == (0,):
             assert peak <= t[0].numel() * t[0].element_size() + N * H * 4 + (2 << 20)
+
+
+def test_norm_eps_is_finite_in_fp32():
+    """An eps that fp32 holds as infinity would make every result 0."""
+    x, w = torch.ones(2, 16, device=DEV), torch.ones(16, device=DEV)
+    for call in (tk().rms_norm_residual, tk().rms_norm_residual_q8):
+        with pytest.raises(ValueError, match="eps"):
+            call(x, x, w, eps=1e39)
