@@ -89,6 +89,7 @@ struct WArgs {
 // there again, and not held in registers through the first pass (that spilled scalar registers in the first's loop:
 // forward 104 -> 111 us at 8192 tokens, key-major pass 162 -> 175; as a function that is called it needs a stack,
 // which costs the launch after it 0.45 us).
+//
 // The waves on a SIMD that a kernel's first pass reaches, which the second must not lower; it may spill for them.
 // P: 0 forward, 1 dQ, 2 dK / dV, 3 few rows, 4 far rows; widths 32, 64, 96, 128 in bf16, then in fp32.
 template <typename T, int DP> constexpr int simd_waves(int P) {
@@ -96,7 +97,7 @@ template <typename T, int DP> constexpr int simd_waves(int P) {
                            {2, 2, 1, 1, 1, 1, 1, 1}, {2, 2, 1, 1, 1, 1, 1, 1}};
   return w[P][(sizeof(T) == 2 ? 0 : 4) + DP / 32 - 1];
 }
-// As the largest number too: the scheduler gives up the order that interleave() asks for where that takes a kernel
+// Given as the largest number too: the scheduler gives up the order that interleave() asks for where that takes a kernel
 // from more waves to fewer (key-major pass, width 64: 28.8 -> 32.7 us).
 #define SIMD_WAVES(P) __attribute__((amdgpu_waves_per_eu(simd_waves<T, DP>(P), simd_waves<T, DP>(P))))
 struct Again {
@@ -783,7 +784,8 @@ __device__ __forceinline__ void finish_rows(const WArgs& a, int bh, int split, i
 // Measured at 8192 tokens, 16 / 4 heads of 128, window 1024: 104 us, 620 TFLOP/s of the 1145 that a large
 // library product reaches here; 25 us of it are the reads of q and the writes of o, its rest and lse, the
 // matrix unit is busy 30 % of the time, the vector unit (exponentials, maxima, sums) 38 % (counters, 2.4 GHz).
-// all tiles, their results written; true: some are not finite.  lse: of the lane's row, formed by the first pass
+//
+// A pass: all tiles, their results written; true: some are not finite.  lse: of the lane's row, formed by the first pass
 template <typename T, int DP, bool strict>
 __device__ __forceinline__ bool fwd_pass(const WArgs& a, const Spot& at, int tid, char* smem, int* s_bad, float& lse) {
   typedef Img<T, DP> I;
@@ -832,8 +834,7 @@ __device__ __forceinline__ bool fwd_pass(const WArgs& a, const Spot& at, int tid
       st.template step<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, !sees_all(a, seq, my, key0, key0 + KT), mask, lane,
                                 tl.n <= kFewTiles ? 0.f : kGrow);
     else if (bad)
-      st.template again<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, mask, lane,
-                                   lse == kNegInf ? -kNegInf : lse);
+      st.template again<KT / 32>(im, cur, cur + I::BYTES, key0, q, a.scale2, mask, lane, lse == kNegInf ? -kNegInf : lse);
   }
   float lsum = st.l + __shfl_xor(st.l, 32, 64);
   if constexpr (!strict) {
@@ -1081,7 +1082,8 @@ __global__ void __launch_bounds__(256) wattn_join_kernel(const WArgs a) {
 // As the forward, with S and dP per key tile; also writes delta = dO . O for the key-major pass.
 // Measured as above: 135 us, 720 TFLOP/s over its three products; its rows' q, dO, O and O's rest are
 // 134 MB of the 250 that the whole call has to move.
-// all tiles, their results written; true: some are not finite
+//
+// A pass: all tiles, their results written; true: some are not finite
 template <typename T, int DP, bool strict>
 __device__ __forceinline__ bool dq_pass(const WArgs& a, const Spot& at, int tid, char* smem, int* s_bad) {
   typedef Img<T, DP> I;

@@ -107,7 +107,8 @@ def window_attention(q, k, v, window, sinks=0, causal=True, scale=None, lengths=
     Token p sees token j when |p - j| < window or j < sinks, and, if causal, j <= p.  window = N (or
     more) is plain attention.  scale: of the scores, 1/sqrt(D) unless given.  lengths: int32 [B], the
     valid tokens of each sequence, the first ones (clamped to [0, N]); rows behind them are padding:
-    whatever they hold, they are not seen, their results and gradients are zeros.
+    whatever they hold, they are not seen, their results and gradients are zeros.  A NaN or infinity reaches
+    what sees it, however small its weight, and nothing else; it costs time (a call about four times as long).
     bf16 or fp32, D a multiple of 8 up to 128.  Differentiable in q, k and v.  Tensors are read in place
     where their channels are contiguous and their strides multiples of 16 bytes, else from a copy.
     The cost follows N * (window + sinks); nothing N x N is stored."""

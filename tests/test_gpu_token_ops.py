@@ -1217,3 +1217,23 @@ def test_norm_eps_is_finite_in_fp32():
     for call in (tk().rms_norm_residual, tk().rms_norm_residual_q8):
         with pytest.raises(ValueError, match="eps"):
             call(x, x, w, eps=1e39)
+
+
+@pytest.mark.parametrize("ty", [BF, F32])
+def test_one_tensor_in_several_places(ty):
+    """The same tensor as x and residual, as q and k, as k and v, as all three: its gradient is the sum of theirs."""
+    g, t = gen(113), tk()
+    x, w, dy, dr = rand(g, 5, 64, type=ty), torch.ones(64, device=DEV), rand(g, 5, 64, type=ty), rand(g, 5, 64, type=ty)
+    q, do, dk = rand(g, 1, 70, 2, 32, type=ty), rand(g, 1, 70, 2, 32, type=ty), rand(g, 1, 70, 2, 32, type=ty)
+    pos = torch.arange(70, dtype=torch.int32, device=DEV)[:, None]
+    calls = ((x, 2, lambda a, b: t.rms_norm_residual(a, b, w), (dy, dr)), (q, 2, lambda a, b: t.rotary(a, b, pos, (16,)), (do, dk)),
+             (q, 2, lambda a, b: t.window_attention(q, a, b, 9, 2), do), (q, 3, lambda a, b, c: t.window_attention(a, b, c, 9, 2), do))
+    for src, n, call, grads in calls:
+        one, apart = src.clone().requires_grad_(), [src.clone().requires_grad_() for _ in range(n)]
+        a, b = call(*[one] * n), call(*apart)
+        same = zip(a, b) if isinstance(a, tuple) else ((a, b),)
+        assert all(torch.equal(u, v) for u, v in same)
+        (got,) = torch.autograd.grad(a, one, grads)
+        parts = [p.double() for p in torch.autograd.grad(b, apart, grads)]
+        # torch adds the parts in their type: half a step of each sum
+        within(got, sum(parts), n * UT[ty] * sum(p.abs() for p in parts), "sum")
