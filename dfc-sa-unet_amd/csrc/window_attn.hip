@@ -783,7 +783,7 @@ __device__ __forceinline__ void finish_rows(const WArgs& a, int bh, int split, i
 // on a CU, two waves on a SIMD (three with 32-key tiles measured no faster: 118 against 113 us).
 // Measured at 8192 tokens, 16 / 4 heads of 128, window 1024: 104 us, 620 TFLOP/s of the 1145 that a large
 // library product reaches here; 25 us of it are the reads of q and the writes of o, its rest and lse, the
-// matrix unit is busy 30 % of the time, the vector unit (exponentials, maxima, sums) 38 % (counters, 2.4 GHz).
+// matrix unit is busy 30 % of the time, the vector unit (exponentials, maxima, sums) 36 % (counters, 2.4 GHz).
 //
 // A pass: all tiles, their results written; true: some are not finite.  lse: of the lane's row, formed by the first pass
 template <typename T, int DP, bool strict>
