@@ -479,8 +479,8 @@ __device__ __forceinline__ f16_t zero16() {
 // NaN A and for a B of 0, whose product is NaN): t > s where something adds -inf or NaN, t > -s where
 // something adds +inf or NaN.  Both are small whole numbers, exact as matrix products of -1, 0 and 1.  So
 // inputs of nothing but NaN or infinities cost up to 6 times what others do (8192 tokens, 16 / 4 heads of 128,
-// window 1024, forward and backward: 0.42 ms; a row of NaN among the sinks' values 1.2, nothing but NaN in
-// q, v or dO 1.7, 1.6 and 1.4; one row and key after the other, without matrix products, they took up to 160).
+// window 1024, forward and backward: 0.42 ms; a row of NaN among the sinks' values 1.1, nothing but NaN in
+// q, v or dO 1.6, 1.5 and 1.4; one row and key after the other, without matrix products, they took up to 160).
 __device__ __forceinline__ bool finite_all(const f16_t& v) {
   bool ok = true;
 #pragma unroll

@@ -1048,7 +1048,7 @@ def test_attention_cached_infinite_values(T, cap, ty):
 @pytest.mark.parametrize("ty", [BF, F32])
 def test_attention_of_values_that_are_not_finite_takes_no_longer_way(ty):
     """Sums that are not finite are formed again with matrix products: a second pass of four products for one and their
-    operands' classes, 10 times the first's at most, and 25 here for short times.  (One pair after the other: over 100.)"""
+    operands' classes, 10 times the first's at most, and 25 here for short times.  (One pair after the other: 34 to 63.)"""
     g, N, H, Hk, D = gen(103), 4096, 8, 2, 128
     t = [rand(g, 1, N, h, D, type=ty) for h in (H, Hk, Hk, H)]
 
